@@ -15,6 +15,9 @@ FB_OK = 0
 FB_STATUS_CAND_OVERFLOW = 1
 FB_STATUS_WAIT_TIMEOUT = 2
 FB_STATUS_INDEX_RANGE = 4
+FB_STATUS_INDEX_TWICE = 8
+FB_DTYPE_F32, FB_DTYPE_F16, FB_DTYPE_BF16 = 0, 1, 2
+FB_LOGPROBS_MAX_TOP = 64
 
 
 class FunctsB200Error(RuntimeError):
@@ -29,6 +32,16 @@ class AccessDesc(ctypes.Structure):
         ("src_mod", c_int64 * 8),
         ("src_offset", c_int64),
     ]
+
+
+class LinearAttentionArgs(ctypes.Structure):
+    _fields_ = (
+        [(n, c_int32) for n in ("dtype", "batch", "tokens", "heads", "kv_heads", "dk", "dv", "num_slots")]
+        + [(n, c_void_p) for n in ("q", "k", "v", "out")]
+        + [(n, c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride", "out_stride")]
+        + [(n, c_void_p) for n in ("log_decay", "state_in", "state_out", "slots", "lengths", "status")]
+        + [("scale", c_float)]
+    )
 
 
 P = c_void_p  # device pointers travel as integers
@@ -70,6 +83,9 @@ SIGNATURES = {
     "functs_b200_lstm_forward": (c_int32, [P, P, P, P, P, c_int32, c_int32, c_int32, c_int32, P, P, P, P, P]),
     "functs_b200_lstm_forward_mode": (c_int32, [P, P, P, P, P, c_int32, c_int32, c_int32, c_int32, P, P, P, P, P, c_int32]),
     "functs_b200_debug_set": (c_int32, [c_char_p, c_int32]),
+    "functs_b200_linear_attention_scratch_bytes": (c_int64, [POINTER(LinearAttentionArgs)]),
+    "functs_b200_linear_attention": (c_int32, [POINTER(LinearAttentionArgs), P, P]),
+    "functs_b200_token_logprobs": (c_int32, [P, c_int32, c_int64, P, c_int32, c_int32, c_int32, P, P, P, P, P, P]),
     "functs_b200_yolact_masks": (c_int32, [P, P, P, c_int32, c_int32, c_int32, c_int32, c_float, P, P, P]),
     "functs_b200_access": (c_int32, [P, P, POINTER(AccessDesc), c_int32, P]),
     "functs_b200_select_rev": (c_int32, [P, P, P, POINTER(c_int64), c_int32, c_int32, c_int64, c_int32, P]),

@@ -22,6 +22,8 @@ SOURCES = [
     "kernels_lstm.cu",
     "kernels_lstm_tc.cu",
     "kernels_lstm_rec.cu",
+    "kernels_linattn.cu",
+    "kernels_logprobs.cu",
     "no_alloc.cu",
     "kernels_generic.cu",
     "kernels_region.cu",

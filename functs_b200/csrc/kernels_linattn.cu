@@ -1,0 +1,160 @@
+// Attention with a decaying state, token by token:  S = decay * S + k v^T,  out = scale * S^T q.
+//
+// Serves single tokens (a pass over the states) and, so far, prompts of any length.
+#include <type_traits>
+
+#include "linattn.cuh"
+
+namespace fb {
+
+constexpr int kRecurThreads = 256;
+constexpr int kRecurTokens = 8;  // tokens staged at a time
+
+// A CTA owns COLS = 4 * CG columns of one state: thread -> (column group tid % CG, rows tid / CG + i * RG), so a warp reads whole
+// sectors of 32 / CG rows, and every thread keeps its part of S in registers over all tokens.
+template <typename T, int CG, bool VEC>
+__global__ void __launch_bounds__(kRecurThreads) linattn_recurrent_kernel(const LinArgs a, int tiles) {
+    constexpr int RG = kRecurThreads / CG, ROWS = kLinMaxDim / RG, COLS = 4 * CG, WARPS = kRecurThreads / 32;
+    __shared__ float s_q[kRecurTokens][kLinMaxDim], s_k[kRecurTokens][kLinMaxDim], s_v[kRecurTokens][COLS];
+    __shared__ float s_part[kRecurTokens][WARPS][COLS];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tile = blockIdx.x % tiles, bh = blockIdx.x / tiles, h = bh % a.heads, b = bh / a.heads;
+    const int hk = h / (a.heads / a.kv_heads);
+    const int cg = tid % CG, rg = tid / CG, col0 = tile * COLS, c0 = col0 + cg * 4;
+    const int cols = min(COLS, a.dv - col0);
+    int bits;
+    const int slot = lin_slot(a, b, lane, bits);
+    if (bits != 0 && a.status != nullptr && tid == 0) atomicOr(a.status, bits);
+    const int length = slot < 0 ? 0 : lin_length(a, b);
+    // The decay as a sum of two: its rounding would be the same at every token and add up (2e-6 of the state after 63 tokens; now 1e-7).
+    const double exact = exp(static_cast<double>(a.log_decay[h]));
+    const float decay = static_cast<float>(exact), decay_lo = static_cast<float>(exact - static_cast<double>(decay));
+    const int64_t state = (static_cast<int64_t>(slot < 0 ? 0 : slot) * a.heads + h) * a.dk * a.dv;
+
+    float s[ROWS][4];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const int r = rg + i * RG;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = 0.0f;
+        if (slot >= 0 && a.state_in != nullptr && r < a.dk) {
+            const float* at = a.state_in + state + static_cast<int64_t>(r) * a.dv + c0;
+            if (VEC) {
+                if (c0 < a.dv) {
+                    const float4 x = *reinterpret_cast<const float4*>(at);
+                    s[i][0] = x.x, s[i][1] = x.y, s[i][2] = x.z, s[i][3] = x.w;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (c0 + j < a.dv) s[i][j] = at[j];
+            }
+        }
+    }
+    const T* q = static_cast<const T*>(a.q) + b * a.q_stride[0] + h * a.q_stride[2];
+    const T* k = static_cast<const T*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2];
+    const T* v = static_cast<const T*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2] + col0;
+    T* out = static_cast<T*>(a.out) + b * a.out_stride[0] + h * a.out_stride[2] + col0;
+    // rows that nothing reads stay zero
+    for (int i = tid; i < kRecurTokens * kLinMaxDim; i += kRecurThreads) (&s_q[0][0])[i] = (&s_k[0][0])[i] = 0.0f;
+    for (int i = tid; i < kRecurTokens * COLS; i += kRecurThreads) (&s_v[0][0])[i] = 0.0f;
+    __syncthreads();
+    for (int t0 = 0; t0 < length; t0 += kRecurTokens) {
+        const int n = min(kRecurTokens, length - t0);
+        for (int i = tid; i < n * a.dk; i += kRecurThreads) {
+            const int t = i / a.dk, d = i - t * a.dk;
+            s_q[t][d] = lin_float(q[(t0 + t) * a.q_stride[1] + d]);
+            s_k[t][d] = lin_float(k[(t0 + t) * a.k_stride[1] + d]);
+        }
+        for (int i = tid; i < n * cols; i += kRecurThreads) {
+            const int t = i / cols, d = i - t * cols;
+            s_v[t][d] = lin_float(v[(t0 + t) * a.v_stride[1] + d]);
+        }
+        __syncthreads();
+        for (int t = 0; t < n; ++t) {
+            const float4 vv = *reinterpret_cast<const float4*>(&s_v[t][cg * 4]);
+            float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) {
+                const float kr = s_k[t][rg + i * RG], qr = s_q[t][rg + i * RG];
+                s[i][0] = fmaf(kr, vv.x, fmaf(decay, s[i][0], decay_lo * s[i][0]));
+                s[i][1] = fmaf(kr, vv.y, fmaf(decay, s[i][1], decay_lo * s[i][1]));
+                s[i][2] = fmaf(kr, vv.z, fmaf(decay, s[i][2], decay_lo * s[i][2]));
+                s[i][3] = fmaf(kr, vv.w, fmaf(decay, s[i][3], decay_lo * s[i][3]));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] = fmaf(qr, s[i][j], o[j]);
+            }
+#pragma unroll
+            for (int d = CG; d < 32; d *= 2) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] += __shfl_xor_sync(kFullMask, o[j], d);
+            }
+            if (lane < CG) *reinterpret_cast<float4*>(&s_part[t][warp][cg * 4]) = make_float4(o[0], o[1], o[2], o[3]);
+        }
+        __syncthreads();
+        for (int i = tid; i < n * COLS; i += kRecurThreads) {
+            const int t = i / COLS, d = i % COLS;
+            float o = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) o += s_part[t][w][d];
+            if (d < cols) out[(t0 + t) * a.out_stride[1] + d] = lin_from<T>(o * a.scale);
+        }
+    }
+    for (int i = tid; i < (a.tokens - length) * cols; i += kRecurThreads) {
+        const int t = i / cols, d = i - t * cols;
+        out[(length + t) * a.out_stride[1] + d] = lin_from<T>(0.0f);
+    }
+    if (slot < 0) return;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const int r = rg + i * RG;
+        if (r >= a.dk) continue;
+        float* at = a.state_out + state + static_cast<int64_t>(r) * a.dv + c0;
+        if (VEC) {
+            if (c0 < a.dv) *reinterpret_cast<float4*>(at) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (c0 + j < a.dv) at[j] = s[i][j];
+        }
+    }
+}
+
+template <typename T>
+static int launch_recurrent(const LinArgs& a, cudaStream_t st) {
+    const bool vec = a.dv % 4 == 0 && reinterpret_cast<uintptr_t>(a.state_in) % 16 == 0 && reinterpret_cast<uintptr_t>(a.state_out) % 16 == 0;
+    const int64_t bh = static_cast<int64_t>(a.batch) * a.heads;
+    const int tiles = (a.dv + 31) / 32;
+    FB_REQUIRE(bh * tiles < (1ll << 31), "linear_attention: batch * heads is too large");
+    const dim3 grid(static_cast<unsigned>(bh * tiles));
+    if (vec) return launch_after(linattn_recurrent_kernel<T, 8, true>, grid, dim3(kRecurThreads), 0, st, false, "linear_attention", a, tiles);
+    return launch_after(linattn_recurrent_kernel<T, 8, false>, grid, dim3(kRecurThreads), 0, st, false, "linear_attention", a, tiles);
+}
+
+}  // namespace fb
+
+extern "C" int64_t functs_b200_linear_attention_scratch_bytes(const functs_b200_linear_attention_args* a) {
+    (void)a;
+    return 0;
+}
+
+extern "C" int functs_b200_linear_attention(const functs_b200_linear_attention_args* args, void* scratch, void* stream) {
+    using namespace fb;
+    FB_REQUIRE(args != nullptr, "linear_attention: null pointer");
+    const LinArgs& a = *args;
+    FB_REQUIRE(a.dtype >= FB_DTYPE_F32 && a.dtype <= FB_DTYPE_BF16, "linear_attention: unknown dtype %d", a.dtype);
+    FB_REQUIRE(a.batch >= 0 && a.tokens >= 0 && a.heads > 0 && a.kv_heads > 0 && a.heads % a.kv_heads == 0,
+               "linear_attention: sizes must not be negative, and heads (%d) a multiple of kv_heads (%d)", a.heads, a.kv_heads);
+    FB_REQUIRE(a.dk >= 1 && a.dk <= kLinMaxDim && a.dv >= 1 && a.dv <= kLinMaxDim, "linear_attention: dk (%d) and dv (%d) must be 1 .. %d", a.dk,
+               a.dv, kLinMaxDim);
+    FB_REQUIRE(a.slots != nullptr || a.num_slots == a.batch, "linear_attention: without slots there are as many states as sequences");
+    FB_REQUIRE(a.num_slots >= 0, "linear_attention: num_slots must not be negative");
+    if (a.batch == 0) return FB_OK;
+    FB_REQUIRE(a.log_decay != nullptr && a.state_out != nullptr, "linear_attention: null pointer");
+    FB_REQUIRE(a.tokens == 0 || (a.q != nullptr && a.k != nullptr && a.v != nullptr && a.out != nullptr), "linear_attention: null pointer");
+    (void)scratch;
+    const cudaStream_t st = as_stream(stream);
+    if (a.dtype == FB_DTYPE_F32) return launch_recurrent<float>(a, st);
+    if (a.dtype == FB_DTYPE_F16) return launch_recurrent<__half>(a, st);
+    return launch_recurrent<__nv_bfloat16>(a, st);
+}

@@ -1,0 +1,516 @@
+// Log probabilities of given tokens, entropies and the best alternatives: one pass over the logits.
+//
+//   With any reference c_ref near the row's maximum m (in powers of two: y = x log2 e),  s = sum 2^(y - c_ref)  and
+//   t = sum 2^(y - c_ref) (y - c_ref)  give  log sum exp(x) = ln2 c_ref + ln s  and  entropy = ln s - ln2 t / s.
+// Every thread takes the maximum of its first elements as its reference and changes it only where an element lies 2^80 above it, so that
+// the loop is a fused multiply-add, an exponential and two sums per element; partial sums meet at the row's maximum at the end.
+//
+// Alternatives: each thread also keeps the maximum of its elements.  The top-th largest of those maxima bounds the top-th largest element
+// from below, so only the few threads whose maximum reaches it have candidates: their elements are read again (from L2), what reaches
+// the bound is ordered by rank counting.  Elements equal to the bound are listed too, or, where there are many (a masked row with few
+// finite logits, a constant row), taken by one ordered scan that stops as soon as it has enough.  More candidates than the list holds
+// (rows whose large values sit in few threads) select the bound again by radix, exactly.
+//
+// A row is one CTA, or a cluster of up to eight whose parts meet in the first one's shared memory.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace fb {
+
+constexpr int kLpMaxThreads = 512;
+constexpr int kLpMaxTop = FB_LOGPROBS_MAX_TOP;
+constexpr int kLpMaxParts = 8;               // CTAs per row
+constexpr int kLpList = 1024;                // candidates above the bound; as many equal to it
+constexpr int kLpBusy = 128;                 // threads whose elements are looked through one by one
+constexpr float kLpLog2e = 1.44269504088896340736f;
+constexpr float kLpFloor = -1e30f;           // reference of threads that saw nothing finite
+constexpr float kLpFar = 80.0f;              // how far above its reference, in powers of two, a thread's sums may grow
+
+struct LpArgs {
+    const void* logits;
+    int64_t row_stride;
+    const int64_t* tokens;
+    int32_t vocab, top;
+    float *logprobs, *entropy, *top_logprobs;
+    int64_t* top_ids;
+    int32_t* status;
+};
+
+// Order of values as unsigned numbers: NaN above all, both zeros the same, never 0 (which stands for no element).
+__device__ __forceinline__ uint32_t lp_order(float x) {
+    if (x != x) return 0xFFFFFFFFu;
+    const uint32_t u = __float_as_uint(x + 0.0f);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float lp_value(uint32_t order) {
+    if (order == 0xFFFFFFFFu) return __uint_as_float(0x7FFFFFFFu);
+    return __uint_as_float((order & 0x80000000u) ? (order & 0x7FFFFFFFu) : ~order);
+}
+__device__ __forceinline__ uint64_t lp_key(uint32_t order, uint32_t id) { return (static_cast<uint64_t>(order) << 32) | (0xFFFFFFFFu - id); }
+
+__device__ __forceinline__ float lp_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename T>
+struct LpVec;
+template <>
+struct LpVec<float> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ void get(const uint4& u, float (&x)[4]) {
+        x[0] = __uint_as_float(u.x), x[1] = __uint_as_float(u.y), x[2] = __uint_as_float(u.z), x[3] = __uint_as_float(u.w);
+    }
+    static __device__ __forceinline__ float one(const float* p) { return *p; }
+};
+template <>
+struct LpVec<__nv_bfloat16> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void get(const uint4& u, float (&x)[8]) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+    static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+};
+template <>
+struct LpVec<__half> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void get(const uint4& u, float (&x)[8]) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
+    }
+    static __device__ __forceinline__ float one(const __half* p) { return __half2float(*p); }
+};
+
+// sums of one thread, one warp, one part of a row
+struct LpSums {
+    float most;  // the largest element (NaN if there is one)
+    float ref;   // reference, in powers of two
+    float s, t;
+};
+
+// takes `o` into `a`, at the larger of the two references
+__device__ __forceinline__ void lp_join(LpSums& a, const LpSums& o) {
+    const float ref = fmaxf(a.ref, o.ref);
+    const float da = a.ref - ref, db = o.ref - ref;  // one of them is 0
+    const float fa = lp_ex2(da), fb_ = lp_ex2(db);
+    // (a reference at the floor has no sums, and its distance must not meet them)
+    a.t = fa * fmaf(da, fa > 0.0f ? a.s : 0.0f, a.t) + fb_ * fmaf(db, fb_ > 0.0f ? o.s : 0.0f, o.t);
+    a.s = fa * a.s + fb_ * o.s;
+    a.ref = ref;
+    a.most = max_nan(a.most, o.most);
+}
+
+struct LpThread {
+    LpSums sums;
+
+    __device__ __forceinline__ void start() { sums = {__int_as_float(0xff800000), kLpFloor, 0.0f, 0.0f}; }
+    __device__ __forceinline__ void raise(float x) {  // the reference, to x
+        const float to = x * kLpLog2e, d = sums.ref - to, f = lp_ex2(d);
+        sums.t = f > 0.0f ? f * fmaf(d, sums.s, sums.t) : 0.0f;
+        sums.s = f * sums.s;
+        sums.ref = to;
+    }
+    template <int N>
+    __device__ __forceinline__ void take(const float (&x)[N]) {
+        float m = x[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) m = max_nan(m, x[i]);
+        sums.most = max_nan(sums.most, m);
+        if (fmaf(m, kLpLog2e, -sums.ref) > kLpFar) raise(m);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float d = max_nan(fmaf(x[i], kLpLog2e, -sums.ref), -1000.0f);  // (-inf: its power is 0, and 0 * d must be)
+            const float e = lp_ex2(d);
+            sums.s += e;
+            sums.t = fmaf(e, d, sums.t);
+        }
+    }
+};
+
+struct LpShared {
+    LpSums sums[kLpMaxThreads / 32];
+    LpSums part;                              // of this CTA
+    uint64_t most[kLpMaxThreads];             // maxima of the threads that may have candidates
+    uint64_t above[kLpList], equal[kLpList];  // candidates
+    uint64_t best[kLpMaxTop];                 // this CTA's, in order
+    uint64_t row_best[kLpMaxTop];             // the row's
+    double log_sum;
+    uint32_t hist[256];
+    uint32_t warp_count[kLpMaxThreads / 32];
+    int busy[kLpBusy];                        // threads that have candidates
+    int num_threads, num_most, num_above, num_equal;
+    uint32_t bound, digit, wanted;
+    bool empty;
+};
+
+__device__ __forceinline__ uint32_t lp_cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void lp_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t lp_map(const void* p, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float lp_remote_f32(uint32_t at) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint64_t lp_remote_u64(uint32_t at) {
+    uint64_t v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
+    return v;
+}
+
+// The elements of a part of a row: vectors, and single ones in front of (first part) and behind (last part) the row's 16-byte boundaries.
+template <typename T>
+struct LpPart {
+    const T* row;
+    int head, vec_id, num_vec, tail, tail_id;  // ids: of the first vector's first element, of the tail's first
+    __device__ __forceinline__ int id_of(int v) const { return vec_id + v * LpVec<T>::N; }
+    __device__ __forceinline__ uint4 vec(int v) const { return *reinterpret_cast<const uint4*>(row + id_of(v)); }
+    __device__ __forceinline__ int count() const { return head + num_vec * LpVec<T>::N + tail; }
+    __device__ __forceinline__ int id_at(int e) const {  // of the part's e-th element
+        if (e < head) return e;
+        e -= head;
+        return e < num_vec * LpVec<T>::N ? vec_id + e : tail_id + (e - num_vec * LpVec<T>::N);
+    }
+    __device__ __forceinline__ uint32_t order(int id) const { return lp_order(LpVec<T>::one(row + id)); }
+};
+
+// number of entries of a list that is in descending order that are above `key`
+__device__ __forceinline__ int lp_above(uint32_t at, int n, uint64_t key) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (lp_remote_u64(at + mid * 8) > key) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// calls f(order, id) for the elements that thread `who` of the block has, lane `lane` of `lanes` its share of them
+template <typename T, class F>
+__device__ __forceinline__ void lp_each(const LpPart<T>& p, int who, int lane, int lanes, F f) {
+    constexpr int N = LpVec<T>::N;
+    const int threads = blockDim.x;
+    for (int v = who + lane * threads; v < p.num_vec; v += lanes * threads) {
+        float x[N];
+        LpVec<T>::get(p.vec(v), x);
+#pragma unroll
+        for (int i = 0; i < N; ++i) f(lp_order(x[i]), p.id_of(v) + i);
+    }
+    if (lane == 0 && who < p.head) f(p.order(who), who);
+    if (lane == 0 && who < p.tail) f(p.order(p.tail_id + who), p.tail_id + who);
+}
+
+// The `top` best of the part (keys 0 behind them if it has fewer), best first, in sh.best.  most: of this thread's elements.
+template <typename T>
+__device__ void lp_select(LpShared& sh, const LpPart<T>& p, int top, float most) {
+    constexpr int N = LpVec<T>::N;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
+    const uint32_t mine = tid < p.num_vec || tid < p.head || tid < p.tail ? lp_order(most) : 0u;
+    if (tid < top) sh.best[tid] = 0;
+    if (tid == 0) sh.num_threads = sh.num_above = sh.num_equal = sh.num_most = 0, sh.bound = 0;
+    // a first bound: the smallest, over the warps, of their (top / warps)-th largest lane
+    uint32_t left = mine, least = 0;
+    for (int i = 0; i < top; i += warps) {
+        least = __reduce_max_sync(kFullMask, left);
+        if (lane == __ffs(__ballot_sync(kFullMask, left == least)) - 1) left = 0;
+    }
+    if (lane == 0) sh.warp_count[warp] = least;
+    __syncthreads();
+    uint32_t first = sh.warp_count[0];
+    for (int w = 1; w < warps; ++w) first = min(first, sh.warp_count[w]);
+    // the top-th largest of the threads' maxima: among those that reach the first bound, by counting
+    if (mine >= first && mine != 0) sh.most[atomicAdd(&sh.num_most, 1)] = lp_key(mine, tid);
+    __syncthreads();
+    const int reach = sh.num_most;
+    for (int i = tid; i < reach; i += threads) {
+        const uint64_t key = sh.most[i];
+        int rank = 0;
+        for (int j = 0; j < reach; ++j) rank += sh.most[j] > key;
+        if (rank == top - 1) sh.bound = static_cast<uint32_t>(key >> 32);  // (nobody: fewer threads than that have elements, all count)
+    }
+    __syncthreads();
+    uint32_t bound = sh.bound;
+    if (mine != 0 && mine >= bound) {
+        const int at = atomicAdd(&sh.num_threads, 1);
+        if (at < kLpBusy) sh.busy[at] = tid;
+    }
+    __syncthreads();
+    const auto list = [&](uint32_t order, int id) {
+        if (order < bound) return;
+        if (order > bound) {
+            const int at = atomicAdd(&sh.num_above, 1);
+            if (at < kLpList) sh.above[at] = lp_key(order, id);
+        } else {
+            const int at = atomicAdd(&sh.num_equal, 1);
+            if (at < kLpList) sh.equal[at] = lp_key(order, id);
+        }
+    };
+    const int busy = sh.num_threads;
+    if (busy <= kLpBusy) {
+        for (int c = warp; c < busy; c += warps) lp_each(p, sh.busy[c], lane, 32, list);
+    } else {
+        lp_each(p, tid, 0, 1, list);
+    }
+    __syncthreads();
+    if (sh.num_above > kLpList) {
+        // too many: the top-th largest element itself, eight bits at a time
+        uint32_t prefix = 0, mask = 0, wanted = top;
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            for (int i = tid; i < 256; i += threads) sh.hist[i] = 0;
+            __syncthreads();
+            lp_each(p, tid, 0, 1, [&](uint32_t order, int) {
+                if ((order & mask) == prefix) atomicAdd(&sh.hist[(order >> shift) & 255u], 1u);
+            });
+            __syncthreads();
+            if (tid == 0) {
+                uint32_t seen = 0;
+                int digit = 255;
+                for (; digit > 0 && seen + sh.hist[digit] < wanted; --digit) seen += sh.hist[digit];
+                sh.digit = digit;
+                sh.wanted = wanted - seen;
+            }
+            __syncthreads();
+            prefix |= sh.digit << shift;
+            mask |= 255u << shift;
+            wanted = sh.wanted;
+        }
+        __syncthreads();
+        bound = prefix;
+        if (tid == 0) sh.num_above = sh.num_equal = 0;
+        __syncthreads();
+        lp_each(p, tid, 0, 1, list);
+        __syncthreads();
+    }
+    const int above = sh.num_above, equal = sh.num_equal;
+    for (int i = tid; i < above; i += threads) {
+        const uint64_t key = sh.above[i];
+        int rank = 0;
+        for (int j = 0; j < above; ++j) rank += sh.above[j] > key;
+        if (rank < top) sh.best[rank] = key;
+    }
+    int need = max(0, min(top - above, equal)), place = above;
+    if (equal <= kLpList) {
+        if (need > 0) {
+            for (int i = tid; i < equal; i += threads) {
+                const uint64_t key = sh.equal[i];
+                int rank = 0;
+                for (int j = 0; j < equal; ++j) rank += sh.equal[j] > key;
+                if (rank < need) sh.best[place + rank] = key;
+            }
+        }
+    } else {
+        // many are equal to the bound: the first of them, by a scan in order
+        const int total = p.count();
+        for (int base = 0; base < total && need > 0; base += threads * N) {
+            uint32_t hit = 0;
+            for (int i = 0; i < N; ++i) {
+                const int e = base + tid * N + i;
+                if (e < total && p.order(p.id_at(e)) == bound) hit |= 1u << i;
+            }
+            int before = __popc(hit);
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) {
+                const int o = __shfl_up_sync(kFullMask, before, d);
+                if (lane >= d) before += o;
+            }
+            if (lane == 31) sh.warp_count[warp] = before;
+            __syncthreads();
+            before -= __popc(hit);
+            int all = 0;
+            for (int w = 0; w < warps; ++w) {
+                if (w < warp) before += sh.warp_count[w];
+                all += sh.warp_count[w];
+            }
+            for (int i = 0; i < N; ++i) {
+                if (!((hit >> i) & 1u)) continue;
+                if (before < need) sh.best[place + before] = lp_key(bound, p.id_at(base + tid * N + i));
+                ++before;
+            }
+            __syncthreads();
+            place += min(all, need);
+            need -= min(all, need);
+        }
+    }
+    __syncthreads();
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kLpMaxThreads) logprobs_kernel(const LpArgs a, int parts) {
+    constexpr int N = LpVec<T>::N;
+    __shared__ LpShared sh;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
+    const int rank = parts > 1 ? static_cast<int>(lp_cluster_rank()) : 0;
+    const int64_t r = blockIdx.x / parts;
+    LpPart<T> p;
+    p.row = static_cast<const T*>(a.logits) + r * a.row_stride;
+    const int off = static_cast<int>((reinterpret_cast<uintptr_t>(p.row) & 15u) / sizeof(T));
+    const int head = min(a.vocab, off == 0 ? 0 : N - off), vecs = (a.vocab - head) / N, share = (vecs + parts - 1) / parts;
+    const int first = min(vecs, rank * share);
+    p.head = rank == 0 ? head : 0;
+    p.vec_id = head + first * N;
+    p.num_vec = min(share, vecs - first);
+    p.tail_id = head + vecs * N;
+    p.tail = rank == parts - 1 ? a.vocab - p.tail_id : 0;
+    int64_t token = -1;
+    float token_logit = 0.0f;
+    if (rank == 0 && tid == 0) {
+        token = a.tokens[r];
+        if (token >= 0 && token < a.vocab) token_logit = LpVec<T>::one(p.row + token);
+    }
+
+    LpThread th;
+    th.start();
+    if (tid < p.head) th.take({LpVec<T>::one(p.row + tid)});
+    if (tid < p.tail) th.take({LpVec<T>::one(p.row + p.tail_id + tid)});
+    int v = tid;
+    for (; v + 3 * threads < p.num_vec; v += 4 * threads) {
+        uint4 u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = p.vec(v + i * threads);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float x[N];
+            LpVec<T>::get(u[i], x);
+            th.take(x);
+        }
+    }
+    for (; v < p.num_vec; v += threads) {
+        float x[N];
+        LpVec<T>::get(p.vec(v), x);
+        th.take(x);
+    }
+    // the block's sums
+    LpSums sums = th.sums;
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) {
+        LpSums o;
+        o.most = __shfl_xor_sync(kFullMask, sums.most, d);
+        o.ref = __shfl_xor_sync(kFullMask, sums.ref, d);
+        o.s = __shfl_xor_sync(kFullMask, sums.s, d);
+        o.t = __shfl_xor_sync(kFullMask, sums.t, d);
+        lp_join(sums, o);
+    }
+    if (lane == 0) sh.sums[warp] = sums;
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < warps; ++w) lp_join(sums, sh.sums[w]);
+        sh.part = sums;
+    }
+    if (TOP) lp_select<T>(sh, p, a.top, th.sums.most);
+    if (parts > 1) lp_cluster_sync();
+    else __syncthreads();
+    // the row's first CTA finishes it
+    if (rank == 0) {
+        if (tid == 0) {
+            for (int c = 1; c < parts; ++c) {
+                const uint32_t at = lp_map(&sh.part, c);
+                const LpSums o = {lp_remote_f32(at), lp_remote_f32(at + 4), lp_remote_f32(at + 8), lp_remote_f32(at + 12)};
+                lp_join(sums, o);
+            }
+            // (the exponents were x log2e with log2e in 32 bits: the reference goes back by the same number)
+            const double ref = static_cast<double>(sums.ref) / static_cast<double>(kLpLog2e);
+            const double log_s = log(static_cast<double>(sums.s));
+            const bool empty = sums.most == __int_as_float(0xff800000);
+            sh.log_sum = ref + log_s;
+            sh.empty = empty;
+            const double x = static_cast<double>(token_logit);
+            float lp = static_cast<float>(x - sh.log_sum);
+            if (empty) lp = __int_as_float(0xff800000);
+            if (token < 0) lp = 0.0f;
+            if (token >= a.vocab) {
+                lp = __int_as_float(0x7fffffff);
+                if (a.status != nullptr) atomicOr(a.status, FB_STATUS_INDEX_RANGE);
+            }
+            a.logprobs[r] = lp;
+            a.entropy[r] = empty ? 0.0f : static_cast<float>(log_s - static_cast<double>(sums.t) / (static_cast<double>(sums.s) * static_cast<double>(kLpLog2e)));
+        }
+        if (TOP) {
+            // every part's list is in order: a candidate's place is the number of larger ones, found by halving
+            for (int i = tid; i < parts * a.top; i += threads) {
+                const int c = i / a.top;
+                const uint64_t key = lp_remote_u64(lp_map(&sh.best[i - c * a.top], c));
+                int place = 0;
+                for (int o = 0; o < parts; ++o) place += o == c ? i - c * a.top : lp_above(lp_map(sh.best, o), a.top, key);
+                if (key != 0 && place < a.top) sh.row_best[place] = key;
+            }
+            __syncthreads();
+            for (int i = tid; i < a.top; i += threads) {
+                const uint64_t key = sh.row_best[i];
+                const float x = lp_value(static_cast<uint32_t>(key >> 32));
+                a.top_logprobs[r * a.top + i] = sh.empty ? __int_as_float(0xff800000) : static_cast<float>(static_cast<double>(x) - sh.log_sum);
+                a.top_ids[r * a.top + i] = static_cast<int64_t>(0xFFFFFFFFu - static_cast<uint32_t>(key));
+            }
+        }
+    }
+    if (parts > 1) lp_cluster_sync();  // nobody leaves while the first CTA reads
+}
+
+template <typename T, bool TOP>
+static int launch_logprobs(const LpArgs& a, int rows, cudaStream_t st) {
+    const int vecs = a.vocab / LpVec<T>::N;
+    int parts = 1;
+    while (parts < kLpMaxParts && static_cast<int64_t>(rows) * parts * 2 <= 2 * kNumSMs && vecs / (parts * 2) >= 256) parts *= 2;
+    const int each = vecs / parts;
+    const int threads = each >= 1024 ? 512 : each >= 512 ? 256 : each >= 128 ? 128 : 64;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(rows) * parts);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = parts;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = parts > 1 ? 1 : 0;
+    FB_TRY(check_cuda(cudaLaunchKernelEx(&cfg, logprobs_kernel<T, TOP>, a, parts), "token_logprobs"));
+    count_launch();
+    return FB_OK;
+}
+
+template <typename T>
+static int launch_logprobs(const LpArgs& a, int rows, cudaStream_t st) {
+    return a.top > 0 ? launch_logprobs<T, true>(a, rows, st) : launch_logprobs<T, false>(a, rows, st);
+}
+
+}  // namespace fb
+
+extern "C" int functs_b200_token_logprobs(const void* logits, int32_t dtype, int64_t row_stride, const int64_t* tokens, int32_t rows,
+                                          int32_t vocab, int32_t top, float* logprobs, float* entropy, float* top_logprobs,
+                                          int64_t* top_ids, int32_t* status, void* stream) {
+    using namespace fb;
+    FB_REQUIRE(dtype >= FB_DTYPE_F32 && dtype <= FB_DTYPE_BF16, "token_logprobs: unknown dtype %d", dtype);
+    FB_REQUIRE(rows >= 0 && rows <= (1 << 24), "token_logprobs: rows must be 0 .. %d", 1 << 24);
+    FB_REQUIRE(vocab >= 1 && vocab <= (1 << 30), "token_logprobs: vocab must be 1 .. %d", 1 << 30);
+    FB_REQUIRE(top >= 0 && top <= kLpMaxTop && top <= vocab, "token_logprobs: top must be 0 .. %d and at most vocab", kLpMaxTop);
+    if (rows == 0) return FB_OK;
+    FB_REQUIRE(logits != nullptr && tokens != nullptr && logprobs != nullptr && entropy != nullptr, "token_logprobs: null pointer");
+    FB_REQUIRE(top == 0 || (top_logprobs != nullptr && top_ids != nullptr), "token_logprobs: null pointer");
+    FB_REQUIRE(reinterpret_cast<uintptr_t>(logits) % (dtype == FB_DTYPE_F32 ? 4 : 2) == 0, "token_logprobs: logits must lie on a boundary of their type");
+    const LpArgs a = {logits, row_stride, tokens, vocab, top, logprobs, entropy, top_logprobs, top_ids, status};
+    const cudaStream_t st = as_stream(stream);
+    if (dtype == FB_DTYPE_F32) return launch_logprobs<float>(a, rows, st);
+    if (dtype == FB_DTYPE_F16) return launch_logprobs<__half>(a, rows, st);
+    return launch_logprobs<__nv_bfloat16>(a, rows, st);
+}

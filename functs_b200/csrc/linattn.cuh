@@ -1,0 +1,57 @@
+// Attention with a decaying state: what its kernels share.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace fb {
+
+using LinArgs = functs_b200_linear_attention_args;
+
+constexpr int kLinMaxDim = 128;
+
+#ifdef __CUDACC__
+
+__device__ __forceinline__ float lin_float(float x) { return x; }
+__device__ __forceinline__ float lin_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float lin_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T lin_from(float x);
+template <>
+__device__ __forceinline__ float lin_from<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half lin_from<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 lin_from<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// exp(log_decay * n): the weight of a token n steps back.  A decay of -inf forgets at once, but not what it just saw: n = 0 is 1.
+__device__ __forceinline__ float lin_decay(float log_decay, int n) { return expf(fmaxf(log_decay, -1e30f) * static_cast<float>(n)); }
+
+__device__ __forceinline__ int lin_length(const LinArgs& a, int b) {
+    return a.lengths == nullptr ? a.tokens : min(max(a.lengths[b], 0), a.tokens);
+}
+
+// The state that sequence b uses, or -1 for none; `bits` gets the status bit that says why.  Called by a whole warp.
+__device__ __forceinline__ int lin_slot(const LinArgs& a, int b, int lane, int& bits) {
+    bits = 0;
+    if (a.slots == nullptr) return b;
+    const int slot = a.slots[b];
+    if (slot < 0) return -1;
+    if (slot >= a.num_slots) {
+        bits = FB_STATUS_INDEX_RANGE;
+        return -1;
+    }
+    bool twice = false;
+    for (int i = lane; i < b; i += 32) twice |= a.slots[i] == slot;
+    if (__any_sync(kFullMask, twice)) {
+        bits = FB_STATUS_INDEX_TWICE;
+        return -1;
+    }
+    return slot;
+}
+
+#endif
+
+}  // namespace fb

@@ -15,6 +15,7 @@
 #include "../../../include/functs_b200.h"
 #include "detect.h"
 #include "fusion.h"
+#include "sequence.h"
 #include "tensorssa.h"
 
 namespace py = pybind11;
@@ -219,6 +220,10 @@ PYBIND11_MODULE(_C, m) {
                                         static_cast<int32_t>(H), static_cast<int32_t>(W), static_cast<int32_t>(c.size(1)),
                                         static_cast<float>(thr), out.data_ptr<uint8_t>(), nullptr, at::cuda::getCurrentCUDAStream().stream());
     });
+    // sequence operators (functs_b200/ops.py)
+    m.def("_linear_attention", &functs_b200::linearAttention, py::call_guard<py::gil_scoped_release>());
+    m.def("_linear_attention_step", &functs_b200::linearAttentionStep, py::call_guard<py::gil_scoped_release>());
+    m.def("_token_logprobs", &functs_b200::tokenLogprobs, py::call_guard<py::gil_scoped_release>());
     m.def("_count_parallel_functors", [](std::shared_ptr<Graph> g) { return functs_b200::CountParallelFunctors(g); });
     m.def("_jit_pass_freeze", [](torch::jit::Module& module) { return torch::jit::freeze_module(module); });
     m.def("_jit_pass_clone", [](torch::jit::Module& module) { return module.clone(); });

@@ -46,6 +46,8 @@ def raise_on_status(status: torch.Tensor, what: str) -> None:
         msgs.append("a bounded device-side wait ran out")
     if bits & _lib.FB_STATUS_INDEX_RANGE:
         msgs.append("an index was out of range")
+    if bits & _lib.FB_STATUS_INDEX_TWICE:
+        msgs.append("an index was named twice")
     raise _lib.FunctsB200Error(f"{what}: " + "; ".join(msgs) + f" (status={bits})")
 
 
@@ -267,6 +269,53 @@ def lstm_forward(x: torch.Tensor, w_ih: torch.Tensor, w_hh: torch.Tensor, b_ih: 
     if own_status:
         raise_on_status(status, "lstm_forward")
     return hs, cs
+
+
+# ---- sequence models beside the LSTM ---------------------------------------------------------------------------
+
+
+def _native():
+    from . import _C  # built with the package; the calls below do their checks and allocations there
+    return _C
+
+
+def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, scale: float = 1.0,
+                     state: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None,
+                     lengths: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                     status: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Attention with a decaying state over whole prompts: per sequence and head, for every token t,
+    S = exp(log_decay) * S + k[t] v[t]^T,  out[t] = scale * S^T q[t], with S [Dk, Dv] in fp32.
+
+    q [B, T, H, Dk], k [B, T, Hk, Dk], v [B, T, Hk, Dv] in float32, float16 or bfloat16, H a multiple of Hk (heads share keys and
+    values in groups), up to 128 channels; any strides with adjacent channels (others are copied), so views of one fused
+    projection and time-major tensors go in as they are.  log_decay float32 [H].  Returns (out [B, T, H, Dv], states).
+
+    state: float32 [N, H, Dk, Dv], contiguous, read and updated in place: sequence b's is state[slots[b]] (slots int32 [B]), or state[b]
+    without slots.  A negative slot is no sequence (zero rows in out).  So is one of N or above, or one that an earlier sequence has
+    already, and `status` gets the bit that raise_on_status reports.  Without state, sequences start from zero and the states returned
+    are new, [B, H, Dk, Dv].
+    lengths int32 [B] (on the device; taken as 0 to T): a sequence ends there; its later rows are not read, and are zero in out.
+    A token with a NaN or an infinity leaves the outputs before it alone; from it on they are not finite where the formula's are not
+    (an infinity of the formula may be a NaN).  No gradients: inputs that require one are refused."""
+    return _native()._linear_attention(q, k, v, log_decay, scale, state, slots, lengths, out, status)
+
+
+def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, state: torch.Tensor,
+                          scale: float = 1.0, slots: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                          status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """linear_attention for one token per sequence: q [B, H, Dk], k [B, Hk, Dk], v [B, Hk, Dv] -> out [B, H, Dv]; `state` (a pool, with
+    slots) is updated in place.  Nothing is allocated but out, and nothing synchronises: fit for a captured graph."""
+    return _native()._linear_attention_step(q, k, v, log_decay, state, scale, slots, out, status)
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, status: Optional[torch.Tensor] = None):
+    """What a model answers with: logits [R, V] (float32, float16 or bfloat16; rows any distance apart), tokens int64 [R] ->
+    (logprobs float32 [R] of the tokens, entropy float32 [R] in nats, top_logprobs float32 [R, top], top_ids int64 [R, top]).
+
+    top: up to 64 alternatives, best first, of equal ones the lowest id first.  -inf masks a token.  A row of -inf alone: log
+    probabilities -inf, entropy 0, the lowest ids.  A row with NaN or +inf: NaN (the ids still in order, NaN first).  A negative token:
+    0, nothing is scored; a token of V or above: NaN, and `status` (int32, on the device or pinned) gets FB_STATUS_INDEX_RANGE."""
+    return _native()._token_logprobs(logits, tokens, top, status)
 
 
 # ---- C5 ------------------------------------------------------------------------------------------------------

@@ -38,6 +38,7 @@ extern "C" {
 #define FB_STATUS_CAND_OVERFLOW 1 /* a candidate list was longer than its capacity; extra candidates were dropped */
 #define FB_STATUS_WAIT_TIMEOUT 2  /* a bounded device-side wait ran out */
 #define FB_STATUS_INDEX_RANGE 4   /* an index tensor (or a candidate key) named a row outside the indexed extent */
+#define FB_STATUS_INDEX_TWICE 8   /* an index tensor named a row twice that only one may write */
 
 /* ---- library ------------------------------------------------------------------------- */
 
@@ -244,6 +245,50 @@ int functs_b200_lstm_forward(const float* x, const float* w_ih, const float* w_h
 int functs_b200_lstm_forward_mode(const float* x, const float* w_ih, const float* w_hh, const float* b_ih,
                                   const float* b_hh, int32_t seq_len, int32_t batch, int32_t input, int32_t hidden,
                                   float* hs, float* cs, int32_t* status, void* scratch, void* stream, int32_t mode);
+
+/* ---- sequence models beside the LSTM: attention with a decaying state ------------------------- */
+/* element types of the sequence operators */
+#define FB_DTYPE_F32 0
+#define FB_DTYPE_F16 1
+#define FB_DTYPE_BF16 2
+
+/* The loop  for t < tokens: S = exp(log_decay[h]) * S + k[t] v[t]^T;  out[t] = scale * S^T q[t]  for every sequence b and head h, S being a
+ * [dk, dv] matrix in fp32.  q [batch, tokens, heads, dk], k [.., kv_heads, dk], v [.., kv_heads, dv], out [.., heads, dv]: elements of
+ * `dtype`, channels adjacent, the other strides free; head h reads key and value head h / (heads / kv_heads).  1 <= dk, dv <= 128.
+ * log_decay [heads] fp32 (0 or less; -inf forgets at once).
+ * Sequence b starts from state_in and leaves its last state in state_out, both [num_slots, heads, dk, dv] fp32 (the same memory if the
+ * caller likes); state_in = NULL starts from zero.  slots (optional, int32 [batch]) says which of them is sequence b's, else it is b and
+ * num_slots = batch.  A negative slot is no sequence: its rows of out are zero, and no state is touched.  So is, with a status bit, one
+ * of num_slots or above (FB_STATUS_INDEX_RANGE) and one that an earlier sequence has (FB_STATUS_INDEX_TWICE).
+ * lengths (optional, int32 [batch], taken as 0 .. tokens): sequence b ends there; its later rows are not read, and zero in out.
+ * status: optional.  One launch for a few tokens, for longer prompts one, or two and three where sequences are cut into parts.
+ * scratch: functs_b200_linear_attention_scratch_bytes, 16-byte aligned (may be NULL where that is 0). */
+typedef struct {
+    int32_t dtype, batch, tokens, heads, kv_heads, dk, dv, num_slots;
+    const void *q, *k, *v;
+    void* out;
+    int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3]; /* sequence, token, head; in elements */
+    const float* log_decay;
+    const float* state_in;
+    float* state_out;
+    const int32_t* slots;
+    const int32_t* lengths;
+    int32_t* status;
+    float scale;
+} functs_b200_linear_attention_args;
+int64_t functs_b200_linear_attention_scratch_bytes(const functs_b200_linear_attention_args* args);
+int functs_b200_linear_attention(const functs_b200_linear_attention_args* args, void* scratch, void* stream); /* args in HOST memory */
+
+/* What a model answers with: for every row of logits [rows, vocab] (elements of dtype, row_stride elements apart)
+ *   logprobs[r]      = x[tokens[r]] - log sum_i exp(x[i])         (0 where tokens[r] is negative: nothing is scored there)
+ *   entropy[r]       = - sum_i p[i] log p[i],  p = softmax(x)     (a term with p = 0 is 0)
+ *   top_ids, top_logprobs [rows, top]: the `top` best, best first, of equal ones the lowest id first (top <= 64, <= vocab)
+ * A row of nothing but -inf has no distribution: log probabilities -inf, entropy 0.  A row with a NaN or +inf gives NaN (NaN comes
+ * first among the best).  A token of vocab or above gives NaN and FB_STATUS_INDEX_RANGE.  One launch, no scratch. */
+#define FB_LOGPROBS_MAX_TOP 64
+int functs_b200_token_logprobs(const void* logits, int32_t dtype, int64_t row_stride, const int64_t* tokens, int32_t rows, int32_t vocab,
+                               int32_t top, float* logprobs, float* entropy, float* top_logprobs, int64_t* top_ids, int32_t* status,
+                               void* stream);
 
 /* Debugging switches (name -> value); returns FB_ERR_NOT_FOUND for an unknown name.
  *   "yolo_prune": 0 makes functs_b200_yolo_postprocess keep every candidate above the score threshold instead of

@@ -1,0 +1,455 @@
+"""Attention with a decaying state and log probabilities of tokens, against their definitions in 64 bits."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def ops(cuda_device):
+    import functs_b200
+    return functs_b200.ops
+
+
+# ---- attention with a decaying state: the definition --------------------------------------------------------------------
+
+
+def recurrence(q, k, v, log_decay, scale, state, lengths):
+    """The definition, token by token in 64 bits, and the same with every factor's magnitude (what rounding errors are relative to)."""
+    b, t, h, _ = q.shape
+    share = torch.arange(h, device=q.device) // (h // k.size(2))
+    decay = torch.exp(log_decay.double())[None, :, None, None]
+    s = torch.zeros(b, h, q.size(3), v.size(3), dtype=torch.float64, device=q.device) if state is None else state.double()
+    m = s.abs()
+    out = torch.zeros(b, t, h, v.size(3), dtype=torch.float64, device=q.device)
+    mag = torch.zeros_like(out)
+    for i in range(t):
+        live = (i < lengths)[:, None, None, None]
+        qi, ki, vi = (torch.where(live[..., 0], x, 0.0) for x in (q[:, i].double(), k[:, i].double()[:, share], v[:, i].double()[:, share]))
+        step = ki[..., None] * vi[..., None, :]
+        s = torch.where(live, decay * s + step, s)
+        m = torch.where(live, decay * m + step.abs(), m)
+        out[:, i] = (qi[..., None, :] @ s)[..., 0, :] * scale * live[..., 0]
+        mag[:, i] = (qi.abs()[..., None, :] @ m)[..., 0, :] * abs(scale) * live[..., 0]
+    return out, s, mag, m
+
+
+def check_attention(got_out, got_state, want, dtype, tokens, dk):
+    """Errors are bounded relative to the sum of the magnitudes of the terms.  In 32 bits every token adds at most four roundings of 2^-24
+    to what is carried (the product with the decay, the sum, and two units of the decay itself), the dot product dk.  Beside that, 16-bit
+    types may hold the states and the weights of a chunk as two parts of eight bits each for the product that makes `out` (2^-17 per
+    factor, two factors), and `out` is rounded once (half a step)."""
+    out, state, mag, m = want
+    carried = (4 * tokens + dk + 8) * 2.0 ** -24
+    half = 0.0 if dtype == F32 else torch.finfo(dtype).eps / 2
+    tol = half * out.abs() + (carried + (0.0 if dtype == F32 else 2.0 ** -15)) * mag + (torch.finfo(dtype).tiny if dtype != F32 else 0.0)
+    err = (got_out.double() - out).abs()
+    assert bool((err <= tol).all()), f"out: error {float((err - tol).max()):.3g} over its bound"
+    assert bool(((got_state.double() - state).abs() <= carried * m).all()), "state outside its bound"
+    # and together: far inside the bounds above
+    off = float((got_state.double() - state).norm()) / max(float(state.norm()), 1e-30)
+    assert off <= 1e-6, f"state: {off:.3g} off"
+    if dtype == F32:
+        off = float(err.norm()) / max(float(out.norm()), 1e-30)
+        assert off <= 1e-6, f"out: {off:.3g} off"
+
+
+def make(b, t, h, hk, dk, dv, dtype, layout="batch", seed=1):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    if layout == "fused":
+        x = torch.randn(b, t, h * dk + hk * (dk + dv), generator=g, device="cuda").to(dtype)
+        q, k, v = x.split([h * dk, hk * dk, hk * dv], dim=-1)
+        return q.unflatten(-1, (h, dk)), k.unflatten(-1, (hk, dk)), v.unflatten(-1, (hk, dv))
+    qkv = [torch.randn(b, t, n, d, generator=g, device="cuda").to(dtype) for n, d in ((h, dk), (hk, dk), (hk, dv))]
+    if layout == "time":  # [T, B, ...] in memory
+        qkv = [x.transpose(0, 1).contiguous().transpose(0, 1) for x in qkv]
+    if layout == "heads":  # [B, H, T, ...] in memory
+        qkv = [x.transpose(1, 2).contiguous().transpose(1, 2) for x in qkv]
+    if layout == "odd":  # rows that no vector load fits
+        qkv = [torch.nn.functional.pad(x, (1, 2))[..., 1:-2] for x in qkv]
+    return qkv
+
+
+def decays(h, seed=1):
+    return -torch.exp2(-8.0 * torch.arange(1, h + 1, device="cuda", dtype=F32) / h)
+
+
+SHAPES = [
+    # b, t, h, hk, dk, dv
+    (1, 1, 1, 1, 1, 1), (2, 1, 3, 1, 128, 128), (3, 2, 4, 2, 17, 33), (1, 7, 2, 2, 64, 64), (2, 63, 2, 2, 128, 128), (2, 64, 2, 1, 128, 64),
+    (1, 65, 3, 3, 64, 128), (3, 129, 4, 2, 80, 48), (1, 200, 2, 2, 37, 5), (1, 700, 3, 3, 128, 128), (2, 333, 2, 2, 64, 64), (2, 130, 1, 1, 96, 112),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_prompt(ops, shape, dtype):
+    b, t, h, hk, dk, dv = shape
+    q, k, v = make(*shape, dtype)
+    full = torch.full((b,), t, device="cuda")
+    out, state = ops.linear_attention(q, k, v, decays(h), scale=dk ** -0.5)
+    assert out.dtype == dtype and out.shape == (b, t, h, dv) and state.dtype == F32 and state.shape == (b, h, dk, dv)
+    check_attention(out, state, recurrence(q, k, v, decays(h), dk ** -0.5, None, full), dtype, t, dk)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("layout", ["fused", "time", "heads", "odd"])
+@pytest.mark.parametrize("shape", [(3, 150, 4, 2, 64, 64), (2, 70, 6, 3, 128, 128), (5, 9, 4, 4, 40, 72)], ids=str)
+def test_prompt_lengths_pool_and_layouts(ops, shape, layout, dtype):
+    """Sequences of uneven lengths (none, one, all tokens) that go on from states in any order; rows behind them are not read."""
+    b, t, h, hk, dk, dv = shape
+    q, k, v = make(*shape, dtype, layout)
+    lengths = torch.tensor([t, 0, 1, t // 2, 3][:b], device="cuda", dtype=torch.int32)
+    pool = torch.randn(b + 4, h, dk, dv, device="cuda")
+    slots = torch.randperm(b + 4, device="cuda")[:b].to(torch.int32)
+    start, before = pool[slots.long()].clone(), pool.clone()
+    want = recurrence(q, k, v, decays(h), 0.3, start, lengths)
+    for i in range(b):
+        for x in (q, k, v):
+            x[i, int(lengths[i]):] = math.nan
+    out, state = ops.linear_attention(q, k, v, decays(h), scale=0.3, state=pool, slots=slots, lengths=lengths)
+    assert state.data_ptr() == pool.data_ptr()
+    check_attention(out, pool[slots.long()], want, dtype, t, dk)
+    for i in range(b):
+        assert bool((out[i, int(lengths[i]):] == 0).all())
+    others = torch.ones(b + 4, dtype=torch.bool, device="cuda")
+    others[slots.long()] = False
+    assert torch.equal(pool[others], before[others])
+    assert torch.equal(pool[slots[1].long()], start[1])  # (no tokens: the state as it was)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("shape", [(1, 1, 1, 1, 1), (1, 16, 16, 128, 128), (33, 12, 4, 72, 40), (7, 4, 2, 128, 17), (70, 8, 8, 64, 64)], ids=str)
+def test_step(ops, shape, dtype):
+    b, h, hk, dk, dv = shape
+    q, k, v = (x[:, 0] for x in make(b, 1, h, hk, dk, dv, dtype, "fused"))
+    pool = torch.randn(2 * b + 1, h, dk, dv, device="cuda")
+    slots = torch.randperm(2 * b + 1, device="cuda")[:b].to(torch.int32)
+    want = recurrence(q[:, None], k[:, None], v[:, None], decays(h), 0.5, pool[slots.long()], torch.ones(b, device="cuda"))
+    before = pool.clone()
+    out = ops.linear_attention_step(q, k, v, decays(h), pool, scale=0.5, slots=slots)
+    check_attention(out[:, None], pool[slots.long()], want, dtype, 1, dk)
+    others = torch.ones(2 * b + 1, dtype=torch.bool, device="cuda")
+    others[slots.long()] = False
+    assert torch.equal(pool[others], before[others])
+
+
+@pytest.mark.parametrize("tokens", [1, 5, 200])
+def test_slots_that_are_none_out_of_range_or_named_twice(ops, tokens):
+    import functs_b200
+    b, h, d = 6, 2, 64
+    q, k, v = make(b, tokens, h, h, d, d, BF16)
+    pool = torch.randn(4, h, d, d, device="cuda")
+    start = pool.clone()
+    slots = torch.tensor([2, -1, 4, 2, 0, -7], device="cuda", dtype=torch.int32)
+    status = ops.new_status("cuda")
+    out, _ = ops.linear_attention(q, k, v, decays(h), state=pool, slots=slots, status=status)
+    live = torch.tensor([0, 4], device="cuda")
+    want = recurrence(q[live], k[live], v[live], decays(h), 1.0, start[[2, 0]], torch.full((2,), tokens, device="cuda"))
+    check_attention(out[live], pool[[2, 0]], want, BF16, tokens, d)
+    assert bool((out[[1, 2, 3, 5]] == 0).all()) and torch.equal(pool[[1, 3]], start[[1, 3]])
+    assert int(status) == 4 | 8
+    with pytest.raises(functs_b200.FunctsB200Error, match="out of range; an index was named twice"):
+        ops.raise_on_status(status, "linear_attention")
+    ok = ops.new_status("cuda")
+    ops.linear_attention(q, k, v, decays(h), state=pool, slots=torch.tensor([3, -1, 1, 0, -1, 2], device="cuda", dtype=torch.int32), status=ok)
+    assert int(ok) == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("tokens", [5, 150])
+def test_values_that_are_not_finite(ops, tokens, dtype):
+    """They reach the outputs from their token on, in their own channels or rows, and nothing before them."""
+    b, h, d, at = 1, 2, 64, tokens - 3
+    for which in range(3):
+        qkv = [x.clone() for x in make(b, tokens, h, h, d, d, dtype)]
+        clean, clean_state = ops.linear_attention(*qkv, decays(h))
+        qkv[which][0, at, 0, 7] = (math.nan, math.inf, -math.inf)[which]
+        out, state = ops.linear_attention(*qkv, decays(h))
+        assert torch.equal(out[:, :at], clean[:, :at]) and torch.equal(out[:, :, 1], clean[:, :, 1])
+        bad = ~torch.isfinite(out[0, at:, 0])
+        if which == 0:  # a query: its own row alone
+            assert bool(bad[0].all()) and torch.equal(out[:, at + 1:], clean[:, at + 1:]) and torch.equal(state, clean_state)
+        elif which == 1:  # a key: a row of the state, so every channel from here on
+            assert bool(bad.all()) and bool((~torch.isfinite(state[0, 0, 7])).all())
+        else:  # a value: its channel from here on
+            assert bool(bad[:, 7].all()) and not bool(bad[:, :7].any()) and not bool(bad[:, 8:].any())
+            assert bool((~torch.isfinite(state[0, 0, :, 7])).all()) and bool(torch.isfinite(state[0, 0, :, :7]).all())
+
+
+@pytest.mark.parametrize("tokens", [3, 100])
+def test_decays_at_their_ends(ops, tokens):
+    """No decay, one that forgets at once (-inf), and one whose powers leave the range of fp32."""
+    g = torch.tensor([0.0, -math.inf, -1e4, -60.0], device="cuda")
+    q, k, v = make(2, tokens, 4, 4, 64, 64, BF16)
+    state = torch.randn(2, 4, 64, 64, device="cuda")
+    want = recurrence(q, k, v, g, 1.0, state, torch.full((2,), tokens, device="cuda"))
+    out, state = ops.linear_attention(q, k, v, g, state=state)
+    check_attention(out, state, want, BF16, tokens, 64)
+
+
+def test_no_tokens_and_no_sequences(ops):
+    q, k, v = make(2, 0, 2, 2, 16, 16, F32)
+    state = torch.randn(2, 2, 16, 16, device="cuda")
+    before = state.clone()
+    out, _ = ops.linear_attention(q, k, v, decays(2), state=state)
+    assert out.shape == (2, 0, 2, 16) and torch.equal(state, before)
+    assert float(ops.linear_attention(q, k, v, decays(2))[1].abs().sum()) == 0.0
+    q, k, v = make(0, 5, 2, 2, 16, 16, F32)
+    out, state = ops.linear_attention(q, k, v, decays(2))
+    assert out.shape == (0, 5, 2, 16) and state.shape == (0, 2, 16, 16)
+
+
+@pytest.mark.parametrize("tokens", [4, 140])
+def test_output_given_as_a_part_of_a_larger_one(ops, tokens):
+    q, k, v = make(2, tokens, 3, 3, 64, 40, BF16)
+    room = torch.full((2, tokens + 2, 5, 48), 7.0, device="cuda", dtype=BF16)
+    part = room[:, 1:-1, 1:4, 3:43]
+    out, _ = ops.linear_attention(q, k, v, decays(3), out=part)
+    assert out.data_ptr() == part.data_ptr() and torch.equal(part, ops.linear_attention(q, k, v, decays(3))[0])
+    room[:, 1:-1, 1:4, 3:43] = 7.0
+    assert bool((room == 7).all())
+
+
+def test_large_pool(ops):
+    """States behind the 2^31st element."""
+    h, d = 16, 128
+    n = 2 ** 31 // (h * d * d) + 2
+    pool = torch.empty(n, h, d, d, device="cuda")
+    for tokens in (1, 90):
+        q, k, v = make(1, tokens, h, h, d, d, BF16)
+        pool[n - 1] = 1.0
+        pool[0] = 2.0
+        slots = torch.tensor([n - 1], device="cuda", dtype=torch.int32)
+        want = recurrence(q, k, v, decays(h), 0.1, pool[n - 1:], torch.full((1,), tokens, device="cuda"))
+        out, _ = ops.linear_attention(q, k, v, decays(h), scale=0.1, state=pool, slots=slots)
+        check_attention(out, pool[n - 1:], want, BF16, tokens, d)
+        assert bool((pool[0] == 2).all())
+
+
+def test_attention_refuses(ops):
+    q, k, v = make(2, 3, 4, 2, 16, 16, F32)
+    g, state = decays(4), torch.zeros(2, 4, 16, 16, device="cuda")
+    i32 = lambda *x: torch.tensor(x, device="cuda", dtype=torch.int32)  # noqa: E731
+    call = ops.linear_attention
+    for error, match, f in [
+        (ValueError, "CUDA tensor", lambda: call(q.cpu(), k, v, g)),
+        (ValueError, "CUDA tensor", lambda: call(q, k.cpu(), v, g)),
+        (TypeError, "q must be torch.float32", lambda: call(q.double(), k.double(), v.double(), g)),
+        (TypeError, "k must be", lambda: call(q, k.half(), v, g)),
+        (TypeError, "log_decay must be", lambda: call(q, k, v, g.half())),
+        (ValueError, "log_decay must be of sizes", lambda: call(q, k, v, g[:2])),
+        (ValueError, "multiple of the key", lambda: call(q[:, :, :3], k, v, g[:3])),
+        (ValueError, "fit one another", lambda: call(q, k[:, :2], v, g)),
+        (ValueError, "fit one another", lambda: call(q, k[..., :8], v, g)),
+        (ValueError, "1 to 128 channels", lambda: call(*[torch.zeros(1, 1, 1, 129, device="cuda")] * 3, g[:1])),
+        (ValueError, "state must be a contiguous", lambda: call(q, k, v, g, state=state[..., :8])),
+        (ValueError, "without slots", lambda: call(q, k, v, g, state=state[:1])),
+        (ValueError, "give one", lambda: call(q, k, v, g, slots=i32(0, 1))),
+        (TypeError, "slots must be", lambda: call(q, k, v, g, state=state, slots=torch.tensor([0, 1], device="cuda"))),
+        (ValueError, "slots must be of sizes", lambda: call(q, k, v, g, state=state, slots=i32(0))),
+        (ValueError, "lengths must be of sizes", lambda: call(q, k, v, g, lengths=i32(0, 1, 2))),
+        (ValueError, "out must not share", lambda: call(q, k, v, g, out=q)),
+        (ValueError, "overlap itself", lambda: call(q, k, v, g, out=torch.zeros(1, 1, 4, 16, device="cuda").expand(2, 3, 4, 16))),
+        (ValueError, "status must be", lambda: call(q, k, v, g, status=torch.zeros(1, device="cuda"))),
+        (NotImplementedError, "gradient", lambda: call(q.clone().requires_grad_(), k, v, g)),
+        (ValueError, r"\[B, heads, channels\]", lambda: ops.linear_attention_step(q, k, v, g, state)),
+    ]:
+        with pytest.raises(error, match=match):
+            f()
+    with torch.no_grad():
+        call(q.clone().requires_grad_(), k, v, g)
+
+
+def test_prompt_then_tokens_is_the_whole_prompt(ops):
+    """A prompt, then single tokens from the pool it left (captured into a graph and replayed, with a second one that shares nothing), and
+    the log probabilities of what they answer: the same as one prompt of all tokens."""
+    b, t, n, h, d, vocab = 3, 100, 6, 4, 64, 1000
+    q, k, v = make(b, t + n, h, h, d, d, BF16, "fused")
+    slots = torch.tensor([4, 0, 2], device="cuda", dtype=torch.int32)
+    w = torch.randn(h * d, vocab, device="cuda", dtype=BF16) * 0.3
+    whole, end = ops.linear_attention(q, k, v, decays(h), scale=d ** -0.5)
+    pool = torch.zeros(5, h, d, d, device="cuda")
+    ops.linear_attention(q[:, :t], k[:, :t], v[:, :t], decays(h), scale=d ** -0.5, state=pool, slots=slots)
+    one = [torch.empty(b, x.size(2), x.size(3), device="cuda", dtype=BF16) for x in (q, k, v)]
+    ids = torch.zeros(b, dtype=torch.int64, device="cuda")
+    g = decays(h)
+
+    def step(pool):
+        o = ops.linear_attention_step(*one, g, pool, scale=d ** -0.5, slots=slots)
+        return (o,) + tuple(ops.token_logprobs(o.flatten(1) @ w, ids, top=3))
+
+    spare = pool.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(spare.clone())
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for p in (pool, spare):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            got = step(p)
+        graphs.append(got)
+    for i in range(n):
+        for x, y in zip(one, (q, k, v)):
+            x.copy_(y[:, t + i])
+        ids.copy_((whole[:, t + i].flatten(1) @ w).argmax(1))
+        graphs[0].replay()
+        graphs[2].replay()
+        for got in (graphs[1], graphs[3]):
+            o, lp, entropy, top_lp, top_ids = got
+            # one more rounding of what the prompt carried: two halves of a step apart at most, beside what is carried
+            assert float((o.double() - whole[:, t + i].double()).norm()) <= 2 * 2.0 ** -8 * float(whole[:, t + i].double().norm())
+            want = torch.log_softmax((o.flatten(1) @ w).double(), 1)
+            assert torch.allclose(lp.double(), want.gather(1, ids[:, None])[:, 0], atol=1e-4)
+            assert torch.equal(top_ids, torch.sort((o.flatten(1) @ w).float(), dim=1, descending=True, stable=True)[1][:, :3])
+    for p in (pool, spare):
+        assert float((p[slots.long()] - end).norm()) <= 2e-6 * float(end.norm())
+
+
+def test_two_streams_at_once(ops):
+    """Calls on two streams do not touch one another."""
+    cases = [make(2, 300, 4, 4, 128, 128, BF16, seed=s) for s in (1, 2)]
+    want = [ops.linear_attention(*c, decays(4)) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for c, s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                got.append(ops.linear_attention(*c, decays(4)))
+        torch.cuda.synchronize()
+        for (o, s), (wo, ws) in zip(got, want):
+            assert torch.equal(o, wo) and torch.equal(s, ws)
+
+
+# ---- log probabilities -----------------------------------------------------------------------------------------------
+
+
+def check_logprobs(ops, logits, tokens, top):
+    """A sum of V powers: each within 2^-22 of its value and, for its exponent, |d| 2^-24 (d within 2^8 of the maximum, beyond that
+    it is nothing), at most V / 64 additions in one thread and 32 more above.  The logarithm turns that into an absolute error."""
+    rows, vocab = logits.shape
+    x = logits.double()
+    want_ids = torch.sort(x, dim=1, descending=True, stable=True)[1][:, :top]
+    lp, entropy, top_lp, top_ids = ops.token_logprobs(logits, tokens, top=top)
+    assert lp.dtype == entropy.dtype == top_lp.dtype == F32 and top_ids.dtype == torch.int64 and top_ids.shape == (rows, top)
+    assert torch.equal(top_ids, want_ids)
+    p = torch.log_softmax(x, dim=1)
+    eps = 2.0 ** -22 + (vocab / 64 + 32 + 2 ** 8) * 2.0 ** -24
+    tol = lambda want: eps + 2.0 ** -24 * want.abs()  # noqa: E731
+    want = p.gather(1, tokens[:, None])[:, 0]
+    fine = torch.isfinite(want)
+    assert torch.equal(lp[~fine].double(), want[~fine])
+    assert bool(((lp.double() - want).abs() <= tol(want))[fine].all())
+    want = p.gather(1, want_ids)
+    fine = torch.isfinite(want)
+    assert torch.equal(top_lp[~fine].double(), want[~fine])
+    assert bool(((top_lp.double() - want).abs() <= tol(want))[fine].all())
+    want = -torch.where(p > -math.inf, p.exp() * p, 0.0).sum(1)
+    # two sums of that kind, one of them of terms |d| e^d
+    assert bool(((entropy.double() - want).abs() <= 2 * eps * (1 + want) + 2.0 ** -24 * want).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (1, 3, 3), (3, 64, 64), (2, 100, 50), (5, 369, 5), (1, 32000, 5), (2, 32001, 64), (40, 4097, 7),
+                                            (300, 5003, 20), (3, 262144, 20), (200, 1000, 0)])
+def test_logprobs(ops, rows, vocab, top, dtype):
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    logits = (torch.randn(rows, vocab, generator=g, device="cuda") * 3).to(dtype)
+    check_logprobs(ops, logits, torch.randint(0, vocab, (rows,), generator=g, device="cuda"), top)
+
+
+@pytest.mark.parametrize("rows", [2, 300])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("kind", ["constant", "two values", "rising", "falling", "few finite", "one finite", "few threads", "shifted", "huge range", "zeros"])
+def test_logprobs_of_rows_that_are_hard_to_select_from(ops, kind, dtype, rows):
+    vocab, top = 40000, 20
+    at = torch.arange(vocab, device="cuda", dtype=F32)
+    x = torch.randn(rows, vocab, device="cuda")
+    if kind == "constant":
+        x = torch.full((rows, vocab), -3.5, device="cuda")
+    elif kind == "two values":
+        x = torch.where(x > 1.5, 1.0, 0.25)
+    elif kind == "rising":
+        x = (at / 1000).repeat(rows, 1)
+    elif kind == "falling":
+        x = (-at / 1000).repeat(rows, 1)
+    elif kind == "few finite":
+        x[:, 7:] = -math.inf
+    elif kind == "one finite":
+        x = torch.full((rows, vocab), -math.inf, device="cuda")
+        x[:, 31234] = 2.0
+    elif kind == "few threads":  # the large values all sit where a handful of threads read
+        x = torch.where((at // 4) % 128 < 4, x.abs() + 10, x)
+    elif kind == "shifted":
+        x = x * 5 + 1000
+    elif kind == "huge range":
+        x = x * 1e4
+    elif kind == "zeros":  # of both signs: equal, the lowest ids first
+        x = torch.where(x > 0, 0.0, -0.0)
+    check_logprobs(ops, x.to(dtype).contiguous(), torch.randint(0, vocab, (rows,), device="cuda"), top)
+
+
+@pytest.mark.parametrize("vocab", [50, 9000])
+def test_logprobs_of_rows_without_a_distribution(ops, vocab):
+    x = torch.randn(6, vocab, device="cuda")
+    x[0] = -math.inf
+    x[1, 17] = math.nan
+    x[2, 23] = math.inf
+    x[3, 40] = -math.nan
+    tokens = torch.tensor([3, 4, 23, 40, 5, 49], device="cuda")
+    lp, entropy, top_lp, top_ids = ops.token_logprobs(x, tokens, top=4)
+    assert float(lp[0]) == -math.inf and float(entropy[0]) == 0.0 and bool((top_lp[0] == -math.inf).all()) and top_ids[0].tolist() == [0, 1, 2, 3]
+    for r, first in ((1, 17), (2, 23), (3, 40)):
+        assert math.isnan(float(lp[r])) and math.isnan(float(entropy[r])) and bool(torch.isnan(top_lp[r]).all()) and int(top_ids[r, 0]) == first
+    check_logprobs(ops, x[4:], tokens[4:], 4)
+
+
+def test_logprobs_tokens_that_are_none_or_out_of_range(ops):
+    x = torch.randn(4, 100, device="cuda")
+    status = ops.new_status("cuda")
+    lp, entropy, _, _ = ops.token_logprobs(x, torch.tensor([-1, 100, 5, -100], device="cuda"), status=status)
+    assert float(lp[0]) == 0.0 == float(lp[3]) and math.isnan(float(lp[1])) and int(status) == 4
+    assert bool((entropy > 0).all())
+    ok = ops.new_status("cuda")
+    ops.token_logprobs(x, torch.tensor([-1, 99, 5, 0], device="cuda"), status=ok)
+    assert int(ok) == 0
+
+
+def test_logprobs_rows_in_a_larger_tensor(ops):
+    """Rows apart, off every 16-byte boundary, and behind the 2^31st element."""
+    for dtype in (F32, F16, BF16):
+        big = torch.randn(7, 1033, device="cuda").to(dtype)
+        for first in range(9):
+            check_logprobs(ops, big[:, first:first + 1001], torch.arange(7, device="cuda"), 9)
+    store = torch.empty(2 ** 31 + 5000, device="cuda", dtype=BF16)
+    x = store.as_strided((2, 3000), (2 ** 31, 1), 11)
+    x.copy_(torch.randn(2, 3000, device="cuda"))
+    check_logprobs(ops, x, torch.tensor([5, 2999], device="cuda"), 5)
+
+
+def test_logprobs_refuses(ops):
+    x, t = torch.randn(3, 50, device="cuda"), torch.zeros(3, device="cuda", dtype=torch.int64)
+    for error, match, f in [
+        (ValueError, "CUDA tensor", lambda: ops.token_logprobs(x.cpu(), t)),
+        (ValueError, "CUDA tensor", lambda: ops.token_logprobs(x, t.cpu())),
+        (TypeError, "logits must be torch.float32", lambda: ops.token_logprobs(x.double(), t)),
+        (TypeError, "tokens must be", lambda: ops.token_logprobs(x, t.int())),
+        (ValueError, "rows, vocab", lambda: ops.token_logprobs(x[0], t)),
+        (ValueError, "rows, vocab", lambda: ops.token_logprobs(x[:, :0], t)),
+        (ValueError, "tokens must be of sizes", lambda: ops.token_logprobs(x, t[:2])),
+        (ValueError, "top must be", lambda: ops.token_logprobs(x, t, top=51)),
+        (ValueError, "top must be", lambda: ops.token_logprobs(x, t, top=-1)),
+        (ValueError, "top must be", lambda: ops.token_logprobs(torch.randn(3, 500, device="cuda"), t, top=65)),
+        (NotImplementedError, "gradient", lambda: ops.token_logprobs(x.clone().requires_grad_(), t)),
+    ]:
+        with pytest.raises(error, match=match):
+            f()
+    lp, entropy, top_lp, top_ids = ops.token_logprobs(x[:0], t[:0], top=2)
+    assert lp.shape == (0,) and top_ids.shape == (0, 2)

@@ -1,0 +1,65 @@
+"""Refusals of the sequence operators that need no GPU: wrong tensors at the Python entries, wrong arguments at the C ones (nothing is
+launched, pointers are never followed)."""
+import ctypes
+
+import pytest
+import torch
+
+
+def args(**over):
+    from functs_b200 import _lib
+    p = 4096
+    a = _lib.LinearAttentionArgs(dtype=2, batch=2, tokens=3, heads=4, kv_heads=2, dk=16, dv=16, num_slots=2, q=p, k=p, v=p, out=p, log_decay=p,
+                                 state_in=p, state_out=p, scale=1.0)
+    for name, value in over.items():
+        setattr(a, name, value)
+    return a
+
+
+@pytest.mark.parametrize("over,match", [
+    ({"dtype": 3}, "dtype"), ({"dtype": -1}, "dtype"), ({"batch": -1}, "negative"), ({"tokens": -1}, "negative"), ({"heads": 0}, "multiple"),
+    ({"kv_heads": 3}, "multiple"), ({"kv_heads": 0}, "multiple"), ({"dk": 0}, "dk"), ({"dk": 129}, "dk"), ({"dv": 129}, "dv"),
+    ({"num_slots": 3}, "as many states"), ({"num_slots": -1, "slots": 4096}, "negative"), ({"log_decay": None}, "null pointer"),
+    ({"state_out": None}, "null pointer"), ({"q": None}, "null pointer"), ({"v": None}, "null pointer"), ({"out": None}, "null pointer"),
+])
+def test_linear_attention_arguments(over, match):
+    from functs_b200 import _lib
+    assert _lib.lib.functs_b200_linear_attention(ctypes.byref(args(**over)), None, None) == -1
+    assert match in _lib.last_error()
+
+
+def test_linear_attention_of_nothing():
+    from functs_b200 import _lib
+    assert _lib.lib.functs_b200_linear_attention(ctypes.byref(args(batch=0, num_slots=0)), None, None) == 0
+    assert _lib.lib.functs_b200_linear_attention(None, None, None) == -1
+
+
+@pytest.mark.parametrize("at,value,match", [
+    (1, 3, "dtype"), (4, -1, "rows"), (5, 0, "vocab"), (6, -1, "top"), (6, 65, "top"), (6, 11, "top"), (0, None, "null pointer"), (3, None, "null pointer"),
+    (7, None, "null pointer"), (8, None, "null pointer"), (9, None, "null pointer"), (10, None, "null pointer"), (0, 4097, "boundary"),
+])
+def test_token_logprobs_arguments(at, value, match):
+    from functs_b200 import _lib
+    p = 4096
+    a = [p, 2, 10, p, 1, 10, 5, p, p, p, p, None, None]
+    a[at] = value
+    if match == "top" and value == 65:
+        a[5] = 100
+    assert _lib.lib.functs_b200_token_logprobs(*a) == -1
+    assert match in _lib.last_error()
+
+
+def test_token_logprobs_of_nothing():
+    from functs_b200 import _lib
+    assert _lib.lib.functs_b200_token_logprobs(None, 0, 10, None, 0, 10, 5, None, None, None, None, None, None) == 0
+
+
+def test_there_is_no_cpu_path():
+    from functs_b200 import ops
+    x = torch.zeros(1, 2, 3, 4)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.linear_attention(x, x, x, torch.zeros(3))
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.linear_attention_step(x[0], x[0], x[0], torch.zeros(3), torch.zeros(2, 3, 4, 4))
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.token_logprobs(torch.zeros(2, 3), torch.zeros(2, dtype=torch.int64))
