@@ -23,6 +23,7 @@ SOURCES = [
     "kernels_lstm_tc.cu",
     "kernels_lstm_rec.cu",
     "kernels_linattn.cu",
+    "kernels_linattn_tc.cu",
     "kernels_logprobs.cu",
     "no_alloc.cu",
     "kernels_generic.cu",

@@ -154,6 +154,7 @@ extern "C" int functs_b200_linear_attention(const functs_b200_linear_attention_a
     FB_REQUIRE(a.tokens == 0 || (a.q != nullptr && a.k != nullptr && a.v != nullptr && a.out != nullptr), "linear_attention: null pointer");
     (void)scratch;
     const cudaStream_t st = as_stream(stream);
+    if (a.tokens > 32) return launch_linattn_chunk(a, st);
     if (a.dtype == FB_DTYPE_F32) return launch_recurrent<float>(a, st);
     if (a.dtype == FB_DTYPE_F16) return launch_recurrent<__half>(a, st);
     return launch_recurrent<__nv_bfloat16>(a, st);

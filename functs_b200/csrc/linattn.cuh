@@ -12,6 +12,8 @@ using LinArgs = functs_b200_linear_attention_args;
 
 constexpr int kLinMaxDim = 128;
 
+int launch_linattn_chunk(const LinArgs& a, cudaStream_t st);  // kernels_linattn_tc.cu
+
 #ifdef __CUDACC__
 
 __device__ __forceinline__ float lin_float(float x) { return x; }
