@@ -143,7 +143,7 @@ extern "C" int functs_b200_linear_attention(const functs_b200_linear_attention_a
     FB_REQUIRE(args != nullptr, "linear_attention: null pointer");
     const LinArgs& a = *args;
     FB_REQUIRE(a.dtype >= FB_DTYPE_F32 && a.dtype <= FB_DTYPE_BF16, "linear_attention: unknown dtype %d", a.dtype);
-    FB_REQUIRE(a.batch >= 0 && a.tokens >= 0 && a.heads > 0 && a.kv_heads > 0 && a.heads % a.kv_heads == 0,
+    FB_REQUIRE(a.batch >= 0 && a.tokens >= 0 && a.tokens <= (1 << 30) && a.heads > 0 && a.kv_heads > 0 && a.heads % a.kv_heads == 0,
                "linear_attention: sizes must not be negative, and heads (%d) a multiple of kv_heads (%d)", a.heads, a.kv_heads);
     FB_REQUIRE(a.dk >= 1 && a.dk <= kLinMaxDim && a.dv >= 1 && a.dv <= kLinMaxDim, "linear_attention: dk (%d) and dv (%d) must be 1 .. %d", a.dk,
                a.dv, kLinMaxDim);

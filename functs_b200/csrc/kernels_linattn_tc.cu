@@ -3,20 +3,30 @@
 // Within a chunk whose first token follows the state S (l = decay, i and j count from 0, n = its tokens):
 //   out_i = scale * ( l^(i+1) S^T q_i  +  sum_{j <= i} l^(i-j) (q_i . k_j) v_j )          S' = l^n S + sum_j l^(n-1-j) k_j v_j^T
 // which is four products:  G = Q K^T,  X = S^T Q^T,  Y = V^T P^T with P = G masked and decayed,  U = K^T W with W = decayed V.
-// S stays in registers in fp32 and is decayed and added there (the tensor core truncates when it adds); the decay is a sum of two floats,
-// because its rounding would be the same for every chunk.
+// S is decayed and added to in fp32 outside the tensor core (which truncates when it adds); the decay is a sum of two floats, because
+// its rounding would be the same for every chunk.
 //
-// Operands have 8 bits, so what has more is a sum of parts: S and P of two (what they make is rounded to 16 bits at once, 2^-17 apart),
+// Operands have 8 bits, so what has more is a sum of parts: S and P of two (what they make is rounded to 16 bits at once, 2^-16 apart),
 // W of three (it makes the state, which is fp32).  Q, K and V are their own part in bf16, two in fp16 (exact), three in fp32; products of
 // parts that are below the result's precision are left out, and the small ones are added first.
 //
-// One layout serves all products: core matrices of 8 tokens x 16 bytes (8 channels), channel groups 1024 bytes apart.  Read along channels
-// a tile is a K-major operand of rows = tokens, read along tokens an MN-major operand of rows = channels, with the two strides of the
-// descriptor exchanged.  All products have M = 128 rows; where there are 64, the others are whatever follows in shared memory, and their
-// results, which are rows of their own, are not looked at.
+// X, Y and U are formed transposed, with the channels of V as rows, so that S^T is an operand in TMEM (in shared memory it cost 128 KB of
+// writes and reads per chunk, and shared memory's bandwidth was the bound), and stores of S and of the outputs are coalesced.  All products
+// have M = 128 rows; where there are 64, the others are whatever follows in memory, and their results, which are rows of their own, are not
+// looked at.  Q, K and V lie as rows of 64 channels (128 bytes, swizzled), read along channels (K-major) or along tokens (MN-major); W and P,
+// which threads write, as core matrices of 8 rows x 16 bytes.
+//
+// Roles, so that loads, conversions, products and stores of neighbouring chunks overlap (one CTA per SM):
+//   S   8 warps: S' = l^n S + U in TMEM, a channel of V per thread, half of the channels of K; S' as operand parts
+//   W   W from V (and, where tiles cannot be had by TMA, or are split into parts, the tiles themselves)
+//   O   the outputs from X and Y
+//   P   P from G: four warps (there are 64 rows); beside them one warp that issues the products, in the order U, G, X, Y, so that there is
+//       always one to run while the threads are at the next, and one that issues the copies
 //
 // NaN and infinities: a masked entry of P is 0 by selection, but 0 * V is not 0 for a V that is not finite, so such entries are taken as 0 in
 // Y (not in W) and the outputs of their channel, from their token on, are set to NaN.
+#include <cuda.h>
+
 #include <type_traits>
 
 #include "linattn.cuh"
@@ -24,36 +34,56 @@
 
 namespace fb {
 
-constexpr int kLtThreads = 256;
 constexpr int kLtChunk = 64;
-constexpr uint32_t kLtWaitLimit = 4000000u;
-constexpr uint32_t kLtTmemCols = 512;
-// TMEM columns of the four products
-constexpr uint32_t kLtG = 0, kLtX = 64, kLtY = 128, kLtU = 192;
+constexpr int kLtWarpsS = 8, kLtWarpsP = 8;  // (of the P group four make P, one issues products, one copies)
+constexpr uint32_t kLtWaitLimit = 1000000u;
+constexpr int kLtMarks = 4;  // chunks whose marks of values that are not finite are kept
+// TMEM columns: U, X, Y (and, before it, G), S^T in fp32 and as two operand parts of DK / 2 columns, or as three parts, which are exact
+constexpr uint32_t kLtU = 0, kLtX = 128, kLtY = 192, kLtS = 256, kLtTmemCols = 512;
 
 template <typename T, int DK_, int DV_>
 struct LtCfg {
     static constexpr int DK = DK_, DV = DV_;
-    static constexpr bool kAsync = std::is_same<T, __nv_bfloat16>::value;
-    static constexpr int NX = kAsync ? 1 : std::is_same<T, __half>::value ? 2 : 3;  // parts of q, k, v
-    static constexpr int NS = std::is_same<T, float>::value ? 3 : 2;                // parts of S and P
-    static constexpr int NW = 3;                                                    // parts of W
-    static constexpr int kStages = kAsync ? 2 : 1;
-    static constexpr int kTileK = kLtChunk * DK * 2, kTileV = kLtChunk * DV * 2, kPartS = DK * DV * 2, kPartP = kLtChunk * kLtChunk * 2;
+    static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    static constexpr int NX = kBf16 ? 1 : std::is_same<T, __half>::value ? 2 : 3;  // parts of q, k, v
+    static constexpr int NS = std::is_same<T, float>::value ? 3 : 2;               // parts of S and P
+    static constexpr int NW = 3;                                                   // parts of W
+    static constexpr int kStages = kBf16 ? 2 : 1;                                  // of Q, K and V, and of W
+    static constexpr int kWarpsW = kBf16 ? 4 : 8, kWarpsO = kBf16 ? 8 : 4;
+    static constexpr int kFirstW = kLtWarpsS, kFirstO = kFirstW + kWarpsW, kFirstP = kFirstO + kWarpsO, kThreads = 32 * (kFirstP + kLtWarpsP);
+    static_assert(kFirstO % 4 == 0 && kFirstP % 4 == 0, "a warp's TMEM lanes go by its number");
+    static constexpr int kTileK = kLtChunk * DK * 2, kTileV = kLtChunk * DV * 2, kPartP = kLtChunk * kLtChunk * 2;
     static constexpr int kStage = NX * (2 * kTileK + kTileV);
-    static constexpr int oS = kStages * kStage, oW = oS + NS * kPartS, oP = oW + NW * kTileV, oMisc = oP + NS * kPartP;
+    static constexpr int oK = NX * kTileK, oV = 2 * NX * kTileK;  // in a stage, behind Q
+    static constexpr int oW = kStages * kStage, oP = oW + kStages * NW * kTileV, oMisc = oP + NS * kPartP;
+    static constexpr uint32_t kParts = NS == 3 ? kLtS : kLtS + 128;  // TMEM columns of the parts of S^T
 };
 
 struct LtMisc {
-    uint64_t bar_g, bar_u, bar_y;
+    uint64_t full[2], empty[2], w_full[2], w_free[2];  // stages
+    uint64_t g_full, u_full, u_free, s_full, x_full, p_full, y_full, xy_free;
     uint32_t tmem;
-    int dead;          // a wait ran out
-    int any_bad;       // the chunk has a V that is not finite
+    int dead;                                      // a wait ran out
     int b;
-    float power_lo;    // what power[64] leaves of decay^64
-    float power[kLtChunk + 1];
-    int first_bad[128];  // per channel: the first such token of the chunk
+    float power_next, power_gap, power_off;        // the float beyond power[64] on decay^64's side, how far, and how far decay^64 is (relative)
+    float power[kLtChunk + 4], scaled[kLtChunk + 4];  // decay^i, scale * decay^i
+    __align__(16) float scaled_next[kLtChunk];        // scale * decay^(i+1)
+    uint2 weight[kLtChunk];                        // decay^i as three bf16 parts, each twice: w0 w0, w1 w1 (w2 below)
+    uint32_t weight2[kLtChunk];
+    int any_bad[kLtMarks];                         // 1 + the last chunk that marked some
+    int first_bad[kLtMarks][128];                  // per channel: (how far the chunk is from 2^24, the first such token)
 };
+
+struct LtPlan {
+    int tiles;       // of DV columns
+    int segs;        // parts of a sequence
+    int seg_tokens;  // a multiple of the chunk
+    int mode;        // 0: whole sequences; 1: the state that each part adds, 2: outputs of the parts
+    bool aligned;
+    float* states;   // [batch * heads][segs][dk][dv]
+};
+
+// ---- small pieces ---------------------------------------------------------------------------------------------------
 
 __device__ __forceinline__ void lt_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
     asm volatile(
@@ -61,33 +91,127 @@ __device__ __forceinline__ void lt_mma(uint32_t d, uint64_t a, uint64_t b, uint3
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
         : "memory");
 }
+// One lane of a whole warp.  (Where the compiler knows that one thread alone is active, it keeps descriptors in uniform registers: 2094
+// cycles to issue a chunk's 44 products instead of 2732 behind `lane == 0`.)
+__device__ __forceinline__ bool lt_elect() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+// tiles of rows of 128 bytes with the 128-byte swizzle: the 8-row groups `sbo` apart, the next 64 channels (MN-major) `lbo`
+__device__ __forceinline__ uint64_t lt_desc_swizzled(uint32_t addr, uint32_t lbo, uint32_t sbo) { return make_smem_desc(addr, lbo, sbo) | (2ull << 61); }
 
-__device__ __forceinline__ uint32_t lt_pack(float a, float b) {
-    const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&p);
+__device__ __forceinline__ void lt_mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+        : "memory");
+}
+// 16 TMEM columns of the thread's lane; 8 columns
+__device__ __forceinline__ void lt_ld(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void lt_ld(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+// (the values are operands of the wait, so that nothing uses them before it)
+__device__ __forceinline__ void lt_ld_wait(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+}
+__device__ __forceinline__ void lt_ld_wait(uint32_t (&r)[8]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])::"memory");
+}
+__device__ __forceinline__ void lt_st(uint32_t taddr, const float (&x)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"f"(x[0]),
+        "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]), "f"(x[8]), "f"(x[9]), "f"(x[10]), "f"(x[11]), "f"(x[12]),
+        "f"(x[13]), "f"(x[14]), "f"(x[15]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void lt_st(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void lt_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// One box of 64 channels x 64 tokens of a head.
+__device__ __forceinline__ void lt_tma(void* dst, const CUtensorMap* map, int channel, int token, int head, int seq, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(channel), "r"(token), "r"(head), "r"(seq), "r"(smem_u32(bar))
+        : "memory");
 }
 
-// Eight values as N parts of eight bf16 each; part p goes to at + p * stride.
+// Waits for a phase; gives up when the limit runs out or somebody else has given up.
+__device__ __forceinline__ bool lt_test(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool lt_wait_one(LtMisc& m, uint64_t* bar, uint32_t parity) {
+    for (uint32_t i = 0; i < kLtWaitLimit; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 63u) == 63u && *reinterpret_cast<volatile int*>(&m.dead)) return false;
+    }
+    *reinterpret_cast<volatile int*>(&m.dead) = 1;
+    return false;
+}
+__device__ __forceinline__ bool lt_wait(LtMisc& m, uint64_t* bar, uint32_t parity) {
+    const bool ok = lt_wait_one(m, bar, parity);
+    return __all_sync(kFullMask, ok) != 0;
+}
+// A warp's shared-memory writes are operands from here on: one arrival.
+__device__ __forceinline__ void lt_arrive_operands(uint64_t* bar, int lane) {
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+}
+// A warp has read its TMEM columns: one arrival.
+__device__ __forceinline__ void lt_arrive_read(uint64_t* bar, int lane) {
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+}
+
+// A bf16 part of two values: their upper halves, taken out of them; as the last part what is left, rounded.
+__device__ __forceinline__ uint32_t lt_part(float& x, float& y, bool last) {
+    if (last) {
+        const __nv_bfloat162 r = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+    const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+    x = __fsub_rn(x, __uint_as_float(a & 0xFFFF0000u));
+    y = __fsub_rn(y, __uint_as_float(b & 0xFFFF0000u));
+    return __byte_perm(a, b, 0x7632);
+}
+// Eight values as N parts of eight bf16 each, part p at `at + p * stride`.
 template <int N>
 __device__ __forceinline__ void lt_store_parts(unsigned char* at, int stride, float (&x)[8]) {
 #pragma unroll
     for (int p = 0; p < N; ++p) {
         uint32_t u[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = lt_pack(x[2 * i], x[2 * i + 1]);
+        for (int i = 0; i < 4; ++i) u[i] = lt_part(x[2 * i], x[2 * i + 1], p + 1 == N);
         *reinterpret_cast<uint4*>(at + p * stride) = make_uint4(u[0], u[1], u[2], u[3]);
-        if (p + 1 < N) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[2 * i] = __fsub_rn(x[2 * i], __uint_as_float(u[i] << 16));
-                x[2 * i + 1] = __fsub_rn(x[2 * i + 1], __uint_as_float(u[i] & 0xFFFF0000u));
-            }
-        }
     }
-}
-
-__device__ __forceinline__ void lt_cp16(void* dst, const void* src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
 }
 
 // Eight channels of one row in fp32, zeros behind `valid`.
@@ -108,28 +232,50 @@ __device__ __forceinline__ void lt_load8(const T* p, int valid, bool aligned, fl
         for (int i = 0; i < 8; ++i) x[i] = i < valid ? lin_float(p[i]) : 0.0f;
     }
 }
-
-// (8-channel group, token) of the `i`-th of a tile's 16-byte pieces: eight tokens beside one another, then four groups
-__device__ __forceinline__ void lt_piece(int i, int groups, int& group, int& token) {
-    const int lane = i & 31, w = i >> 5, per = groups / 4;  // groups is a multiple of 4
-    group = (w % per) * 4 + (lane >> 3);
-    token = (w / per) * 8 + (lane & 7);
+// Eight bf16 values times a weight of three parts, as three parts, in bf16 arithmetic: with a fused multiply-add that rounds once, products
+// and their errors are exact.  v w0 = p + r and v w1 = t0 + t1; r + t0 = s + e (D. Knuth, The Art of Computer Programming, volume 2, 4.2.2,
+// theorem B); the parts are p, s and e + t1 + v w2, which is rounded below 2^-25 of the product.
+__device__ __forceinline__ void lt_weigh(unsigned char* at, int stride, const uint32_t (&v)[4], uint2 w01, uint32_t w2) {
+    const auto bf = [](const uint32_t& u) { return *reinterpret_cast<const __nv_bfloat162*>(&u); };
+    uint32_t part[3][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 x = bf(v[i]), w0 = bf(w01.x), w1 = bf(w01.y);
+        const __nv_bfloat162 p = __hmul2_rn(x, w0), r = __hfma2(x, w0, __hneg2(p)), t0 = __hmul2_rn(x, w1), t1 = __hfma2(x, w1, __hneg2(t0));
+        const __nv_bfloat162 s = __hadd2_rn(r, t0), rest = __hsub2_rn(s, r);
+        const __nv_bfloat162 e = __hadd2_rn(__hsub2_rn(r, __hsub2_rn(s, rest)), __hsub2_rn(t0, rest));
+        const __nv_bfloat162 q = __hadd2_rn(e, __hfma2(x, bf(w2), t1));
+        part[0][i] = *reinterpret_cast<const uint32_t*>(&p);
+        part[1][i] = *reinterpret_cast<const uint32_t*>(&s);
+        part[2][i] = *reinterpret_cast<const uint32_t*>(&q);
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4*>(at + k * stride) = make_uint4(part[k][0], part[k][1], part[k][2], part[k][3]);
 }
-__device__ __forceinline__ int lt_offset(int group, int token) { return group * 1024 + (token >> 3) * 128 + (token & 7) * 16; }
+// (a swizzled tile: rows of 64 channels; a plain one: groups of 8 channels 1024 bytes apart)
+__device__ __forceinline__ int lt_swizzled(int group, int token) { return (group >> 3) * 8192 + token * 128 + (((group ^ token) & 7) << 4); }
+__device__ __forceinline__ int lt_plain(int group, int token) { return group * 1024 + (token >> 3) * 128 + (token & 7) * 16; }
+__device__ __forceinline__ bool lt_finite(float x) { return fabsf(x) <= 3.4028234663852886e38f; }
 
-template <typename T, int DK, int DV>
-__global__ void __launch_bounds__(kLtThreads, 1) linattn_chunk_kernel(const LinArgs a, int tiles, bool aligned) {
+// ---- the kernel -----------------------------------------------------------------------------------------------------
+
+template <typename T, int DK, int DV, bool TMA>
+__global__ void __launch_bounds__(LtCfg<T, DK, DV>::kThreads, 1)
+linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                     const __grid_constant__ CUtensorMap map_v) {
     using C = LtCfg<T, DK, DV>;
+    constexpr int kWarpsW = C::kWarpsW;
     extern __shared__ __align__(1024) unsigned char smem[];
     LtMisc& m = *reinterpret_cast<LtMisc*>(smem + C::oMisc);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int tile = blockIdx.x % tiles, h = (blockIdx.x / tiles) % a.heads, order = blockIdx.x / (tiles * a.heads);
+    const int seg = blockIdx.x % plan.segs, rest = blockIdx.x / plan.segs;
+    const int tile = rest % plan.tiles, h = (rest / plan.tiles) % a.heads, order = rest / (plan.tiles * a.heads);
     const int hk = h / (a.heads / a.kv_heads), col0 = tile * DV, dv = min(DV, a.dv - col0);
 
     // long sequences first, so that the last CTAs are short ones
     if (tid == 0) m.b = order;
     __syncthreads();
-    if (a.lengths != nullptr && a.batch <= kLtThreads) {
+    if (a.lengths != nullptr && a.batch <= C::kThreads) {
         if (tid < a.batch) {
             const int mine = lin_length(a, tid);
             int before = 0;
@@ -144,44 +290,65 @@ __global__ void __launch_bounds__(kLtThreads, 1) linattn_chunk_kernel(const LinA
     const int b = m.b;
     int bits;
     const int slot = lin_slot(a, b, lane, bits);
-    if (bits != 0 && a.status != nullptr && tid == 0 && tile == 0) atomicOr(a.status, bits);
+    if (bits != 0 && a.status != nullptr && tid == 0 && tile == 0 && seg == 0) atomicOr(a.status, bits);
     const int length = slot < 0 ? 0 : lin_length(a, b);
-    const int64_t state_at = (static_cast<int64_t>(slot < 0 ? 0 : slot) * a.heads + h) * a.dk * a.dv + col0;
-    const T* q = static_cast<const T*>(a.q) + b * a.q_stride[0] + h * a.q_stride[2];
-    const T* k = static_cast<const T*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2];
-    const T* v = static_cast<const T*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2] + col0;
+    const int seg0 = plan.segs > 1 ? seg * plan.seg_tokens : 0;                                        // first token of this part
+    const int seg_end = plan.segs > 1 && seg + 1 < plan.segs ? min(length, seg0 + plan.seg_tokens) : length;
+    const bool outputs = plan.mode != 1;
     T* out = static_cast<T*>(a.out) + b * a.out_stride[0] + h * a.out_stride[2] + col0;
-
-    // rows behind the sequence
-    for (int64_t i = tid; i < static_cast<int64_t>(a.tokens - length) * dv; i += kLtThreads) {
-        const int64_t t = i / dv;
-        out[(length + t) * a.out_stride[1] + (i - t * dv)] = lin_from<T>(0.0f);
+    if (outputs) {  // rows behind the sequence, those that fall in this part
+        const int z0 = max(length, seg0), z1 = plan.segs > 1 && seg + 1 < plan.segs ? min(a.tokens, seg0 + plan.seg_tokens) : a.tokens;
+        for (int64_t i = tid; i < static_cast<int64_t>(max(0, z1 - z0)) * dv; i += C::kThreads) {
+            const int64_t t = i / dv;
+            out[(z0 + t) * a.out_stride[1] + (i - t * dv)] = lin_from<T>(0.0f);
+        }
     }
-    if (slot < 0) return;
+    if (slot < 0 || (plan.mode == 2 && seg_end <= seg0)) return;
+    const int chunks = max(0, seg_end - seg0 + kLtChunk - 1) / kLtChunk;
 
-    // S: thread -> row (its TMEM lane) and half of the columns
-    constexpr int SC = DV / 2;
-    const int row = (warp & 3) * 32 + lane, half = warp >> 2;
-    const bool has_row = row < a.dk;
-    float s[SC];
-    {
-        const float* at = a.state_in + state_at + static_cast<int64_t>(row) * a.dv + half * SC;
-#pragma unroll
-        for (int c = 0; c < SC; ++c) s[c] = a.state_in != nullptr && has_row && half * SC + c < dv ? at[c] : 0.0f;
-    }
     const double log_decay = static_cast<double>(fmaxf(a.log_decay[h], -1e30f));
     if (tid <= kLtChunk) {
         const double p = exp(log_decay * tid);
         m.power[tid] = static_cast<float>(p);
-        if (tid == kLtChunk) m.power_lo = static_cast<float>(p - static_cast<double>(static_cast<float>(p)));
+        m.scaled[tid] = static_cast<float>(p * static_cast<double>(a.scale));
+        if (tid > 0) m.scaled_next[tid - 1] = m.scaled[tid];
+        if (tid < kLtChunk) {
+            double left = p;
+            uint32_t w[3];
+            for (int i = 0; i < 3; ++i) {
+                const __nv_bfloat16 part = __float2bfloat16_rn(static_cast<float>(left));
+                left -= static_cast<double>(__bfloat162float(part));
+                const __nv_bfloat162 twice = __halves2bfloat162(part, part);
+                w[i] = *reinterpret_cast<const uint32_t*>(&twice);
+            }
+            m.weight[tid] = make_uint2(w[0], w[1]);
+            m.weight2[tid] = w[2];
+        } else {
+            const float near = static_cast<float>(p), off = static_cast<float>(p - static_cast<double>(near));
+            const float next = __uint_as_float(__float_as_uint(near) + (off > 0.0f ? 1u : 0xffffffffu));
+            m.power_next = off != 0.0f && near > 0.0f ? next : near;
+            m.power_gap = near > 0.0f ? fabsf(next - near) / near : 1.0f;
+            m.power_off = near > 0.0f ? fabsf(off) / near : 0.0f;
+        }
     }
-    if (tid < 128) m.first_bad[tid] = kLtChunk;
+    if (tid < 128) {
+        for (int i = 0; i < kLtMarks; ++i) m.first_bad[i][tid] = 0x7fffffff;
+    }
     if (tid == 0) {
-        mbar_init(&m.bar_g, 1);
-        mbar_init(&m.bar_u, 1);
-        mbar_init(&m.bar_y, 1);
+        for (int i = 0; i < C::kStages; ++i) {
+            mbar_init(&m.full[i], TMA ? 1 : kWarpsW);
+            mbar_init(&m.empty[i], 1);
+            mbar_init(&m.w_full[i], kWarpsW);
+            mbar_init(&m.w_free[i], 1);
+        }
+        mbar_init(&m.g_full, 1), mbar_init(&m.u_full, 1), mbar_init(&m.x_full, 1), mbar_init(&m.y_full, 1);
+        mbar_init(&m.p_full, 4);
+        mbar_init(&m.u_free, kLtWarpsS);
+        mbar_init(&m.s_full, kLtWarpsS);
+        mbar_init(&m.xy_free, C::kWarpsO);
         fence_barrier_init();
-        m.dead = m.any_bad = 0;
+        m.dead = 0;
+        for (int i = 0; i < kLtMarks; ++i) m.any_bad[i] = 0;
     }
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&m.tmem)), "r"(kLtTmemCols) : "memory");
@@ -191,273 +358,436 @@ __global__ void __launch_bounds__(kLtThreads, 1) linattn_chunk_kernel(const LinA
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = m.tmem, lane_base = tmem + ((static_cast<uint32_t>(warp & 3) * 32u) << 16);
-    // instruction descriptors: fp32 accumulators, bf16 operands, M = 128; N, and which operands are MN-major
-    constexpr uint32_t kD = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24), kMnA = 1u << 15, kMnB = 1u << 16;
-    constexpr uint32_t kIdescG = kD | ((kLtChunk / 8) << 17), kIdescX = kD | kMnA | ((kLtChunk / 8) << 17), kIdescU = kD | kMnA | kMnB | ((DV / 8) << 17);
 
-    const int chunks = (length + kLtChunk - 1) / kLtChunk;
-    // brings chunk c into its stage
-    const auto fetch = [&](int c) {
-        unsigned char* st = smem + (c % C::kStages) * C::kStage;
-        const int t0 = c * kLtChunk, n = min(kLtChunk, length - t0);
-        if (C::kAsync && aligned) {
+    if (warp < kLtWarpsS) {
+        // ---- S: row = channel of V
+        constexpr int kHalf = DK / 2;
+        const int row = (warp & 3) * 32 + lane, k0 = (warp >> 2) * kHalf;
+        const bool has_row = row < dv;
+        const int64_t cell = static_cast<int64_t>(k0) * a.dv + col0 + row;
+        const int64_t own = (static_cast<int64_t>(slot) * a.heads + h) * a.dk * a.dv + cell;
+        const int64_t part = ((static_cast<int64_t>(b) * a.heads + h) * plan.segs + seg) * a.dk * a.dv + cell;
+        const float* from = plan.mode == 2 ? plan.states + part : plan.mode == 0 && a.state_in != nullptr ? a.state_in + own : nullptr;
+        float* to = plan.mode == 2 ? nullptr : plan.mode == 1 ? plan.states + part : a.state_out + own;
+        // (loops stay loops here and below: unrolled, the roles' code did not fit the instruction cache, and a third of all stalls was for it)
+        const auto keep = [&](int g, float (&s)[16]) {
+            if (C::NS == 2) lt_st(lane_base + kLtS + k0 + g, s);
+            if (C::NS == 3 || outputs) {
 #pragma unroll
-            for (int i = tid; i < kLtChunk * DK / 8; i += kLtThreads) {
-                int g, t;
-                lt_piece(i, DK / 8, g, t);
-                const int bytes = t < n ? max(0, min(16, (a.dk - g * 8) * 2)) : 0;
-                const int at = lt_offset(g, t);
-                lt_cp16(st + at, bytes > 0 ? q + (t0 + t) * a.q_stride[1] + g * 8 : q, bytes);
-                lt_cp16(st + C::kTileK + at, bytes > 0 ? k + (t0 + t) * a.k_stride[1] + g * 8 : k, bytes);
-            }
+                for (int p = 0; p < C::NS; ++p) {
+                    uint32_t u[8];
 #pragma unroll
-            for (int i = tid; i < kLtChunk * DV / 8; i += kLtThreads) {
-                int g, t;
-                lt_piece(i, DV / 8, g, t);
-                const int bytes = t < n ? max(0, min(16, (dv - g * 8) * 2)) : 0;
-                lt_cp16(st + 2 * C::kTileK + lt_offset(g, t), bytes > 0 ? v + (t0 + t) * a.v_stride[1] + g * 8 : v, bytes);
+                    for (int e = 0; e < 8; ++e) u[e] = lt_part(s[2 * e], s[2 * e + 1], p + 1 == C::NS);
+                    lt_st(lane_base + C::kParts + p * kHalf + (k0 + g) / 2, u);
+                }
             }
-        } else {
-            for (int i = tid; i < kLtChunk * DK / 8; i += kLtThreads) {
-                int g, t;
-                lt_piece(i, DK / 8, g, t);
-                const int valid = t < n ? max(0, min(8, a.dk - g * 8)) : 0;
-                const int at = lt_offset(g, t);
-                float x[8];
-                lt_load8(q + (t0 + t) * a.q_stride[1] + g * 8, valid, aligned, x);
-                lt_store_parts<C::NX>(st + at, C::kTileK, x);
-                lt_load8(k + (t0 + t) * a.k_stride[1] + g * 8, valid, aligned, x);
-                lt_store_parts<C::NX>(st + C::NX * C::kTileK + at, C::kTileK, x);
-            }
-            for (int i = tid; i < kLtChunk * DV / 8; i += kLtThreads) {
-                int g, t;
-                lt_piece(i, DV / 8, g, t);
-                const int valid = t < n ? max(0, min(8, dv - g * 8)) : 0;
-                const int at = lt_offset(g, t);
-                float x[8];
-                lt_load8(v + (t0 + t) * a.v_stride[1] + g * 8, valid, aligned, x);
-                if (!C::kAsync) {  // W from the values themselves
-                    const float w = m.power[t < n ? n - 1 - t : 0];
-                    float y[8];
-                    bool bad = false;
+        };
+        const auto at_end = [&](int g, const float (&s)[16]) {
+            if (to == nullptr || !has_row) return;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        y[e] = x[e] * w;
-                        bad |= !(fabsf(x[e]) <= 3.4028234663852886e38f);
+            for (int e = 0; e < 16; ++e)
+                if (k0 + g + e < a.dk) to[static_cast<int64_t>(g + e) * a.dv] = s[e];
+        };
+#pragma unroll 1
+        for (int g = 0; g < kHalf; g += 16) {
+            float s[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = from != nullptr && has_row && k0 + g + e < a.dk ? from[static_cast<int64_t>(g + e) * a.dv] : 0.0f;
+            if (chunks == 0) at_end(g, s);
+            keep(g, s);
+        }
+        lt_st_wait();
+        lt_arrive_read(&m.s_full, lane);
+        // The decay of a chunk is one of the two floats beside it, by turns, so that their product stays within half a step of the decay's
+        // power: rounded the same way every time it would be off by 2^-25 per chunk.
+        float drift = 0.0f;
+#pragma unroll 1
+        for (int c = 0; c < chunks; ++c) {  // S behind chunk c
+            const bool last = c + 1 == chunks;
+            if (!lt_wait(m, &m.u_full, c & 1) || (outputs && !last && !lt_wait(m, &m.x_full, c & 1))) break;
+            tc_fence_after();
+            const int n = min(kLtChunk, seg_end - seg0 - c * kLtChunk);
+            float pn = m.power[n];
+            if (n == kLtChunk) {
+                drift += m.power_off;
+                if (2.0f * drift >= m.power_gap) {
+                    drift -= m.power_gap;
+                    pn = m.power_next;
+                }
+            }
+#pragma unroll 1
+            for (int g = 0; g < kHalf; g += 16) {
+                float s[16];
+                uint32_t ru[16];
+                lt_ld(lane_base + kLtU + k0 + g, ru);
+                if (C::NS == 3) {
+                    uint32_t p0[8], p1[8], p2[8];
+                    lt_ld(lane_base + C::kParts + (k0 + g) / 2, p0);
+                    lt_ld(lane_base + C::kParts + kHalf + (k0 + g) / 2, p1);
+                    lt_ld(lane_base + C::kParts + 2 * kHalf + (k0 + g) / 2, p2);
+                    lt_ld_wait(p0);
+                    lt_ld_wait(p1);
+                    lt_ld_wait(p2);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {  // (exact: the parts are 24 bits)
+                        s[2 * e] = __uint_as_float(p0[e] << 16) + (__uint_as_float(p1[e] << 16) + __uint_as_float(p2[e] << 16));
+                        s[2 * e + 1] = __uint_as_float(p0[e] & 0xFFFF0000u) + (__uint_as_float(p1[e] & 0xFFFF0000u) + __uint_as_float(p2[e] & 0xFFFF0000u));
                     }
-                    if (bad) {
-                        m.any_bad = 1;
+                } else {
+                    uint32_t rs[16];
+                    lt_ld(lane_base + kLtS + k0 + g, rs);
+                    lt_ld_wait(rs);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (!(fabsf(x[e]) <= 3.4028234663852886e38f)) {
-                                atomicMin(&m.first_bad[g * 8 + e], t);
-                                x[e] = 0.0f;
+                    for (int e = 0; e < 16; ++e) s[e] = __uint_as_float(rs[e]);
+                }
+                lt_ld_wait(ru);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] = fmaf(pn, s[e], __uint_as_float(ru[e]));
+                if (last) at_end(g, s);
+                else keep(g, s);
+            }
+            lt_st_wait();
+            lt_arrive_read(&m.u_free, lane);
+            if (!last) lt_arrive_read(&m.s_full, lane);  // (one more would be a phase ahead of the products' wait for this one)
+        }
+    } else if (warp < C::kFirstO) {
+        // ---- W (and tiles)
+        constexpr int threads = 32 * kWarpsW;
+        const int id = tid - 32 * C::kFirstW;
+        const T* q = static_cast<const T*>(a.q) + b * a.q_stride[0] + h * a.q_stride[2] + seg0 * a.q_stride[1];
+        const T* k = static_cast<const T*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2] + seg0 * a.k_stride[1];
+        const T* v = static_cast<const T*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2] + seg0 * a.v_stride[1] + col0;
+        for (int c = 0; c < chunks; ++c) {
+            const int t0 = c * kLtChunk, n = min(kLtChunk, seg_end - seg0 - t0), stage = c % C::kStages, mark = c % kLtMarks;
+            const uint32_t turn = (c / C::kStages) & 1;
+            unsigned char* st = smem + stage * C::kStage;
+            bool bad = false;
+            if (TMA) {
+                if (!lt_wait(m, &m.full[stage], turn)) break;
+                // rows behind the sequence are somebody's: K (here) and V (below) must be zero there; Q's make rows that nobody reads
+                for (int i = id; i < (kLtChunk - n) * (DK / 8); i += threads)
+                    *reinterpret_cast<uint4*>(st + C::oK + lt_swizzled(i % (DK / 8), n + i / (DK / 8))) = make_uint4(0, 0, 0, 0);
+            } else {
+                if (c >= C::kStages && !lt_wait(m, &m.empty[stage], turn ^ 1u)) break;
+                static_assert(kLtChunk * DK / 8 / threads % 2 == 0, "pieces");
+#pragma unroll 1
+                for (int i0 = 0; i0 < kLtChunk * DK / 8 / threads; i0 += 2) {
+                    float x[2][8], y[2][8];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int i = id + (i0 + j) * threads, g = i % (DK / 8), t = i / (DK / 8);
+                        const int valid = t < n ? max(0, min(8, a.dk - g * 8)) : 0;
+                        lt_load8(k + (t0 + t) * a.k_stride[1] + g * 8, valid, plan.aligned, y[j]);
+                        if (outputs) lt_load8(q + (t0 + t) * a.q_stride[1] + g * 8, valid, plan.aligned, x[j]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int i = id + (i0 + j) * threads, at = lt_swizzled(i % (DK / 8), i / (DK / 8));
+                        if (outputs) lt_store_parts<C::NX>(st + at, C::kTileK, x[j]);
+                        lt_store_parts<C::NX>(st + C::oK + at, C::kTileK, y[j]);
+                    }
+                }
+            }
+            // V, and W (free when the product before that has it is done)
+            if (c >= C::kStages && !lt_wait(m, &m.w_free[stage], turn ^ 1u)) break;
+            unsigned char* wt = smem + C::oW + stage * C::NW * C::kTileV;
+            constexpr int kPieces = kLtChunk * DV / 8 / threads, kBatch = 2;  // of a thread; on their way together
+            static_assert(kPieces % kBatch == 0, "pieces");
+#pragma unroll 1
+            for (int i0 = 0; i0 < kPieces; i0 += kBatch) {
+                const auto token_of = [&](int i) { return (i & 7) | ((i >> 5) & 7) << 3; };  // eight tokens beside one another, four groups
+                const auto group_of = [&](int i) { return ((i >> 3) & 3) | (i >> 8) << 2; };
+                if (TMA) {
+                    uint4 u[kBatch];
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {
+                        const int i = id + (i0 + j) * threads, t = token_of(i);
+                        uint4* vp = reinterpret_cast<uint4*>(st + C::oV + lt_swizzled(group_of(i), t));
+                        if (t >= n) *vp = make_uint4(0, 0, 0, 0);
+                        u[j] = *vp;
+                    }
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {
+                        const int i = id + (i0 + j) * threads, t = token_of(i), g = group_of(i), back = t < n ? n - 1 - t : 0;
+                        uint32_t w4[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
+                        lt_weigh(wt + lt_plain(g, t), C::kTileV, w4, m.weight[back], m.weight2[back]);
+                        uint32_t high = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) high = __vmaxu2(high, w4[e] & 0x7FFF7FFFu);
+                        if ((high & 0xFFFFu) >= 0x7F80u || high >= 0x7F800000u) {
+                            bad = true;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                if (((w4[e / 2] >> (16 * (e & 1))) & 0x7F80u) != 0x7F80u) continue;
+                                w4[e / 2] &= (e & 1) != 0 ? 0x0000FFFFu : 0xFFFF0000u;
+                                atomicMin(&m.first_bad[mark][g * 8 + e], ((1 << 24) - c) * kLtChunk + t);
                             }
+                            *reinterpret_cast<uint4*>(st + C::oV + lt_swizzled(g, t)) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+                        }
                     }
-                    lt_store_parts<C::NW>(smem + C::oW + at, C::kTileV, y);
+                } else {
+                    float x[kBatch][8];
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {
+                        const int i = id + (i0 + j) * threads, t = token_of(i), g = group_of(i);
+                        lt_load8(v + (t0 + t) * a.v_stride[1] + g * 8, t < n ? max(0, min(8, dv - g * 8)) : 0, plan.aligned, x[j]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {
+                        const int i = id + (i0 + j) * threads, t = token_of(i), g = group_of(i);
+                        const float w = m.power[t < n ? n - 1 - t : 0];
+                        float y[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) y[e] = x[j][e] * w;
+                        lt_store_parts<C::NW>(wt + lt_plain(g, t), C::kTileV, y);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            if (lt_finite(x[j][e])) continue;
+                            bad = true;
+                            x[j][e] = 0.0f;
+                            atomicMin(&m.first_bad[mark][g * 8 + e], ((1 << 24) - c) * kLtChunk + t);
+                        }
+                        lt_store_parts<C::NX>(st + C::oV + lt_swizzled(g, t), C::kTileV, x[j]);
+                    }
                 }
-                lt_store_parts<C::NX>(st + 2 * C::NX * C::kTileK + at, C::kTileV, x);
             }
-        }
-    };
-
-    if (C::kStages == 2 && chunks > 0) fetch(0);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    for (int c = 0; c < chunks; ++c) {
-        const uint32_t parity = c & 1;
-        const int t0 = c * kLtChunk, n = min(kLtChunk, length - t0);
-        unsigned char* st = smem + (c % C::kStages) * C::kStage;
-        const uint32_t sq = smem_u32(st), sk = sq + C::NX * C::kTileK, sv = sk + C::NX * C::kTileK, ss = smem_u32(smem + C::oS),
-                       sw = smem_u32(smem + C::oW), sp = smem_u32(smem + C::oP);
-        if (C::kStages == 2) {
-            if (c + 1 < chunks) fetch(c + 1);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-        } else {
-            fetch(c);
-        }
-        fence_proxy_async();
-        __syncthreads();
-        if (tid == 0) {  // G = Q K^T
-            tc_fence_after();
-            bool add = false;
-#pragma unroll
-            for (int sum = C::NX - 1; sum >= 0; --sum)
-#pragma unroll
-                for (int p = 0; p <= sum; ++p)
-#pragma unroll
-                    for (int i = 0; i < DK / 16; ++i) {
-                        lt_mma(tmem + kLtG, make_smem_desc(sq + p * C::kTileK + i * 2048, 1024, 128),
-                               make_smem_desc(sk + (sum - p) * C::kTileK + i * 2048, 1024, 128), kIdescG, add);
-                        add = true;
-                    }
-            tc_commit(&m.bar_g);
-        }
-        if (C::kAsync) {  // W = decayed V
-            for (int i = tid; i < kLtChunk * DV / 8; i += kLtThreads) {
-                int g, t;
-                lt_piece(i, DV / 8, g, t);
-                const int at = lt_offset(g, t);
-                uint4* vp = reinterpret_cast<uint4*>(st + 2 * C::kTileK + at);
-                const uint4 u = *vp;
-                const uint32_t w4[4] = {u.x, u.y, u.z, u.w};
-                const float w = m.power[t < n ? n - 1 - t : 0];
-                float x[8];
-                bool bad = false;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    bad |= (w4[e] & 0x7F80u) == 0x7F80u || (w4[e] & 0x7F800000u) == 0x7F800000u;
-                    x[2 * e] = __uint_as_float(w4[e] << 16) * w;
-                    x[2 * e + 1] = __uint_as_float(w4[e] & 0xFFFF0000u) * w;
-                }
-                if (bad) {
-                    m.any_bad = 1;
-                    uint32_t fix[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        fix[e] = w4[e];
-                        if ((w4[e] & 0x7F80u) == 0x7F80u) fix[e] &= 0xFFFF0000u, atomicMin(&m.first_bad[g * 8 + 2 * e], t);
-                        if ((w4[e] & 0x7F800000u) == 0x7F800000u) fix[e] &= 0xFFFFu, atomicMin(&m.first_bad[g * 8 + 2 * e + 1], t);
-                    }
-                    *vp = make_uint4(fix[0], fix[1], fix[2], fix[3]);
-                }
-                lt_store_parts<C::NW>(smem + C::oW + at, C::kTileV, x);
-            }
-        }
-        // S as an operand: rows dk, groups of 8 columns DK * 16 bytes apart
-        if (row < DK) {
-#pragma unroll
-            for (int g = 0; g < SC / 8; ++g) {
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = s[g * 8 + e];
-                lt_store_parts<C::NS>(smem + C::oS + (half * (SC / 8) + g) * (DK * 16) + (row >> 3) * 128 + (row & 7) * 16, C::kPartS, x);
-            }
-        }
-        fence_proxy_async();
-        __syncthreads();
-        if (tid == 0) {
-            tc_fence_after();
-            bool add = false;
-            // X = S^T Q^T
-#pragma unroll
-            for (int sum = C::NS - 1; sum >= 0; --sum)
-#pragma unroll
-                for (int p = 0; p <= sum; ++p) {
-                    if (sum - p >= C::NX) continue;
-#pragma unroll
-                    for (int i = 0; i < DK / 16; ++i) {
-                        lt_mma(tmem + kLtX, make_smem_desc(ss + p * C::kPartS + i * 256, 128, DK * 16),
-                               make_smem_desc(sq + (sum - p) * C::kTileK + i * 2048, 1024, 128), kIdescX, add);
-                        add = true;
-                    }
-                }
-            // U = K^T W
-            add = false;
-#pragma unroll
-            for (int sum = C::NW - 1; sum >= 0; --sum)
-#pragma unroll
-                for (int p = 0; p <= sum; ++p) {
-                    if (sum - p >= C::NX) continue;
-#pragma unroll
-                    for (int i = 0; i < kLtChunk / 16; ++i) {
-                        lt_mma(tmem + kLtU, make_smem_desc(sk + (sum - p) * C::kTileK + i * 256, 128, 1024),
-                               make_smem_desc(sw + p * C::kTileV + i * 256, 128, 1024), kIdescU, add);
-                        add = true;
-                    }
-                }
-            tc_commit(&m.bar_u);
-        }
-        // P: rows = tokens i, in the first two warps of each half
-        if ((warp & 3) < 2) {
-            if (!mbar_wait_bounded(&m.bar_g, parity, kLtWaitLimit)) m.dead = 1;
-            tc_fence_after();
-            float g[32];
-            tc_ld_32cols(lane_base + kLtG + half * 32, g);
-#pragma unroll
-            for (int o = 0; o < 4; ++o) {
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int j = half * 32 + o * 8 + e;
-                    x[e] = j <= row ? g[o * 8 + e] * m.power[row - j < 0 ? 0 : row - j] : 0.0f;
-                }
-                lt_store_parts<C::NS>(smem + C::oP + (half * 4 + o) * 1024 + (row >> 3) * 128 + (row & 7) * 16, C::kPartP, x);
-            }
+            if (bad) *reinterpret_cast<volatile int*>(&m.any_bad[mark]) = c + 1;
             fence_proxy_async();
-            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (!TMA) mbar_arrive(&m.full[stage]);
+                mbar_arrive(&m.w_full[stage]);
+            }
         }
-        __syncthreads();
-        if (m.dead) break;
-        if (tid == 0) {  // Y = V^T P^T
-            tc_fence_after();
-            bool add = false;
+    } else if (warp < C::kFirstP) {
+        // ---- the outputs: row = channel of V, a share of the tokens
+        constexpr int kShare = kLtChunk / (C::kWarpsO / 4);
+        const int row = (warp & 3) * 32 + lane, token0 = ((warp - C::kFirstO) >> 2) * kShare;
+        if (outputs) {
+            out += seg0 * a.out_stride[1] + row;
+#pragma unroll 1
+            for (int c = 0; c < chunks; ++c) {
+                if (!lt_wait(m, &m.y_full, c & 1)) break;
+                tc_fence_after();
+                const int mark = c % kLtMarks;
+                int first = kLtChunk;
+                if (*reinterpret_cast<volatile int*>(&m.any_bad[mark]) == c + 1) {
+                    const int at = m.first_bad[mark][row];
+                    if ((at >> 6) == (1 << 24) - c) first = at & 63;
+                }
+#pragma unroll 1
+                for (int block = token0; block < token0 + kShare; block += 32) {
+                    T o[32];
 #pragma unroll
-            for (int sum = C::NS - 1; sum >= 0; --sum)
+                    for (int u = 0; u < 32; u += 16) {
+                        uint32_t x[16], y[16];
+                        lt_ld(lane_base + kLtX + block + u, x);
+                        lt_ld(lane_base + kLtY + block + u, y);
+                        lt_ld_wait(x);
+                        lt_ld_wait(y);
+                        if (u == 16 && block + 32 == token0 + kShare) lt_arrive_read(&m.xy_free, lane);
 #pragma unroll
-                for (int p = 0; p <= sum; ++p) {
-                    if (sum - p >= C::NX) continue;
+                        for (int i = 0; i < 16; ++i)
+                            o[u + i] = lin_from<T>(fmaf(m.scaled_next[block + u + i], __uint_as_float(x[i]), __uint_as_float(y[i])));
+                    }
+                    const int t0 = c * kLtChunk + block, n = seg_end - seg0 - t0;
+                    T* at = out + t0 * a.out_stride[1];
+                    if (row < dv) {
 #pragma unroll
-                    for (int i = 0; i < kLtChunk / 16; ++i) {
-                        lt_mma(tmem + kLtY, make_smem_desc(sv + (sum - p) * C::kTileV + i * 256, 128, 1024),
-                               make_smem_desc(sp + p * C::kPartP + i * 2048, 1024, 128), kIdescX, add);
-                        add = true;
+                        for (int i = 0; i < 32; ++i)
+                            if (i < n) at[i * a.out_stride[1]] = o[i];
+                        for (int i = max(0, first - block); i < min(32, n); ++i) at[i * a.out_stride[1]] = lin_from<T>(__int_as_float(0x7fffffff));
                     }
                 }
-            tc_commit(&m.bar_y);
-        }
-        if (!mbar_wait_bounded(&m.bar_u, parity, kLtWaitLimit)) m.dead = 1;
-        tc_fence_after();
-        {
-            const float pn = m.power[n], pn_lo = n == kLtChunk ? m.power_lo : 0.0f;
-#pragma unroll
-            for (int g = 0; g < SC / 32; ++g) {
-                float u[32];
-                tc_ld_32cols(lane_base + kLtU + half * SC + g * 32, u);
-#pragma unroll
-                for (int e = 0; e < 32; ++e) s[g * 32 + e] = fmaf(pn, s[g * 32 + e], fmaf(pn_lo, s[g * 32 + e], u[e]));
             }
         }
-        if (!mbar_wait_bounded(&m.bar_y, parity, kLtWaitLimit)) m.dead = 1;
-        tc_fence_after();
-        {
-            float x[32], y[32];
-            tc_ld_32cols(lane_base + kLtX + half * 32, x);
-            tc_ld_32cols(lane_base + kLtY + half * 32, y);
-            const int first_bad = m.any_bad ? m.first_bad[row] : kLtChunk;
-            if (row < dv) {
-                T* at = out + (t0 + half * 32) * a.out_stride[1] + row;
+    } else if ((warp & 3) < 2) {
+        // ---- P: row = token i; half of the tokens j
+        const int row = (warp & 3) * 32 + lane, half = (warp - C::kFirstP) >> 2;
+        if (outputs) {
+            unsigned char* at = smem + C::oP + half * 4 * 1024 + (row >> 3) * 128 + (row & 7) * 16;
+            const int d0 = row - half * 32;
+            float power[32];  // of the thread's 32 entries, in every chunk the same
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const int t = half * 32 + i;
-                    float o = fmaf(m.power[t + 1], x[i], y[i]) * a.scale;
-                    if (t >= first_bad) o = __int_as_float(0x7fffffff);
-                    if (t < n) *at = lin_from<T>(o);
-                    at += a.out_stride[1];
+            for (int e = 0; e < 32; ++e) power[e] = m.scaled[max(d0 - e, 0)];
+            const bool nothing = half > (warp & 3), whole = half < (warp & 3);  // tokens behind all of the rows, in front of all
+#pragma unroll 1
+            for (int c = 0; c < chunks; ++c) {
+                if (!lt_wait(m, &m.g_full, c & 1)) break;  // (and so the product before that read P is done)
+                tc_fence_after();
+#pragma unroll
+                for (int u = 0; u < 32; u += 16) {
+                    uint32_t g[16];
+                    if (!nothing) {
+                        lt_ld(lane_base + kLtY + half * 32 + u, g);
+                        lt_ld_wait(g);
+                    }
+#pragma unroll
+                    for (int f = 0; f < 16; f += 8) {
+                        float x[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            x[e] = __uint_as_float(g[f + e]) * power[u + f + e];
+                            if (!whole && (nothing || d0 < u + f + e)) x[e] = 0.0f;
+                        }
+                        lt_store_parts<C::NS>(at + (u / 8 + f / 8) * 1024, C::kPartP, x);
+                    }
                 }
+                tc_fence_before();
+                lt_arrive_operands(&m.p_full, lane);
             }
         }
-        tc_fence_before();
-        __syncthreads();
-        if (m.dead) break;
-        if (m.any_bad) {  // (the next chunk's marks come behind a barrier)
-            if (tid < 128) m.first_bad[tid] = kLtChunk;
-            __syncthreads();
-            if (tid == 0) m.any_bad = 0;
-            __syncthreads();
-        }
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    if (m.dead && tid == 0 && a.status != nullptr) atomicOr(a.status, FB_STATUS_WAIT_TIMEOUT);
-    if (has_row) {
-        float* at = a.state_out + state_at + static_cast<int64_t>(row) * a.dv + half * SC;
+    } else if (warp == C::kFirstP + 2) {
+        // ---- the products
+        {
+            // instruction descriptors: fp32 accumulators, bf16 operands, M = 128; N, and which operands are MN-major
+            constexpr uint32_t kD = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24), kMnA = 1u << 15, kMnB = 1u << 16;
+            constexpr uint32_t kIdescG = kD | ((kLtChunk / 8) << 17), kIdescX = kIdescG, kIdescY = kIdescG | kMnA,
+                               kIdescU = kD | kMnA | kMnB | ((DK / 8) << 17);
+            const uint32_t base = smem_u32(smem);
+            const uint64_t dp = make_smem_desc(base + C::oP, 1024, 128);
+            const auto wait = [&](uint64_t* bar, uint32_t parity) { return lt_wait(m, bar, parity); };
+            // The products of parts p of one operand and r of the other with p + r < parts, the small ones first; mma(p, r, i, add) is one step
+            // of four along the sum.  (The loops stay loops: as straight code this warp waited for its instructions.)
+            const auto parts = [&](int na, int nb, int count, int quads, auto&& mma) {
+                bool add = false;
+#pragma unroll 1
+                for (int sum = count - 1; sum >= 0; --sum)
+#pragma unroll 1
+                    for (int p = max(0, sum - nb + 1); p <= min(sum, na - 1); ++p)
+#pragma unroll 1
+                        for (int quad = 0; quad < quads; ++quad)
 #pragma unroll
-        for (int c = 0; c < SC; ++c)
-            if (half * SC + c < dv) at[c] = s[c];
+                            for (int i = 0; i < 4; ++i) {
+                                mma(p, sum - p, quad, i, add);
+                                add = true;
+                            }
+            };
+            const auto make_u = [&](int c) {  // U^T = W^T K
+                if (!wait(&m.w_full[c % C::kStages], (c / C::kStages) & 1) || (c > 0 && !wait(&m.u_free, (c - 1) & 1))) return false;
+                tc_fence_after();
+                if (lt_elect()) {
+                    const uint64_t dk = lt_desc_swizzled(base + (c % C::kStages) * C::kStage + C::oK, 8192, 1024),
+                                   dw = make_smem_desc(base + C::oW + (c % C::kStages) * C::NW * C::kTileV, 128, 1024);
+                    parts(C::NW, C::NX, C::NW, 1, [&](int p, int r, int, int i, bool add) {
+                        lt_mma(tmem + kLtU, dw + ((p * C::kTileV + i * 256) >> 4), dk + ((r * C::kTileK + i * 2048) >> 4), kIdescU, add);
+                    });
+                    tc_commit(&m.u_full);
+                    tc_commit(&m.w_free[c % C::kStages]);
+                    if (!outputs) tc_commit(&m.empty[c % C::kStages]);
+                }
+                __syncwarp();
+                return true;
+            };
+            bool ok = chunks == 0 || make_u(0);
+#pragma unroll 1
+            for (int c = 0; c < chunks && ok; ++c) {
+                if (outputs) {
+                    const uint32_t at = base + (c % C::kStages) * C::kStage;
+                    const uint64_t dq = lt_desc_swizzled(at, 16, 1024), dk = lt_desc_swizzled(at + C::oK, 16, 1024),
+                                   dv = lt_desc_swizzled(at + C::oV, 8192, 1024);
+                    ok = wait(&m.full[c % C::kStages], (c / C::kStages) & 1) && (c == 0 || wait(&m.xy_free, (c - 1) & 1));
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (lt_elect()) {  // G = Q K^T
+                        parts(C::NX, C::NX, C::NX, DK / 64, [&](int p, int r, int quad, int i, bool add) {
+                            const int step = quad * 8192 + i * 32;
+                            lt_mma(tmem + kLtY, dq + ((p * C::kTileK + step) >> 4), dk + ((r * C::kTileK + step) >> 4), kIdescG, add);
+                        });
+                        tc_commit(&m.g_full);
+                    }
+                    __syncwarp();
+                    ok = wait(&m.s_full, c & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (lt_elect()) {  // X^T = S^T Q^T
+                        parts(C::NS, C::NX, C::NS, DK / 64, [&](int p, int r, int quad, int i, bool add) {
+                            lt_mma_tmem(tmem + kLtX, tmem + C::kParts + p * (DK / 2) + quad * 32 + i * 8,
+                                        dq + ((r * C::kTileK + quad * 8192 + i * 32) >> 4), kIdescX, add);
+                        });
+                        tc_commit(&m.x_full);
+                    }
+                    __syncwarp();
+                    ok = wait(&m.p_full, c & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (lt_elect()) {  // Y^T = V^T P^T
+                        parts(C::NS, C::NX, C::NS, 1, [&](int p, int r, int, int i, bool add) {
+                            lt_mma(tmem + kLtY, dv + ((r * C::kTileV + i * 2048) >> 4), dp + ((p * C::kPartP + i * 2048) >> 4), kIdescY, add);
+                        });
+                        tc_commit(&m.y_full);
+                        tc_commit(&m.empty[c % C::kStages]);
+                    }
+                    __syncwarp();
+                }
+                if (c + 1 < chunks) ok = make_u(c + 1);
+            }
+        }
+    } else if (TMA && warp == C::kFirstP + 3 && lane == 0) {
+        // ---- the copies
+        constexpr uint32_t kBytesK = C::kTileK, kBytesV = C::kTileV;
+        int issued = 0;
+        for (int c = 0; c < chunks; ++c) {
+            const int stage = c % C::kStages;
+            if (c >= C::kStages && !lt_wait_one(m, &m.empty[stage], ((c / C::kStages) & 1) ^ 1u)) break;
+            unsigned char* st = smem + stage * C::kStage;
+            mbar_arrive_expect_tx(&m.full[stage], (outputs ? 2 : 1) * kBytesK + kBytesV);
+            const int t = seg0 + c * kLtChunk;
+            for (int i = 0; i < DK / 64; ++i) {
+                if (outputs) lt_tma(st + i * 8192, &map_q, i * 64, t, h, b, &m.full[stage]);
+                lt_tma(st + C::oK + i * 8192, &map_k, i * 64, t, hk, b, &m.full[stage]);
+            }
+            for (int i = 0; i < DV / 64; ++i) lt_tma(st + C::oV + i * 8192, &map_v, col0 + i * 64, t, hk, b, &m.full[stage]);
+            issued = c + 1;
+        }
+        // nothing is in flight when the CTA ends, not even where somebody gave up
+        for (int c = max(0, issued - C::kStages); c < issued; ++c) mbar_wait_bounded(&m.full[c % C::kStages], (c / C::kStages) & 1, kLtWaitLimit);
     }
     tc_fence_before();
     __syncthreads();
+    if (m.dead && tid == 0 && a.status != nullptr) atomicOr(a.status, FB_STATUS_WAIT_TIMEOUT);
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kLtTmemCols) : "memory");
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------
+
+// The driver's encoder of tensor maps, found through the runtime (the library does not link the driver).
+using LtEncode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static LtEncode lt_encoder() {
+    static const LtEncode fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &r) != cudaSuccess || r != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        cudaGetLastError();
+        return reinterpret_cast<LtEncode>(p);
+    }();
+    return fn;
+}
+
+// Whether [seq, token, head, channel] can be copied in boxes, and the map for it.
+static bool lt_encode(CUtensorMap* map, const void* base, const int64_t* stride, int channels, int tokens, int heads, int batch) {
+    const LtEncode fn = lt_encoder();
+    if (fn == nullptr) return false;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(channels), static_cast<cuuint64_t>(tokens), static_cast<cuuint64_t>(heads),
+                                static_cast<cuuint64_t>(batch)};
+    const int64_t by_dim[3] = {stride[1], stride[2], stride[0]};
+    cuuint64_t strides[3];
+    for (int i = 0; i < 3; ++i) {
+        const int64_t bytes = by_dim[i] * 2;
+        strides[i] = dims[i + 1] == 1 ? 16 : static_cast<cuuint64_t>(bytes);
+        if (dims[i + 1] > 1 && (bytes <= 0 || bytes >= (1ll << 40))) return false;
+    }
+    const cuuint32_t box[4] = {64, kLtChunk, 1, 1}, step[4] = {1, 1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class K>
+static int launch_chunk(K* kernel, dim3 grid, int threads, int bytes, cudaStream_t st, const LinArgs& a, const LtPlan& plan, const CUtensorMap* maps) {
+    FB_TRY(check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "linear_attention"));
+    return launch_after(kernel, grid, dim3(threads), bytes, st, false, "linear_attention", a, plan, maps[0], maps[1], maps[2]);
 }
 
 template <typename T, int DK, int DV>
@@ -465,26 +795,37 @@ static int launch_chunk(const LinArgs& a, cudaStream_t st) {
     using C = LtCfg<T, DK, DV>;
     constexpr int bytes = C::oMisc + static_cast<int>(sizeof(LtMisc));
     static_assert(bytes <= 232448, "shared memory");
-    const int tiles = (a.dv + DV - 1) / DV;
-    const int64_t ctas = static_cast<int64_t>(a.batch) * a.heads * tiles;
+    LtPlan plan = {};
+    plan.tiles = (a.dv + DV - 1) / DV;
+    plan.segs = 1;
+    const int64_t ctas = static_cast<int64_t>(a.batch) * a.heads * plan.tiles * plan.segs;
     FB_REQUIRE(ctas < (1ll << 31), "linear_attention: batch * heads is too large");
-    bool aligned = true;
+    plan.aligned = true;
     const void* base[3] = {a.q, a.k, a.v};
     const int64_t* stride[3] = {a.q_stride, a.k_stride, a.v_stride};
+    const int64_t sizes[3] = {a.batch, a.tokens, 0};
     for (int i = 0; i < 3; ++i) {
-        aligned = aligned && reinterpret_cast<uintptr_t>(base[i]) % 16 == 0;
-        for (int j = 0; j < 3; ++j) aligned = aligned && stride[i][j] * static_cast<int64_t>(sizeof(T)) % 16 == 0;
+        plan.aligned = plan.aligned && reinterpret_cast<uintptr_t>(base[i]) % 16 == 0;
+        for (int j = 0; j < 3; ++j) {
+            const int64_t size = j < 2 ? sizes[j] : i == 0 ? a.heads : a.kv_heads;
+            plan.aligned = plan.aligned && (size == 1 || stride[i][j] * static_cast<int64_t>(sizeof(T)) % 16 == 0);
+        }
     }
-    FB_TRY(check_cuda(cudaFuncSetAttribute(linattn_chunk_kernel<T, DK, DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "linear_attention"));
-    return launch_after(linattn_chunk_kernel<T, DK, DV>, dim3(static_cast<unsigned>(ctas)), dim3(kLtThreads), bytes, st, false, "linear_attention",
-                        a, tiles, aligned);
+    CUtensorMap maps[3] = {};
+    const bool tma = C::kBf16 && plan.aligned && lt_encode(&maps[0], a.q, a.q_stride, a.dk, a.tokens, a.heads, a.batch) &&
+               lt_encode(&maps[1], a.k, a.k_stride, a.dk, a.tokens, a.kv_heads, a.batch) &&
+               lt_encode(&maps[2], a.v, a.v_stride, a.dv, a.tokens, a.kv_heads, a.batch);
+    const dim3 grid(static_cast<unsigned>(ctas));
+    if constexpr (C::kBf16) {
+        if (tma) return launch_chunk(linattn_chunk_kernel<T, DK, DV, true>, grid, C::kThreads, bytes, st, a, plan, maps);
+    }
+    return launch_chunk(linattn_chunk_kernel<T, DK, DV, false>, grid, C::kThreads, bytes, st, a, plan, maps);
 }
 
 template <typename T>
 static int launch_chunk(const LinArgs& a, cudaStream_t st) {
-    constexpr int wide = std::is_same<T, float>::value ? 64 : 128;  // (fp32 operands of 128 x 128 do not fit shared memory)
-    if (a.dk <= 64) return a.dv <= 64 ? launch_chunk<T, 64, 64>(a, st) : launch_chunk<T, 64, wide>(a, st);
-    return a.dv <= 64 ? launch_chunk<T, 128, 64>(a, st) : launch_chunk<T, 128, wide>(a, st);
+    if (a.dk <= 64) return a.dv <= 64 ? launch_chunk<T, 64, 64>(a, st) : launch_chunk<T, 64, 128>(a, st);
+    return a.dv <= 64 ? launch_chunk<T, 128, 64>(a, st) : launch_chunk<T, 128, 128>(a, st);
 }
 
 int launch_linattn_chunk(const LinArgs& a, cudaStream_t st) {
