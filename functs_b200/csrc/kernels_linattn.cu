@@ -7,6 +7,7 @@
 
 namespace fb {
 
+constexpr int kLinFewTokens = 32;  // up to here token by token
 constexpr int kRecurThreads = 256;
 constexpr int kRecurTokens = 8;  // tokens staged at a time
 
@@ -134,8 +135,9 @@ static int launch_recurrent(const LinArgs& a, cudaStream_t st) {
 }  // namespace fb
 
 extern "C" int64_t functs_b200_linear_attention_scratch_bytes(const functs_b200_linear_attention_args* a) {
-    (void)a;
-    return 0;
+    using namespace fb;
+    if (a == nullptr || a->batch <= 0 || a->heads <= 0 || a->dk <= 0 || a->dv <= 0 || a->tokens <= kLinFewTokens) return 0;
+    return linattn_chunk_scratch_bytes(*a);
 }
 
 extern "C" int functs_b200_linear_attention(const functs_b200_linear_attention_args* args, void* scratch, void* stream) {
@@ -152,9 +154,8 @@ extern "C" int functs_b200_linear_attention(const functs_b200_linear_attention_a
     if (a.batch == 0) return FB_OK;
     FB_REQUIRE(a.log_decay != nullptr && a.state_out != nullptr, "linear_attention: null pointer");
     FB_REQUIRE(a.tokens == 0 || (a.q != nullptr && a.k != nullptr && a.v != nullptr && a.out != nullptr), "linear_attention: null pointer");
-    (void)scratch;
     const cudaStream_t st = as_stream(stream);
-    if (a.tokens > 32) return launch_linattn_chunk(a, st);
+    if (a.tokens > kLinFewTokens) return launch_linattn_chunk(a, scratch, st);
     if (a.dtype == FB_DTYPE_F32) return launch_recurrent<float>(a, st);
     if (a.dtype == FB_DTYPE_F16) return launch_recurrent<__half>(a, st);
     return launch_recurrent<__nv_bfloat16>(a, st);

@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(LtCfg<T, DK, DV>::kThreads, 1)
 linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                      const __grid_constant__ CUtensorMap map_v) {
     using C = LtCfg<T, DK, DV>;
-    constexpr int kWarpsW = C::kWarpsW;
+    constexpr int kWarpsW = C::kWarpsW + (TMA ? 2 : 0);  // (two more of the P group, where they do not load as well)
     extern __shared__ __align__(1024) unsigned char smem[];
     LtMisc& m = *reinterpret_cast<LtMisc*>(smem + C::oMisc);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -272,6 +272,7 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
     const int tile = rest % plan.tiles, h = (rest / plan.tiles) % a.heads, order = rest / (plan.tiles * a.heads);
     const int hk = h / (a.heads / a.kv_heads), col0 = tile * DV, dv = min(DV, a.dv - col0);
 
+    if (plan.mode == 1) pdl_launch_dependents();
     // long sequences first, so that the last CTAs are short ones
     if (tid == 0) m.b = order;
     __syncthreads();
@@ -354,6 +355,7 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&m.tmem)), "r"(kLtTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    if (plan.mode == 2) pdl_wait();  // (the parts' states)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -450,10 +452,10 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
             lt_arrive_read(&m.u_free, lane);
             if (!last) lt_arrive_read(&m.s_full, lane);  // (one more would be a phase ahead of the products' wait for this one)
         }
-    } else if (warp < C::kFirstO) {
+    } else if (warp < C::kFirstO || (TMA && warp >= C::kFirstP + 6)) {
         // ---- W (and tiles)
         constexpr int threads = 32 * kWarpsW;
-        const int id = tid - 32 * C::kFirstW;
+        const int rank = warp < C::kFirstO ? warp - C::kFirstW : warp - (C::kFirstP + 6) + C::kWarpsW, id = rank * 32 + lane;
         const T* q = static_cast<const T*>(a.q) + b * a.q_stride[0] + h * a.q_stride[2] + seg0 * a.q_stride[1];
         const T* k = static_cast<const T*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2] + seg0 * a.k_stride[1];
         const T* v = static_cast<const T*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2] + seg0 * a.v_stride[1] + col0;
@@ -469,7 +471,7 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
                     *reinterpret_cast<uint4*>(st + C::oK + lt_swizzled(i % (DK / 8), n + i / (DK / 8))) = make_uint4(0, 0, 0, 0);
             } else {
                 if (c >= C::kStages && !lt_wait(m, &m.empty[stage], turn ^ 1u)) break;
-                static_assert(kLtChunk * DK / 8 / threads % 2 == 0, "pieces");
+                static_assert(TMA || kLtChunk * DK / 8 / threads % 2 == 0, "pieces");
 #pragma unroll 1
                 for (int i0 = 0; i0 < kLtChunk * DK / 8 / threads; i0 += 2) {
                     float x[2][8], y[2][8];
@@ -491,24 +493,26 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
             // V, and W (free when the product before that has it is done)
             if (c >= C::kStages && !lt_wait(m, &m.w_free[stage], turn ^ 1u)) break;
             unsigned char* wt = smem + C::oW + stage * C::NW * C::kTileV;
-            constexpr int kPieces = kLtChunk * DV / 8 / threads, kBatch = 2;  // of a thread; on their way together
-            static_assert(kPieces % kBatch == 0, "pieces");
+            // a warp's piece: 16 bytes of eight tokens beside one another, four groups of channels; two on their way together
+            constexpr int kPieces = kLtChunk * DV / 256;
 #pragma unroll 1
-            for (int i0 = 0; i0 < kPieces; i0 += kBatch) {
-                const auto token_of = [&](int i) { return (i & 7) | ((i >> 5) & 7) << 3; };  // eight tokens beside one another, four groups
-                const auto group_of = [&](int i) { return ((i >> 3) & 3) | (i >> 8) << 2; };
+            for (int i0 = rank; i0 < kPieces; i0 += 2 * kWarpsW) {
+                const auto token_of = [&](int i) { return (i & 7) * 8 + (lane & 7); };
+                const auto group_of = [&](int i) { return (i >> 3) * 4 + (lane >> 3); };
                 if (TMA) {
-                    uint4 u[kBatch];
+                    uint4 u[2];
 #pragma unroll
-                    for (int j = 0; j < kBatch; ++j) {
-                        const int i = id + (i0 + j) * threads, t = token_of(i);
+                    for (int j = 0; j < 2; ++j) {
+                        const int i = i0 + j * kWarpsW, t = token_of(i);
+                        if (i >= kPieces) continue;
                         uint4* vp = reinterpret_cast<uint4*>(st + C::oV + lt_swizzled(group_of(i), t));
                         if (t >= n) *vp = make_uint4(0, 0, 0, 0);
                         u[j] = *vp;
                     }
 #pragma unroll
-                    for (int j = 0; j < kBatch; ++j) {
-                        const int i = id + (i0 + j) * threads, t = token_of(i), g = group_of(i), back = t < n ? n - 1 - t : 0;
+                    for (int j = 0; j < 2; ++j) {
+                        const int i = i0 + j * kWarpsW, t = token_of(i), g = group_of(i), back = t < n ? n - 1 - t : 0;
+                        if (i >= kPieces) continue;
                         uint32_t w4[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
                         lt_weigh(wt + lt_plain(g, t), C::kTileV, w4, m.weight[back], m.weight2[back]);
                         uint32_t high = 0;
@@ -526,15 +530,16 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
                         }
                     }
                 } else {
-                    float x[kBatch][8];
+                    float x[2][8];
 #pragma unroll
-                    for (int j = 0; j < kBatch; ++j) {
-                        const int i = id + (i0 + j) * threads, t = token_of(i), g = group_of(i);
-                        lt_load8(v + (t0 + t) * a.v_stride[1] + g * 8, t < n ? max(0, min(8, dv - g * 8)) : 0, plan.aligned, x[j]);
+                    for (int j = 0; j < 2; ++j) {
+                        const int i = i0 + j * kWarpsW, t = token_of(i), g = group_of(i);
+                        if (i < kPieces) lt_load8(v + (t0 + t) * a.v_stride[1] + g * 8, t < n ? max(0, min(8, dv - g * 8)) : 0, plan.aligned, x[j]);
                     }
 #pragma unroll
-                    for (int j = 0; j < kBatch; ++j) {
-                        const int i = id + (i0 + j) * threads, t = token_of(i), g = group_of(i);
+                    for (int j = 0; j < 2; ++j) {
+                        const int i = i0 + j * kWarpsW, t = token_of(i), g = group_of(i);
+                        if (i >= kPieces) continue;
                         const float w = m.power[t < n ? n - 1 - t : 0];
                         float y[8];
 #pragma unroll
@@ -784,20 +789,79 @@ static bool lt_encode(CUtensorMap* map, const void* base, const int64_t* stride,
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// The states in front of a sequence's parts, from what each part adds, and the state behind the last one.  One thread per cell of S: the
+// parts' decays are products of decays of whole parts.
+__global__ void __launch_bounds__(256) linattn_carry_kernel(const LinArgs a, float* __restrict__ states, int segs, int seg_tokens) {
+    const int64_t cells = static_cast<int64_t>(a.dk) * a.dv, cell = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int h = blockIdx.y % a.heads, b = blockIdx.y / a.heads, lane = threadIdx.x & 31;
+    int bits;
+    const int slot = lin_slot(a, b, lane, bits);
+    pdl_wait();
+    if (slot < 0 || cell >= cells) return;
+    const int length = lin_length(a, b);
+    const int64_t own = (static_cast<int64_t>(slot) * a.heads + h) * cells + cell;
+    float* part = states + (static_cast<int64_t>(b) * a.heads + h) * segs * cells + cell;
+    float s = a.state_in != nullptr ? a.state_in[own] : 0.0f;
+    const float log_decay = a.log_decay[h];
+    for (int i = 0; i < segs; ++i) {
+        const int n = min(max(length - i * seg_tokens, 0), i + 1 < segs ? seg_tokens : length);
+        const float added = part[i * cells];
+        part[i * cells] = s;
+        s = fmaf(lin_decay(log_decay, n), s, added);
+    }
+    a.state_out[own] = s;
+}
+
+// How many parts a sequence is cut into.  Cutting costs a second reading of K and V for the states of the parts (about 0.4 of a chunk's time
+// for each of its chunks) and two more launches, so it pays where whole sequences leave SMs without work.
+static void lt_cut(const LinArgs& a, int64_t rows, int& segs, int& seg_tokens) {
+    const int chunks = (a.tokens + kLtChunk - 1) / kLtChunk;
+    segs = 1;
+    seg_tokens = 0;
+    const double whole = static_cast<double>((rows + kNumSMs - 1) / kNumSMs) * chunks;
+    double best = whole;
+    for (int n = 2; n <= 64 && n * 4 <= chunks; ++n) {
+        const int each = (chunks + n - 1) / n;
+        const int parts = (chunks + each - 1) / each;
+        const double cost = static_cast<double>((rows * parts + kNumSMs - 1) / kNumSMs) * (each * 1.4 + 1.0) + 4.0;
+        if (cost < best) {
+            best = cost;
+            segs = parts;
+            seg_tokens = each * kLtChunk;
+        }
+    }
+}
+
+int64_t linattn_chunk_scratch_bytes(const LinArgs& a) {
+    int segs, seg_tokens;
+    lt_cut(a, static_cast<int64_t>(a.batch) * a.heads, segs, seg_tokens);
+    return segs == 1 ? 0 : static_cast<int64_t>(a.batch) * a.heads * segs * a.dk * a.dv * 4;
+}
+
 template <class K>
-static int launch_chunk(K* kernel, dim3 grid, int threads, int bytes, cudaStream_t st, const LinArgs& a, const LtPlan& plan, const CUtensorMap* maps) {
+static int launch_chunk(K* kernel, dim3 grid, int threads, int bytes, cudaStream_t st, const LinArgs& a, LtPlan plan, const CUtensorMap* maps) {
     FB_TRY(check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "linear_attention"));
-    return launch_after(kernel, grid, dim3(threads), bytes, st, false, "linear_attention", a, plan, maps[0], maps[1], maps[2]);
+    if (plan.segs == 1) return launch_after(kernel, grid, dim3(threads), bytes, st, false, "linear_attention", a, plan, maps[0], maps[1], maps[2]);
+    plan.mode = 1;
+    FB_TRY(launch_after(kernel, grid, dim3(threads), bytes, st, false, "linear_attention", a, plan, maps[0], maps[1], maps[2]));
+    const dim3 carry(static_cast<unsigned>((a.dk * a.dv + 255) / 256), static_cast<unsigned>(a.batch * a.heads));
+    FB_TRY(launch_after(linattn_carry_kernel, carry, dim3(256), 0, st, true, "linear_attention", a, plan.states, plan.segs, plan.seg_tokens));
+    plan.mode = 2;
+    return launch_after(kernel, grid, dim3(threads), bytes, st, true, "linear_attention", a, plan, maps[0], maps[1], maps[2]);
 }
 
 template <typename T, int DK, int DV>
-static int launch_chunk(const LinArgs& a, cudaStream_t st) {
+static int launch_chunk(const LinArgs& a, void* scratch, cudaStream_t st) {
     using C = LtCfg<T, DK, DV>;
     constexpr int bytes = C::oMisc + static_cast<int>(sizeof(LtMisc));
     static_assert(bytes <= 232448, "shared memory");
     LtPlan plan = {};
     plan.tiles = (a.dv + DV - 1) / DV;
-    plan.segs = 1;
+    const int64_t rows = static_cast<int64_t>(a.batch) * a.heads;
+    lt_cut(a, rows, plan.segs, plan.seg_tokens);
+    if (rows > 65535) plan.segs = 1;
+    FB_REQUIRE(plan.segs == 1 || (scratch != nullptr && reinterpret_cast<uintptr_t>(scratch) % 16 == 0), "linear_attention: scratch must be given, 16-byte aligned");
+    plan.states = static_cast<float*>(scratch);
     const int64_t ctas = static_cast<int64_t>(a.batch) * a.heads * plan.tiles * plan.segs;
     FB_REQUIRE(ctas < (1ll << 31), "linear_attention: batch * heads is too large");
     plan.aligned = true;
@@ -823,15 +887,15 @@ static int launch_chunk(const LinArgs& a, cudaStream_t st) {
 }
 
 template <typename T>
-static int launch_chunk(const LinArgs& a, cudaStream_t st) {
-    if (a.dk <= 64) return a.dv <= 64 ? launch_chunk<T, 64, 64>(a, st) : launch_chunk<T, 64, 128>(a, st);
-    return a.dv <= 64 ? launch_chunk<T, 128, 64>(a, st) : launch_chunk<T, 128, 128>(a, st);
+static int launch_chunk(const LinArgs& a, void* scratch, cudaStream_t st) {
+    if (a.dk <= 64) return a.dv <= 64 ? launch_chunk<T, 64, 64>(a, scratch, st) : launch_chunk<T, 64, 128>(a, scratch, st);
+    return a.dv <= 64 ? launch_chunk<T, 128, 64>(a, scratch, st) : launch_chunk<T, 128, 128>(a, scratch, st);
 }
 
-int launch_linattn_chunk(const LinArgs& a, cudaStream_t st) {
-    if (a.dtype == FB_DTYPE_F32) return launch_chunk<float>(a, st);
-    if (a.dtype == FB_DTYPE_F16) return launch_chunk<__half>(a, st);
-    return launch_chunk<__nv_bfloat16>(a, st);
+int launch_linattn_chunk(const LinArgs& a, void* scratch, cudaStream_t st) {
+    if (a.dtype == FB_DTYPE_F32) return launch_chunk<float>(a, scratch, st);
+    if (a.dtype == FB_DTYPE_F16) return launch_chunk<__half>(a, scratch, st);
+    return launch_chunk<__nv_bfloat16>(a, scratch, st);
 }
 
 }  // namespace fb

@@ -12,7 +12,9 @@ using LinArgs = functs_b200_linear_attention_args;
 
 constexpr int kLinMaxDim = 128;
 
-int launch_linattn_chunk(const LinArgs& a, cudaStream_t st);  // kernels_linattn_tc.cu
+// kernels_linattn_tc.cu
+int64_t linattn_chunk_scratch_bytes(const LinArgs& a);
+int launch_linattn_chunk(const LinArgs& a, void* scratch, cudaStream_t st);
 
 #ifdef __CUDACC__
 

@@ -81,7 +81,7 @@ def decays(h, seed=1):
 SHAPES = [
     # b, t, h, hk, dk, dv
     (1, 1, 1, 1, 1, 1), (2, 1, 3, 1, 128, 128), (3, 2, 4, 2, 17, 33), (1, 7, 2, 2, 64, 64), (2, 63, 2, 2, 128, 128), (2, 64, 2, 1, 128, 64),
-    (1, 65, 3, 3, 64, 128), (3, 129, 4, 2, 80, 48), (1, 200, 2, 2, 37, 5), (1, 700, 3, 3, 128, 128), (2, 333, 2, 2, 64, 64), (2, 130, 1, 1, 96, 112),
+    (1, 65, 3, 3, 64, 128), (3, 129, 4, 2, 80, 48), (1, 200, 2, 2, 37, 5), (1, 700, 3, 3, 128, 128), (2, 333, 2, 2, 64, 64), (2, 130, 1, 1, 96, 112), (1, 1500, 3, 1, 128, 128), (2, 2113, 1, 1, 64, 40),
 ]
 
 
@@ -98,7 +98,7 @@ def test_prompt(ops, shape, dtype):
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("layout", ["fused", "time", "heads", "odd"])
-@pytest.mark.parametrize("shape", [(3, 150, 4, 2, 64, 64), (2, 70, 6, 3, 128, 128), (5, 9, 4, 4, 40, 72)], ids=str)
+@pytest.mark.parametrize("shape", [(3, 150, 4, 2, 64, 64), (2, 70, 6, 3, 128, 128), (5, 9, 4, 4, 40, 72), (4, 1300, 2, 1, 128, 64)], ids=str)
 def test_prompt_lengths_pool_and_layouts(ops, shape, layout, dtype):
     """Sequences of uneven lengths (none, one, all tokens) that go on from states in any order; rows behind them are not read."""
     b, t, h, hk, dk, dv = shape
