@@ -37,7 +37,6 @@ namespace fb {
 constexpr int kLtChunk = 64;
 constexpr int kLtWarpsS = 8, kLtWarpsP = 8;  // (of the P group four make P, one issues products, one copies)
 constexpr uint32_t kLtWaitLimit = 1000000u;
-constexpr int kLtMarks = 4;  // chunks whose marks of values that are not finite are kept
 // TMEM columns: U, X, Y (and, before it, G), S^T in fp32 and as two operand parts of DK / 2 columns, or as three parts, which are exact
 constexpr uint32_t kLtU = 0, kLtX = 128, kLtY = 192, kLtS = 256, kLtTmemCols = 512;
 
@@ -48,19 +47,19 @@ struct LtCfg {
     static constexpr int NX = kBf16 ? 1 : std::is_same<T, __half>::value ? 2 : 3;  // parts of q, k, v
     static constexpr int NS = std::is_same<T, float>::value ? 3 : 2;               // parts of S and P
     static constexpr int NW = 3;                                                   // parts of W
-    static constexpr int kStages = kBf16 ? 2 : 1;                                  // of Q, K and V, and of W
+    static constexpr int kStages = kBf16 ? 2 : 1;   // of Q and K, and of W
+    static constexpr int kStagesV = kBf16 ? 3 : 1;  // (V is read a chunk ahead, for W)
     static constexpr int kWarpsW = kBf16 ? 4 : 8, kWarpsO = kBf16 ? 8 : 4;
     static constexpr int kFirstW = kLtWarpsS, kFirstO = kFirstW + kWarpsW, kFirstP = kFirstO + kWarpsO, kThreads = 32 * (kFirstP + kLtWarpsP);
     static_assert(kFirstO % 4 == 0 && kFirstP % 4 == 0, "a warp's TMEM lanes go by its number");
     static constexpr int kTileK = kLtChunk * DK * 2, kTileV = kLtChunk * DV * 2, kPartP = kLtChunk * kLtChunk * 2;
-    static constexpr int kStage = NX * (2 * kTileK + kTileV);
-    static constexpr int oK = NX * kTileK, oV = 2 * NX * kTileK;  // in a stage, behind Q
-    static constexpr int oW = kStages * kStage, oP = oW + kStages * NW * kTileV, oMisc = oP + NS * kPartP;
+    static constexpr int kStage = 2 * NX * kTileK, oK = NX * kTileK;  // Q, and K behind it
+    static constexpr int oV = kStages * kStage, oW = oV + kStagesV * NX * kTileV, oP = oW + kStages * NW * kTileV, oMisc = oP + NS * kPartP;
     static constexpr uint32_t kParts = NS == 3 ? kLtS : kLtS + 128;  // TMEM columns of the parts of S^T
 };
 
 struct LtMisc {
-    uint64_t full[2], empty[2], w_full[2], w_free[2];  // stages
+    uint64_t full[2], full_v[3], empty[2], w_full[2], w_free[2];  // stages
     uint64_t g_full, u_full, u_free, s_full, x_full, p_full, y_full, xy_free;
     uint32_t tmem;
     int dead;                                      // a wait ran out
@@ -70,8 +69,8 @@ struct LtMisc {
     __align__(16) float scaled_next[kLtChunk];        // scale * decay^(i+1)
     uint2 weight[kLtChunk];                        // decay^i as three bf16 parts, each twice: w0 w0, w1 w1 (w2 below)
     uint32_t weight2[kLtChunk];
-    int any_bad[kLtMarks];                         // 1 + the last chunk that marked some
-    int first_bad[kLtMarks][128];                  // per channel: (how far the chunk is from 2^24, the first such token)
+    int bad;                                       // the first token with a V that is not finite
+    int first_bad[128];                            // the same per channel (behind it the channel's state is not finite either)
 };
 
 struct LtPlan {
@@ -332,10 +331,9 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
             m.power_off = near > 0.0f ? fabsf(off) / near : 0.0f;
         }
     }
-    if (tid < 128) {
-        for (int i = 0; i < kLtMarks; ++i) m.first_bad[i][tid] = 0x7fffffff;
-    }
+    if (tid < 128) m.first_bad[tid] = 0x7fffffff;
     if (tid == 0) {
+        for (int i = 0; i < C::kStagesV; ++i) mbar_init(&m.full_v[i], 1);
         for (int i = 0; i < C::kStages; ++i) {
             mbar_init(&m.full[i], TMA ? 1 : kWarpsW);
             mbar_init(&m.empty[i], 1);
@@ -349,7 +347,7 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
         mbar_init(&m.xy_free, C::kWarpsO);
         fence_barrier_init();
         m.dead = 0;
-        for (int i = 0; i < kLtMarks; ++i) m.any_bad[i] = 0;
+        m.bad = 0x7fffffff;
     }
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&m.tmem)), "r"(kLtTmemCols) : "memory");
@@ -460,13 +458,13 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
         const T* k = static_cast<const T*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2] + seg0 * a.k_stride[1];
         const T* v = static_cast<const T*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2] + seg0 * a.v_stride[1] + col0;
         for (int c = 0; c < chunks; ++c) {
-            const int t0 = c * kLtChunk, n = min(kLtChunk, seg_end - seg0 - t0), stage = c % C::kStages, mark = c % kLtMarks;
+            const int t0 = c * kLtChunk, n = min(kLtChunk, seg_end - seg0 - t0), stage = c % C::kStages;
             const uint32_t turn = (c / C::kStages) & 1;
-            unsigned char* st = smem + stage * C::kStage;
-            bool bad = false;
+            unsigned char *st = smem + stage * C::kStage, *vt = smem + C::oV + (c % C::kStagesV) * C::NX * C::kTileV;
             if (TMA) {
-                if (!lt_wait(m, &m.full[stage], turn)) break;
+                if (!lt_wait(m, &m.full_v[c % C::kStagesV], (c / C::kStagesV) & 1)) break;
                 // rows behind the sequence are somebody's: K (here) and V (below) must be zero there; Q's make rows that nobody reads
+                if (n < kLtChunk && !lt_wait(m, &m.full[stage], turn)) break;
                 for (int i = id; i < (kLtChunk - n) * (DK / 8); i += threads)
                     *reinterpret_cast<uint4*>(st + C::oK + lt_swizzled(i % (DK / 8), n + i / (DK / 8))) = make_uint4(0, 0, 0, 0);
             } else {
@@ -505,7 +503,7 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
                     for (int j = 0; j < 2; ++j) {
                         const int i = i0 + j * kWarpsW, t = token_of(i);
                         if (i >= kPieces) continue;
-                        uint4* vp = reinterpret_cast<uint4*>(st + C::oV + lt_swizzled(group_of(i), t));
+                        uint4* vp = reinterpret_cast<uint4*>(vt + lt_swizzled(group_of(i), t));
                         if (t >= n) *vp = make_uint4(0, 0, 0, 0);
                         u[j] = *vp;
                     }
@@ -519,14 +517,14 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
 #pragma unroll
                         for (int e = 0; e < 4; ++e) high = __vmaxu2(high, w4[e] & 0x7FFF7FFFu);
                         if ((high & 0xFFFFu) >= 0x7F80u || high >= 0x7F800000u) {
-                            bad = true;
+                            atomicMin(&m.bad, t0 + t);
 #pragma unroll
                             for (int e = 0; e < 8; ++e) {
                                 if (((w4[e / 2] >> (16 * (e & 1))) & 0x7F80u) != 0x7F80u) continue;
                                 w4[e / 2] &= (e & 1) != 0 ? 0x0000FFFFu : 0xFFFF0000u;
-                                atomicMin(&m.first_bad[mark][g * 8 + e], ((1 << 24) - c) * kLtChunk + t);
+                                atomicMin(&m.first_bad[g * 8 + e], t0 + t);
                             }
-                            *reinterpret_cast<uint4*>(st + C::oV + lt_swizzled(g, t)) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+                            *reinterpret_cast<uint4*>(vt + lt_swizzled(g, t)) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
                         }
                     }
                 } else {
@@ -548,15 +546,14 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             if (lt_finite(x[j][e])) continue;
-                            bad = true;
+                            atomicMin(&m.bad, t0 + t);
                             x[j][e] = 0.0f;
-                            atomicMin(&m.first_bad[mark][g * 8 + e], ((1 << 24) - c) * kLtChunk + t);
+                            atomicMin(&m.first_bad[g * 8 + e], t0 + t);
                         }
-                        lt_store_parts<C::NX>(st + C::oV + lt_swizzled(g, t), C::kTileV, x[j]);
+                        lt_store_parts<C::NX>(vt + lt_swizzled(g, t), C::kTileV, x[j]);
                     }
                 }
             }
-            if (bad) *reinterpret_cast<volatile int*>(&m.any_bad[mark]) = c + 1;
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
@@ -574,12 +571,7 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
             for (int c = 0; c < chunks; ++c) {
                 if (!lt_wait(m, &m.y_full, c & 1)) break;
                 tc_fence_after();
-                const int mark = c % kLtMarks;
-                int first = kLtChunk;
-                if (*reinterpret_cast<volatile int*>(&m.any_bad[mark]) == c + 1) {
-                    const int at = m.first_bad[mark][row];
-                    if ((at >> 6) == (1 << 24) - c) first = at & 63;
-                }
+                const int first = *reinterpret_cast<volatile int*>(&m.bad) < (c + 1) * kLtChunk ? m.first_bad[row] - c * kLtChunk : kLtChunk;
 #pragma unroll 1
                 for (int block = token0; block < token0 + kShare; block += 32) {
                     T o[32];
@@ -669,7 +661,9 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
                             }
             };
             const auto make_u = [&](int c) {  // U^T = W^T K
-                if (!wait(&m.w_full[c % C::kStages], (c / C::kStages) & 1) || (c > 0 && !wait(&m.u_free, (c - 1) & 1))) return false;
+                if (!wait(&m.w_full[c % C::kStages], (c / C::kStages) & 1) || !wait(&m.full[c % C::kStages], (c / C::kStages) & 1) ||
+                    (c > 0 && !wait(&m.u_free, (c - 1) & 1)))
+                    return false;
                 tc_fence_after();
                 if (lt_elect()) {
                     const uint64_t dk = lt_desc_swizzled(base + (c % C::kStages) * C::kStage + C::oK, 8192, 1024),
@@ -690,8 +684,8 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
                 if (outputs) {
                     const uint32_t at = base + (c % C::kStages) * C::kStage;
                     const uint64_t dq = lt_desc_swizzled(at, 16, 1024), dk = lt_desc_swizzled(at + C::oK, 16, 1024),
-                                   dv = lt_desc_swizzled(at + C::oV, 8192, 1024);
-                    ok = wait(&m.full[c % C::kStages], (c / C::kStages) & 1) && (c == 0 || wait(&m.xy_free, (c - 1) & 1));
+                                   dv = lt_desc_swizzled(base + C::oV + (c % C::kStagesV) * C::NX * C::kTileV, 8192, 1024);
+                    ok = c == 0 || wait(&m.xy_free, (c - 1) & 1);
                     if (!ok) break;
                     tc_fence_after();
                     if (lt_elect()) {  // G = Q K^T
@@ -729,24 +723,32 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
             }
         }
     } else if (TMA && warp == C::kFirstP + 3 && lane == 0) {
-        // ---- the copies
-        constexpr uint32_t kBytesK = C::kTileK, kBytesV = C::kTileV;
-        int issued = 0;
+        // ---- the copies: Q and K of a chunk and V of the next
+        int issued = 0, issued_v = 0;
+        const auto copy_v = [&](int c) {
+            uint64_t* bar = &m.full_v[c % C::kStagesV];
+            mbar_arrive_expect_tx(bar, C::kTileV);
+            for (int i = 0; i < DV / 64; ++i)
+                lt_tma(smem + C::oV + (c % C::kStagesV) * C::kTileV + i * 8192, &map_v, col0 + i * 64, seg0 + c * kLtChunk, hk, b, bar);
+            issued_v = c + 1;
+        };
+        if (chunks > 0) copy_v(0);
         for (int c = 0; c < chunks; ++c) {
             const int stage = c % C::kStages;
             if (c >= C::kStages && !lt_wait_one(m, &m.empty[stage], ((c / C::kStages) & 1) ^ 1u)) break;
             unsigned char* st = smem + stage * C::kStage;
-            mbar_arrive_expect_tx(&m.full[stage], (outputs ? 2 : 1) * kBytesK + kBytesV);
-            const int t = seg0 + c * kLtChunk;
+            mbar_arrive_expect_tx(&m.full[stage], (outputs ? 2 : 1) * C::kTileK);
             for (int i = 0; i < DK / 64; ++i) {
-                if (outputs) lt_tma(st + i * 8192, &map_q, i * 64, t, h, b, &m.full[stage]);
-                lt_tma(st + C::oK + i * 8192, &map_k, i * 64, t, hk, b, &m.full[stage]);
+                if (outputs) lt_tma(st + i * 8192, &map_q, i * 64, seg0 + c * kLtChunk, h, b, &m.full[stage]);
+                lt_tma(st + C::oK + i * 8192, &map_k, i * 64, seg0 + c * kLtChunk, hk, b, &m.full[stage]);
             }
-            for (int i = 0; i < DV / 64; ++i) lt_tma(st + C::oV + i * 8192, &map_v, col0 + i * 64, t, hk, b, &m.full[stage]);
             issued = c + 1;
+            if (c + 1 < chunks) copy_v(c + 1);
         }
         // nothing is in flight when the CTA ends, not even where somebody gave up
         for (int c = max(0, issued - C::kStages); c < issued; ++c) mbar_wait_bounded(&m.full[c % C::kStages], (c / C::kStages) & 1, kLtWaitLimit);
+        for (int c = max(0, issued_v - C::kStagesV); c < issued_v; ++c)
+            mbar_wait_bounded(&m.full_v[c % C::kStagesV], (c / C::kStagesV) & 1, kLtWaitLimit);
     }
     tc_fence_before();
     __syncthreads();
