@@ -20,8 +20,9 @@
 //   S   8 warps: S' = l^n S + U in TMEM, a channel of V per thread, half of the channels of K; S' as operand parts
 //   W   W from V (and, where tiles cannot be had by TMA, or are split into parts, the tiles themselves)
 //   O   the outputs from X and Y
-//   P   P from G: four warps (there are 64 rows); beside them one warp that issues the products, in the order U, G, X, Y, so that there is
-//       always one to run while the threads are at the next, and one that issues the copies
+//   P   P from G: four warps (there are 64 rows)
+//   beside these, one warp issues U and G, one X and Y, so that the tensor core has work while either waits, and one issues the copies.
+// G of the next chunk is formed in U's columns as soon as they have been read, so P is ready long before its product's turn.
 //
 // NaN and infinities: a masked entry of P is 0 by selection, but 0 * V is not 0 for a V that is not finite, so such entries are taken as 0 in
 // Y (not in W) and the outputs of their channel, from their token on, are set to NaN.
@@ -35,10 +36,10 @@
 namespace fb {
 
 constexpr int kLtChunk = 64;
-constexpr int kLtWarpsS = 8, kLtWarpsP = 8;  // (of the P group four make P, one issues products, one copies)
+constexpr int kLtWarpsS = 8, kLtWarpsP = 8;  // (of the P group four make P, two issue products, one copies)
 constexpr uint32_t kLtWaitLimit = 1000000u;
-// TMEM columns: U, X, Y (and, before it, G), S^T in fp32 and as two operand parts of DK / 2 columns, or as three parts, which are exact
-constexpr uint32_t kLtU = 0, kLtX = 128, kLtY = 192, kLtS = 256, kLtTmemCols = 512;
+// TMEM columns: U (and, between two of them, G), X, Y, S^T in fp32 and as two operand parts of DK / 2 columns, or as three parts, which are exact
+constexpr uint32_t kLtU = 0, kLtG = 0, kLtX = 128, kLtY = 192, kLtS = 256, kLtTmemCols = 512;
 
 template <typename T, int DK_, int DV_>
 struct LtCfg {
@@ -59,8 +60,8 @@ struct LtCfg {
 };
 
 struct LtMisc {
-    uint64_t full[2], full_v[3], empty[2], w_full[2], w_free[2];  // stages
-    uint64_t g_full, u_full, u_free, s_full, x_full, p_full, y_full, xy_free;
+    uint64_t full[2], full_v[3], v_whole[3], empty[2], w_full[2], w_free[2];  // stages; v_whole: V with zeros where it must have them
+    uint64_t g_full, g_read, u_full, u_free, s_full, x_full, p_full, y_full, xy_free;
     uint32_t tmem;
     int dead;                                      // a wait ran out
     int b;
@@ -234,16 +235,16 @@ __device__ __forceinline__ void lt_load8(const T* p, int valid, bool aligned, fl
 // Eight bf16 values times a weight of three parts, as three parts, in bf16 arithmetic: with a fused multiply-add that rounds once, products
 // and their errors are exact.  v w0 = p + r and v w1 = t0 + t1; r + t0 = s + e (D. Knuth, The Art of Computer Programming, volume 2, 4.2.2,
 // theorem B); the parts are p, s and e + t1 + v w2, which is rounded below 2^-25 of the product.
-__device__ __forceinline__ void lt_weigh(unsigned char* at, int stride, const uint32_t (&v)[4], uint2 w01, uint32_t w2) {
+__device__ __forceinline__ void lt_weigh(unsigned char* at, int stride, const uint32_t (&v)[4], const uint32_t (&w)[3]) {
     const auto bf = [](const uint32_t& u) { return *reinterpret_cast<const __nv_bfloat162*>(&u); };
     uint32_t part[3][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 x = bf(v[i]), w0 = bf(w01.x), w1 = bf(w01.y);
+        const __nv_bfloat162 x = bf(v[i]), w0 = bf(w[0]), w1 = bf(w[1]);
         const __nv_bfloat162 p = __hmul2_rn(x, w0), r = __hfma2(x, w0, __hneg2(p)), t0 = __hmul2_rn(x, w1), t1 = __hfma2(x, w1, __hneg2(t0));
         const __nv_bfloat162 s = __hadd2_rn(r, t0), rest = __hsub2_rn(s, r);
         const __nv_bfloat162 e = __hadd2_rn(__hsub2_rn(r, __hsub2_rn(s, rest)), __hsub2_rn(t0, rest));
-        const __nv_bfloat162 q = __hadd2_rn(e, __hfma2(x, bf(w2), t1));
+        const __nv_bfloat162 q = __hadd2_rn(e, __hfma2(x, bf(w[2]), t1));
         part[0][i] = *reinterpret_cast<const uint32_t*>(&p);
         part[1][i] = *reinterpret_cast<const uint32_t*>(&s);
         part[2][i] = *reinterpret_cast<const uint32_t*>(&q);
@@ -263,7 +264,7 @@ __global__ void __launch_bounds__(LtCfg<T, DK, DV>::kThreads, 1)
 linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                      const __grid_constant__ CUtensorMap map_v) {
     using C = LtCfg<T, DK, DV>;
-    constexpr int kWarpsW = C::kWarpsW + (TMA ? 2 : 0);  // (two more of the P group, where they do not load as well)
+    constexpr int kWarpsW = C::kWarpsW;
     extern __shared__ __align__(1024) unsigned char smem[];
     LtMisc& m = *reinterpret_cast<LtMisc*>(smem + C::oMisc);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -333,15 +334,16 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
     }
     if (tid < 128) m.first_bad[tid] = 0x7fffffff;
     if (tid == 0) {
-        for (int i = 0; i < C::kStagesV; ++i) mbar_init(&m.full_v[i], 1);
+        for (int i = 0; i < C::kStagesV; ++i) mbar_init(&m.full_v[i], 1), mbar_init(&m.v_whole[i], kWarpsW);
         for (int i = 0; i < C::kStages; ++i) {
             mbar_init(&m.full[i], TMA ? 1 : kWarpsW);
-            mbar_init(&m.empty[i], 1);
+            mbar_init(&m.empty[i], outputs ? 2 : 1);
             mbar_init(&m.w_full[i], kWarpsW);
             mbar_init(&m.w_free[i], 1);
         }
         mbar_init(&m.g_full, 1), mbar_init(&m.u_full, 1), mbar_init(&m.x_full, 1), mbar_init(&m.y_full, 1);
         mbar_init(&m.p_full, 4);
+        mbar_init(&m.g_read, 4);
         mbar_init(&m.u_free, kLtWarpsS);
         mbar_init(&m.s_full, kLtWarpsS);
         mbar_init(&m.xy_free, C::kWarpsO);
@@ -370,23 +372,21 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
         const float* from = plan.mode == 2 ? plan.states + part : plan.mode == 0 && a.state_in != nullptr ? a.state_in + own : nullptr;
         float* to = plan.mode == 2 ? nullptr : plan.mode == 1 ? plan.states + part : a.state_out + own;
         // (loops stay loops here and below: unrolled, the roles' code did not fit the instruction cache, and a third of all stalls was for it)
-        const auto keep = [&](int g, float (&s)[16]) {
-            if (C::NS == 2) lt_st(lane_base + kLtS + k0 + g, s);
-            if (C::NS == 3 || outputs) {
+        const auto keep_parts = [&](int g, float (&s)[16]) {
 #pragma unroll
-                for (int p = 0; p < C::NS; ++p) {
-                    uint32_t u[8];
+            for (int p = 0; p < C::NS; ++p) {
+                uint32_t u[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) u[e] = lt_part(s[2 * e], s[2 * e + 1], p + 1 == C::NS);
-                    lt_st(lane_base + C::kParts + p * kHalf + (k0 + g) / 2, u);
-                }
+                for (int e = 0; e < 8; ++e) u[e] = lt_part(s[2 * e], s[2 * e + 1], p + 1 == C::NS);
+                lt_st(lane_base + C::kParts + p * kHalf + (k0 + g) / 2, u);
             }
         };
         const auto at_end = [&](int g, const float (&s)[16]) {
             if (to == nullptr || !has_row) return;
+            float* at = to + static_cast<int64_t>(g) * a.dv;
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-                if (k0 + g + e < a.dk) to[static_cast<int64_t>(g + e) * a.dv] = s[e];
+            for (int e = 0; e < 16; ++e, at += a.dv)
+                if (k0 + g + e < a.dk) *at = s[e];
         };
 #pragma unroll 1
         for (int g = 0; g < kHalf; g += 16) {
@@ -394,7 +394,8 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = from != nullptr && has_row && k0 + g + e < a.dk ? from[static_cast<int64_t>(g + e) * a.dv] : 0.0f;
             if (chunks == 0) at_end(g, s);
-            keep(g, s);
+            if (C::NS == 2) lt_st(lane_base + kLtS + k0 + g, s);
+            keep_parts(g, s);
         }
         lt_st_wait();
         lt_arrive_read(&m.s_full, lane);
@@ -404,7 +405,8 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
 #pragma unroll 1
         for (int c = 0; c < chunks; ++c) {  // S behind chunk c
             const bool last = c + 1 == chunks;
-            if (!lt_wait(m, &m.u_full, c & 1) || (outputs && !last && !lt_wait(m, &m.x_full, c & 1))) break;
+            if (!lt_wait(m, &m.u_full, c & 1)) break;
+            if (C::NS == 3 && outputs && !last && !lt_wait(m, &m.x_full, c & 1)) break;  // (the parts are S itself)
             tc_fence_after();
             const int n = min(kLtChunk, seg_end - seg0 - c * kLtChunk);
             float pn = m.power[n];
@@ -444,16 +446,33 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = fmaf(pn, s[e], __uint_as_float(ru[e]));
                 if (last) at_end(g, s);
-                else keep(g, s);
+                else if (C::NS == 3) keep_parts(g, s);
+                else lt_st(lane_base + kLtS + k0 + g, s);
+            }
+            lt_arrive_read(&m.u_free, lane);
+            if (last) break;
+            if (C::NS == 2 && outputs) {  // its parts, when the product before is done with the last ones
+                if (!lt_wait(m, &m.x_full, c & 1)) break;
+                tc_fence_after();
+                lt_st_wait();
+#pragma unroll 1
+                for (int g = 0; g < kHalf; g += 16) {
+                    uint32_t rs[16];
+                    float s[16];
+                    lt_ld(lane_base + kLtS + k0 + g, rs);
+                    lt_ld_wait(rs);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[e] = __uint_as_float(rs[e]);
+                    keep_parts(g, s);
+                }
             }
             lt_st_wait();
-            lt_arrive_read(&m.u_free, lane);
-            if (!last) lt_arrive_read(&m.s_full, lane);  // (one more would be a phase ahead of the products' wait for this one)
+            lt_arrive_read(&m.s_full, lane);  // (not behind the last: it would be a phase ahead of the products' wait for this one)
         }
-    } else if (warp < C::kFirstO || (TMA && warp >= C::kFirstP + 6)) {
+    } else if (warp < C::kFirstO) {
         // ---- W (and tiles)
         constexpr int threads = 32 * kWarpsW;
-        const int rank = warp < C::kFirstO ? warp - C::kFirstW : warp - (C::kFirstP + 6) + C::kWarpsW, id = rank * 32 + lane;
+        const int rank = warp - C::kFirstW, id = rank * 32 + lane;
         const T* q = static_cast<const T*>(a.q) + b * a.q_stride[0] + h * a.q_stride[2] + seg0 * a.q_stride[1];
         const T* k = static_cast<const T*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2] + seg0 * a.k_stride[1];
         const T* v = static_cast<const T*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2] + seg0 * a.v_stride[1] + col0;
@@ -491,67 +510,59 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
             // V, and W (free when the product before that has it is done)
             if (c >= C::kStages && !lt_wait(m, &m.w_free[stage], turn ^ 1u)) break;
             unsigned char* wt = smem + C::oW + stage * C::NW * C::kTileV;
-            // a warp's piece: 16 bytes of eight tokens beside one another, four groups of channels; two on their way together
-            constexpr int kPieces = kLtChunk * DV / 256;
+            // a warp's piece: 16 bytes of eight tokens beside one another, four groups of channels.  A thread keeps to its tokens.
+            constexpr int kGroups = DV / 32;
+            if constexpr (TMA) {
+                // (a short loop: the roles' code has to stay in the instruction cache together)
+                constexpr int kPieces = 8 * kGroups / kWarpsW;  // groups of one block of tokens, then of the next
+                const auto token_of = [&](int i) { return (rank + i / kGroups * kWarpsW) * 8 + (lane & 7); };
+                const auto at_of = [&](int i) { return vt + lt_swizzled(i % kGroups * 4 + (lane >> 3), token_of(i)); };
+                uint4 next = *reinterpret_cast<const uint4*>(at_of(0));
+                uint32_t w[3], high = 0;
 #pragma unroll 1
-            for (int i0 = rank; i0 < kPieces; i0 += 2 * kWarpsW) {
-                const auto token_of = [&](int i) { return (i & 7) * 8 + (lane & 7); };
-                const auto group_of = [&](int i) { return (i >> 3) * 4 + (lane >> 3); };
-                if (TMA) {
-                    uint4 u[2];
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const int i = i0 + j * kWarpsW, t = token_of(i);
-                        if (i >= kPieces) continue;
-                        uint4* vp = reinterpret_cast<uint4*>(vt + lt_swizzled(group_of(i), t));
-                        if (t >= n) *vp = make_uint4(0, 0, 0, 0);
-                        u[j] = *vp;
+                for (int i = 0; i < kPieces; ++i) {
+                    const int t = token_of(i);
+                    if (i % kGroups == 0) {
+                        const int back = t < n ? n - 1 - t : 0;
+                        w[0] = m.weight[back].x, w[1] = m.weight[back].y, w[2] = m.weight2[back];
+                        high = 0;
                     }
+                    if (t >= n) *reinterpret_cast<uint4*>(at_of(i)) = next = make_uint4(0, 0, 0, 0);
+                    const uint32_t w4[4] = {next.x, next.y, next.z, next.w};
+                    if (i + 1 < kPieces) next = *reinterpret_cast<const uint4*>(at_of(i + 1));
+                    lt_weigh(wt + lt_plain(i % kGroups * 4 + (lane >> 3), t), C::kTileV, w4, w);
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const int i = i0 + j * kWarpsW, t = token_of(i), g = group_of(i), back = t < n ? n - 1 - t : 0;
-                        if (i >= kPieces) continue;
-                        uint32_t w4[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
-                        lt_weigh(wt + lt_plain(g, t), C::kTileV, w4, m.weight[back], m.weight2[back]);
-                        uint32_t high = 0;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) high = __vmaxu2(high, w4[e] & 0x7FFF7FFFu);
-                        if ((high & 0xFFFFu) >= 0x7F80u || high >= 0x7F800000u) {
-                            atomicMin(&m.bad, t0 + t);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                if (((w4[e / 2] >> (16 * (e & 1))) & 0x7F80u) != 0x7F80u) continue;
-                                w4[e / 2] &= (e & 1) != 0 ? 0x0000FFFFu : 0xFFFF0000u;
-                                atomicMin(&m.first_bad[g * 8 + e], t0 + t);
-                            }
-                            *reinterpret_cast<uint4*>(vt + lt_swizzled(g, t)) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+                    for (int e = 0; e < 4; ++e) high = __vmaxu2(high, w4[e] & 0x7FFF7FFFu);
+                    if (i % kGroups == kGroups - 1 && ((high & 0xFFFFu) >= 0x7F80u || high >= 0x7F800000u)) {
+                        atomicMin(&m.bad, t0 + t);
+#pragma unroll 1
+                        for (int d = 0; d < DV / 4; ++d) {  // (this thread's channels, one by one)
+                            const int g = (d >> 3) * 4 + (lane >> 3);
+                            uint16_t* at = reinterpret_cast<uint16_t*>(vt + lt_swizzled(g, t)) + (d & 7);
+                            if ((*at & 0x7F80u) != 0x7F80u) continue;
+                            *at = 0;
+                            atomicMin(&m.first_bad[g * 8 + (d & 7)], t0 + t);
                         }
                     }
-                } else {
-                    float x[2][8];
+                }
+            } else {
+#pragma unroll 1
+                for (int i = rank; i < 8 * kGroups; i += kWarpsW) {
+                    const int t = (i & 7) * 8 + (lane & 7), g = (i >> 3) * 4 + (lane >> 3);
+                    float x[8], y[8];
+                    lt_load8(v + (t0 + t) * a.v_stride[1] + g * 8, t < n ? max(0, min(8, dv - g * 8)) : 0, plan.aligned, x);
+                    const float w = m.power[t < n ? n - 1 - t : 0];
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const int i = i0 + j * kWarpsW, t = token_of(i), g = group_of(i);
-                        if (i < kPieces) lt_load8(v + (t0 + t) * a.v_stride[1] + g * 8, t < n ? max(0, min(8, dv - g * 8)) : 0, plan.aligned, x[j]);
+                    for (int e = 0; e < 8; ++e) y[e] = x[e] * w;
+                    lt_store_parts<C::NW>(wt + lt_plain(g, t), C::kTileV, y);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        if (lt_finite(x[e])) continue;
+                        atomicMin(&m.bad, t0 + t);
+                        atomicMin(&m.first_bad[g * 8 + e], t0 + t);
+                        x[e] = 0.0f;
                     }
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const int i = i0 + j * kWarpsW, t = token_of(i), g = group_of(i);
-                        if (i >= kPieces) continue;
-                        const float w = m.power[t < n ? n - 1 - t : 0];
-                        float y[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) y[e] = x[j][e] * w;
-                        lt_store_parts<C::NW>(wt + lt_plain(g, t), C::kTileV, y);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            if (lt_finite(x[j][e])) continue;
-                            atomicMin(&m.bad, t0 + t);
-                            x[j][e] = 0.0f;
-                            atomicMin(&m.first_bad[g * 8 + e], t0 + t);
-                        }
-                        lt_store_parts<C::NX>(vt + lt_swizzled(g, t), C::kTileV, x[j]);
-                    }
+                    lt_store_parts<C::NX>(vt + lt_swizzled(g, t), C::kTileV, x);
                 }
             }
             fence_proxy_async();
@@ -559,6 +570,7 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
             if (lane == 0) {
                 if (!TMA) mbar_arrive(&m.full[stage]);
                 mbar_arrive(&m.w_full[stage]);
+                mbar_arrive(&m.v_whole[c % C::kStagesV]);  // (one per stage of V: this warp may be two chunks ahead of the product that waits)
             }
         }
     } else if (warp < C::kFirstP) {
@@ -572,29 +584,28 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
                 if (!lt_wait(m, &m.y_full, c & 1)) break;
                 tc_fence_after();
                 const int first = *reinterpret_cast<volatile int*>(&m.bad) < (c + 1) * kLtChunk ? m.first_bad[row] - c * kLtChunk : kLtChunk;
+                const int t0 = c * kLtChunk + token0, n = row < dv ? seg_end - seg0 - t0 : 0;
+                T* at = out + t0 * a.out_stride[1];
 #pragma unroll 1
-                for (int block = token0; block < token0 + kShare; block += 32) {
-                    T o[32];
+                for (int u = 0; u < kShare; u += 8) {
+                    uint32_t x[8], y[8];
+                    lt_ld(lane_base + kLtX + token0 + u, x);
+                    lt_ld(lane_base + kLtY + token0 + u, y);
+                    float power[8];
+                    *reinterpret_cast<float4*>(power) = *reinterpret_cast<const float4*>(m.scaled_next + token0 + u);
+                    *reinterpret_cast<float4*>(power + 4) = *reinterpret_cast<const float4*>(m.scaled_next + token0 + u + 4);
+                    lt_ld_wait(x);
+                    lt_ld_wait(y);
+                    if (u + 8 == kShare) lt_arrive_read(&m.xy_free, lane);
 #pragma unroll
-                    for (int u = 0; u < 32; u += 16) {
-                        uint32_t x[16], y[16];
-                        lt_ld(lane_base + kLtX + block + u, x);
-                        lt_ld(lane_base + kLtY + block + u, y);
-                        lt_ld_wait(x);
-                        lt_ld_wait(y);
-                        if (u == 16 && block + 32 == token0 + kShare) lt_arrive_read(&m.xy_free, lane);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            o[u + i] = lin_from<T>(fmaf(m.scaled_next[block + u + i], __uint_as_float(x[i]), __uint_as_float(y[i])));
+                    for (int i = 0; i < 8; ++i) {
+                        if (u + i < n) *at = lin_from<T>(fmaf(power[i], __uint_as_float(x[i]), __uint_as_float(y[i])));
+                        at += a.out_stride[1];
                     }
-                    const int t0 = c * kLtChunk + block, n = seg_end - seg0 - t0;
-                    T* at = out + t0 * a.out_stride[1];
-                    if (row < dv) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (i < n) at[i * a.out_stride[1]] = o[i];
-                        for (int i = max(0, first - block); i < min(32, n); ++i) at[i * a.out_stride[1]] = lin_from<T>(__int_as_float(0x7fffffff));
-                    }
+                }
+                if (first < token0 + kShare) {
+#pragma unroll 1
+                    for (int u = max(0, first - token0); u < min(kShare, n); ++u) out[(t0 + u) * a.out_stride[1]] = lin_from<T>(__int_as_float(0x7fffffff));
                 }
             }
         }
@@ -604,37 +615,36 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
         if (outputs) {
             unsigned char* at = smem + C::oP + half * 4 * 1024 + (row >> 3) * 128 + (row & 7) * 16;
             const int d0 = row - half * 32;
-            float power[32];  // of the thread's 32 entries, in every chunk the same
-#pragma unroll
-            for (int e = 0; e < 32; ++e) power[e] = m.scaled[max(d0 - e, 0)];
             const bool nothing = half > (warp & 3), whole = half < (warp & 3);  // tokens behind all of the rows, in front of all
 #pragma unroll 1
             for (int c = 0; c < chunks; ++c) {
-                if (!lt_wait(m, &m.g_full, c & 1)) break;  // (and so the product before that read P is done)
+                if (!lt_wait(m, &m.g_full, c & 1)) break;
                 tc_fence_after();
-#pragma unroll
-                for (int u = 0; u < 32; u += 16) {
-                    uint32_t g[16];
-                    if (!nothing) {
-                        lt_ld(lane_base + kLtY + half * 32 + u, g);
-                        lt_ld_wait(g);
-                    }
-#pragma unroll
-                    for (int f = 0; f < 16; f += 8) {
-                        float x[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            x[e] = __uint_as_float(g[f + e]) * power[u + f + e];
-                            if (!whole && (nothing || d0 < u + f + e)) x[e] = 0.0f;
-                        }
-                        lt_store_parts<C::NS>(at + (u / 8 + f / 8) * 1024, C::kPartP, x);
-                    }
+                uint32_t g[2][16];
+                if (!nothing) {
+                    lt_ld(lane_base + kLtG + half * 32, g[0]);
+                    lt_ld(lane_base + kLtG + half * 32 + 16, g[1]);
+                    lt_ld_wait(g[0]);
+                    lt_ld_wait(g[1]);
                 }
-                tc_fence_before();
+                lt_arrive_read(&m.g_read, lane);
+                if (c > 0 && !lt_wait(m, &m.y_full, (c - 1) & 1)) break;  // (the product before has read P)
+#pragma unroll 1
+                for (int f = 0; f < 32; f += 8) {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[e] = __uint_as_float(g[0][e]) * m.scaled[max(d0 - f - e, 0)];
+                        if (!whole && (nothing || d0 - f < e)) x[e] = 0.0f;
+                    }
+                    lt_store_parts<C::NS>(at + f / 8 * 1024, C::kPartP, x);
+#pragma unroll
+                    for (int e = 0; e < 24; ++e) g[e / 16][e % 16] = g[(e + 8) / 16][(e + 8) % 16];
+                }
                 lt_arrive_operands(&m.p_full, lane);
             }
         }
-    } else if (warp == C::kFirstP + 2) {
+    } else if (warp == C::kFirstP + 2 || warp == C::kFirstP + 6) {
         // ---- the products
         {
             // instruction descriptors: fp32 accumulators, bf16 operands, M = 128; N, and which operands are MN-major
@@ -660,46 +670,54 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
                                 add = true;
                             }
             };
-            const auto make_u = [&](int c) {  // U^T = W^T K
-                if (!wait(&m.w_full[c % C::kStages], (c / C::kStages) & 1) || !wait(&m.full[c % C::kStages], (c / C::kStages) & 1) ||
-                    (c > 0 && !wait(&m.u_free, (c - 1) & 1)))
-                    return false;
-                tc_fence_after();
-                if (lt_elect()) {
-                    const uint64_t dk = lt_desc_swizzled(base + (c % C::kStages) * C::kStage + C::oK, 8192, 1024),
-                                   dw = make_smem_desc(base + C::oW + (c % C::kStages) * C::NW * C::kTileV, 128, 1024);
-                    parts(C::NW, C::NX, C::NW, 1, [&](int p, int r, int, int i, bool add) {
-                        lt_mma(tmem + kLtU, dw + ((p * C::kTileV + i * 256) >> 4), dk + ((r * C::kTileK + i * 2048) >> 4), kIdescU, add);
-                    });
-                    tc_commit(&m.u_full);
-                    tc_commit(&m.w_free[c % C::kStages]);
-                    if (!outputs) tc_commit(&m.empty[c % C::kStages]);
-                }
-                __syncwarp();
-                return true;
-            };
-            bool ok = chunks == 0 || make_u(0);
-#pragma unroll 1
-            for (int c = 0; c < chunks && ok; ++c) {
-                if (outputs) {
-                    const uint32_t at = base + (c % C::kStages) * C::kStage;
-                    const uint64_t dq = lt_desc_swizzled(at, 16, 1024), dk = lt_desc_swizzled(at + C::oK, 16, 1024),
-                                   dv = lt_desc_swizzled(base + C::oV + (c % C::kStagesV) * C::NX * C::kTileV, 8192, 1024);
-                    ok = c == 0 || wait(&m.xy_free, (c - 1) & 1);
-                    if (!ok) break;
+            const auto stage_at = [&](int c) { return base + (c % C::kStages) * C::kStage; };
+            const auto stage_here = [&](int c) { return wait(&m.full[c % C::kStages], (c / C::kStages) & 1); };
+            if (warp == C::kFirstP + 6) {
+                const auto make_g = [&](int c) {  // G = Q K^T
                     tc_fence_after();
-                    if (lt_elect()) {  // G = Q K^T
+                    if (lt_elect()) {
+                        const uint64_t dq = lt_desc_swizzled(stage_at(c), 16, 1024), dk = lt_desc_swizzled(stage_at(c) + C::oK, 16, 1024);
                         parts(C::NX, C::NX, C::NX, DK / 64, [&](int p, int r, int quad, int i, bool add) {
                             const int step = quad * 8192 + i * 32;
-                            lt_mma(tmem + kLtY, dq + ((p * C::kTileK + step) >> 4), dk + ((r * C::kTileK + step) >> 4), kIdescG, add);
+                            lt_mma(tmem + kLtG, dq + ((p * C::kTileK + step) >> 4), dk + ((r * C::kTileK + step) >> 4), kIdescG, add);
                         });
                         tc_commit(&m.g_full);
                     }
                     __syncwarp();
-                    ok = wait(&m.s_full, c & 1);
-                    if (!ok) break;
+                };
+                bool ok = true;
+                if (outputs && chunks > 0) {
+                    ok = stage_here(0);
+                    if (ok) make_g(0);
+                }
+#pragma unroll 1
+                for (int c = 0; c < chunks && ok; ++c) {
+                    if (!wait(&m.w_full[c % C::kStages], (c / C::kStages) & 1)) break;
+                    if (!(outputs ? wait(&m.g_read, c & 1) : stage_here(c) && (c == 0 || wait(&m.u_free, (c - 1) & 1)))) break;
+                    tc_fence_after();
+                    if (lt_elect()) {  // U^T = W^T K
+                        const uint64_t dk = lt_desc_swizzled(stage_at(c) + C::oK, 8192, 1024),
+                                       dw = make_smem_desc(base + C::oW + (c % C::kStages) * C::NW * C::kTileV, 128, 1024);
+                        parts(C::NW, C::NX, C::NW, 1, [&](int p, int r, int, int i, bool add) {
+                            lt_mma(tmem + kLtU, dw + ((p * C::kTileV + i * 256) >> 4), dk + ((r * C::kTileK + i * 2048) >> 4), kIdescU, add);
+                        });
+                        tc_commit(&m.u_full);
+                        tc_commit(&m.w_free[c % C::kStages]);
+                        tc_commit(&m.empty[c % C::kStages]);
+                    }
+                    __syncwarp();
+                    if (outputs && c + 1 < chunks) {
+                        ok = stage_here(c + 1) && wait(&m.u_free, c & 1);
+                        if (ok) make_g(c + 1);
+                    }
+                }
+            } else if (outputs) {
+#pragma unroll 1
+                for (int c = 0; c < chunks; ++c) {
+                    if (!stage_here(c) || !wait(&m.s_full, c & 1) || (c > 0 && !wait(&m.xy_free, (c - 1) & 1))) break;
                     tc_fence_after();
                     if (lt_elect()) {  // X^T = S^T Q^T
+                        const uint64_t dq = lt_desc_swizzled(stage_at(c), 16, 1024);
                         parts(C::NS, C::NX, C::NS, DK / 64, [&](int p, int r, int quad, int i, bool add) {
                             lt_mma_tmem(tmem + kLtX, tmem + C::kParts + p * (DK / 2) + quad * 32 + i * 8,
                                         dq + ((r * C::kTileK + quad * 8192 + i * 32) >> 4), kIdescX, add);
@@ -707,10 +725,10 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
                         tc_commit(&m.x_full);
                     }
                     __syncwarp();
-                    ok = wait(&m.p_full, c & 1);
-                    if (!ok) break;
+                    if (!wait(&m.p_full, c & 1) || !wait(&m.v_whole[c % C::kStagesV], (c / C::kStagesV) & 1)) break;
                     tc_fence_after();
                     if (lt_elect()) {  // Y^T = V^T P^T
+                        const uint64_t dv = lt_desc_swizzled(base + C::oV + (c % C::kStagesV) * C::NX * C::kTileV, 8192, 1024);
                         parts(C::NS, C::NX, C::NS, 1, [&](int p, int r, int, int i, bool add) {
                             lt_mma(tmem + kLtY, dv + ((r * C::kTileV + i * 2048) >> 4), dp + ((p * C::kPartP + i * 2048) >> 4), kIdescY, add);
                         });
@@ -719,7 +737,6 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
                     }
                     __syncwarp();
                 }
-                if (c + 1 < chunks) ok = make_u(c + 1);
             }
         }
     } else if (TMA && warp == C::kFirstP + 3 && lane == 0) {
