@@ -37,7 +37,7 @@ namespace fb {
 
 constexpr int kLtChunk = 64;
 constexpr int kLtWarpsS = 8, kLtWarpsP = 8;  // (of the P group four make P, two issue products, one copies)
-constexpr uint32_t kLtWaitLimit = 1000000u;
+constexpr uint32_t kLtWaitLimit = 200000u;
 // TMEM columns: U (and, between two of them, G), X, Y, S^T in fp32 and as two operand parts of DK / 2 columns, or as three parts, which are exact
 constexpr uint32_t kLtU = 0, kLtG = 0, kLtX = 128, kLtY = 192, kLtS = 256, kLtTmemCols = 512;
 
@@ -50,7 +50,7 @@ struct LtCfg {
     static constexpr int NW = 3;                                                   // parts of W
     static constexpr int kStages = kBf16 ? 2 : 1;   // of Q and K, and of W
     static constexpr int kStagesV = kBf16 ? 3 : 1;  // (V is read a chunk ahead, for W)
-    static constexpr int kWarpsW = kBf16 ? 4 : 8, kWarpsO = kBf16 ? 8 : 4;
+    static constexpr int kWarpsW = 8, kWarpsO = kBf16 ? 8 : 4;
     static constexpr int kFirstW = kLtWarpsS, kFirstO = kFirstW + kWarpsW, kFirstP = kFirstO + kWarpsO, kThreads = 32 * (kFirstP + kLtWarpsP);
     static_assert(kFirstO % 4 == 0 && kFirstP % 4 == 0, "a warp's TMEM lanes go by its number");
     static constexpr int kTileK = kLtChunk * DK * 2, kTileV = kLtChunk * DV * 2, kPartP = kLtChunk * kLtChunk * 2;
@@ -66,7 +66,8 @@ struct LtMisc {
     int dead;                                      // a wait ran out
     int b;
     float power_next, power_gap, power_off;        // the float beyond power[64] on decay^64's side, how far, and how far decay^64 is (relative)
-    float power[kLtChunk + 4], scaled[kLtChunk + 4];  // decay^i, scale * decay^i
+    float power[kLtChunk + 4];                        // decay^i
+    float scaled_front[kLtChunk], scaled[kLtChunk + 4];  // scale * decay^i, and in front of it what masked entries of P read
     __align__(16) float scaled_next[kLtChunk];        // scale * decay^(i+1)
     uint2 weight[kLtChunk];                        // decay^i as three bf16 parts, each twice: w0 w0, w1 w1 (w2 below)
     uint32_t weight2[kLtChunk];
@@ -155,21 +156,22 @@ __device__ __forceinline__ void lt_tma(void* dst, const CUtensorMap* map, int ch
 }
 
 // Waits for a phase; gives up when the limit runs out or somebody else has given up.
-__device__ __forceinline__ bool lt_test(uint64_t* bar, uint32_t parity) {
+// (the hardware holds the thread for up to some ten microseconds: asking again and again took issue slots from the warps that work)
+__device__ __forceinline__ bool lt_try(uint64_t* bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
         : "memory");
     return ok != 0;
 }
 __device__ __forceinline__ bool lt_wait_one(LtMisc& m, uint64_t* bar, uint32_t parity) {
     for (uint32_t i = 0; i < kLtWaitLimit; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 63u) == 63u && *reinterpret_cast<volatile int*>(&m.dead)) return false;
+        if (lt_try(bar, parity)) return true;
+        if ((i & 7u) == 7u && *reinterpret_cast<volatile int*>(&m.dead)) return false;
     }
     *reinterpret_cast<volatile int*>(&m.dead) = 1;
     return false;
@@ -333,6 +335,7 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
         }
     }
     if (tid < 128) m.first_bad[tid] = 0x7fffffff;
+    if (tid < kLtChunk) m.scaled_front[tid] = 0.0f;
     if (tid == 0) {
         for (int i = 0; i < C::kStagesV; ++i) mbar_init(&m.full_v[i], 1), mbar_init(&m.v_whole[i], kWarpsW);
         for (int i = 0; i < C::kStages; ++i) {
@@ -476,6 +479,8 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
         const T* q = static_cast<const T*>(a.q) + b * a.q_stride[0] + h * a.q_stride[2] + seg0 * a.q_stride[1];
         const T* k = static_cast<const T*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2] + seg0 * a.k_stride[1];
         const T* v = static_cast<const T*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2] + seg0 * a.v_stride[1] + col0;
+        uint32_t w[3] = {0, 0, 0};  // the weight of this thread's token
+#pragma unroll 1
         for (int c = 0; c < chunks; ++c) {
             const int t0 = c * kLtChunk, n = min(kLtChunk, seg_end - seg0 - t0), stage = c % C::kStages;
             const uint32_t turn = (c / C::kStages) & 1;
@@ -514,35 +519,34 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
             constexpr int kGroups = DV / 32;
             if constexpr (TMA) {
                 // (a short loop: the roles' code has to stay in the instruction cache together)
-                constexpr int kPieces = 8 * kGroups / kWarpsW;  // groups of one block of tokens, then of the next
-                const auto token_of = [&](int i) { return (rank + i / kGroups * kWarpsW) * 8 + (lane & 7); };
-                const auto at_of = [&](int i) { return vt + lt_swizzled(i % kGroups * 4 + (lane >> 3), token_of(i)); };
+                static_assert(kWarpsW == 8, "a warp has eight tokens");
+                const int t = rank * 8 + (lane & 7);
+                if (c == 0 || n < kLtChunk) {
+                    const int back = t < n ? n - 1 - t : 0;
+                    w[0] = m.weight[back].x, w[1] = m.weight[back].y, w[2] = m.weight2[back];
+                }
+                unsigned char *from = vt + lt_swizzled(lane >> 3, t), *to = wt + lt_plain(lane >> 3, t);
+                const auto at_of = [&](int g) { return from + (((t & 4) != 0 ? -64 : 64) * (g & 1)) + (g >> 1) * 8192; };  // (four groups on is one bit of the swizzle)
                 uint4 next = *reinterpret_cast<const uint4*>(at_of(0));
-                uint32_t w[3], high = 0;
+                uint32_t high = 0;
 #pragma unroll 1
-                for (int i = 0; i < kPieces; ++i) {
-                    const int t = token_of(i);
-                    if (i % kGroups == 0) {
-                        const int back = t < n ? n - 1 - t : 0;
-                        w[0] = m.weight[back].x, w[1] = m.weight[back].y, w[2] = m.weight2[back];
-                        high = 0;
-                    }
-                    if (t >= n) *reinterpret_cast<uint4*>(at_of(i)) = next = make_uint4(0, 0, 0, 0);
+                for (int g = 0; g < kGroups; ++g) {
+                    if (t >= n) *reinterpret_cast<uint4*>(at_of(g)) = next = make_uint4(0, 0, 0, 0);
                     const uint32_t w4[4] = {next.x, next.y, next.z, next.w};
-                    if (i + 1 < kPieces) next = *reinterpret_cast<const uint4*>(at_of(i + 1));
-                    lt_weigh(wt + lt_plain(i % kGroups * 4 + (lane >> 3), t), C::kTileV, w4, w);
+                    if (g + 1 < kGroups) next = *reinterpret_cast<const uint4*>(at_of(g + 1));
+                    lt_weigh(to + g * 4096, C::kTileV, w4, w);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) high = __vmaxu2(high, w4[e] & 0x7FFF7FFFu);
-                    if (i % kGroups == kGroups - 1 && ((high & 0xFFFFu) >= 0x7F80u || high >= 0x7F800000u)) {
-                        atomicMin(&m.bad, t0 + t);
+                }
+                if ((high & 0xFFFFu) >= 0x7F80u || high >= 0x7F800000u) {
+                    atomicMin(&m.bad, t0 + t);
 #pragma unroll 1
-                        for (int d = 0; d < DV / 4; ++d) {  // (this thread's channels, one by one)
-                            const int g = (d >> 3) * 4 + (lane >> 3);
-                            uint16_t* at = reinterpret_cast<uint16_t*>(vt + lt_swizzled(g, t)) + (d & 7);
-                            if ((*at & 0x7F80u) != 0x7F80u) continue;
-                            *at = 0;
-                            atomicMin(&m.first_bad[g * 8 + (d & 7)], t0 + t);
-                        }
+                    for (int d = 0; d < DV / 4; ++d) {  // (this thread's channels, one by one)
+                        const int g = (d >> 3) * 4 + (lane >> 3);
+                        uint16_t* at = reinterpret_cast<uint16_t*>(vt + lt_swizzled(g, t)) + (d & 7);
+                        if ((*at & 0x7F80u) != 0x7F80u) continue;
+                        *at = 0;
+                        atomicMin(&m.first_bad[g * 8 + (d & 7)], t0 + t);
                     }
                 }
             } else {
@@ -584,8 +588,9 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
                 if (!lt_wait(m, &m.y_full, c & 1)) break;
                 tc_fence_after();
                 const int first = *reinterpret_cast<volatile int*>(&m.bad) < (c + 1) * kLtChunk ? m.first_bad[row] - c * kLtChunk : kLtChunk;
-                const int t0 = c * kLtChunk + token0, n = row < dv ? seg_end - seg0 - t0 : 0;
+                const int t0 = c * kLtChunk + token0, n = row < dv ? min(kShare, seg_end - seg0 - t0) : 0;
                 T* at = out + t0 * a.out_stride[1];
+                const bool whole = n == kShare;
 #pragma unroll 1
                 for (int u = 0; u < kShare; u += 8) {
                     uint32_t x[8], y[8];
@@ -597,11 +602,18 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
                     lt_ld_wait(x);
                     lt_ld_wait(y);
                     if (u + 8 == kShare) lt_arrive_read(&m.xy_free, lane);
+                    T o[8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        if (u + i < n) *at = lin_from<T>(fmaf(power[i], __uint_as_float(x[i]), __uint_as_float(y[i])));
-                        at += a.out_stride[1];
+                    for (int i = 0; i < 8; ++i) o[i] = lin_from<T>(fmaf(power[i], __uint_as_float(x[i]), __uint_as_float(y[i])));
+                    if (whole) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) at[i * a.out_stride[1]] = o[i];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (u + i < n) at[i * a.out_stride[1]] = o[i];
                     }
+                    at += 8 * a.out_stride[1];
                 }
                 if (first < token0 + kShare) {
 #pragma unroll 1
@@ -629,17 +641,27 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
                 }
                 lt_arrive_read(&m.g_read, lane);
                 if (c > 0 && !lt_wait(m, &m.y_full, (c - 1) & 1)) break;  // (the product before has read P)
+                if (nothing) {
 #pragma unroll 1
-                for (int f = 0; f < 32; f += 8) {
-                    float x[8];
+                    for (int f = 0; f < 4 * C::NS; ++f) *reinterpret_cast<uint4*>(at + (f & 3) * 1024 + (f >> 2) * C::kPartP) = make_uint4(0, 0, 0, 0);
+                } else {
+                    const float* power = m.scaled + d0;
+#pragma unroll 1
+                    for (int f = 0; f < 32; f += 16) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x[e] = __uint_as_float(g[0][e]) * m.scaled[max(d0 - f - e, 0)];
-                        if (!whole && (nothing || d0 - f < e)) x[e] = 0.0f;
+                        for (int r = 0; r < 16; r += 8) {
+                            float x[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(g[0][r + e]) * power[-f - r - e];
+                            if (!whole) {
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) x[e] = d0 - f >= r + e ? x[e] : 0.0f;
+                            }
+                            lt_store_parts<C::NS>(at + (f + r) / 8 * 1024, C::kPartP, x);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) g[0][e] = g[1][e];
                     }
-                    lt_store_parts<C::NS>(at + f / 8 * 1024, C::kPartP, x);
-#pragma unroll
-                    for (int e = 0; e < 24; ++e) g[e / 16][e % 16] = g[(e + 8) / 16][(e + 8) % 16];
                 }
                 lt_arrive_operands(&m.p_full, lane);
             }
