@@ -28,6 +28,7 @@
 // Y (not in W) and the outputs of their channel, from their token on, are set to NaN.
 #include <cuda.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "linattn.cuh"
@@ -48,13 +49,14 @@ struct LtCfg {
     static constexpr int NX = kBf16 ? 1 : std::is_same<T, __half>::value ? 2 : 3;  // parts of q, k, v
     static constexpr int NS = std::is_same<T, float>::value ? 3 : 2;               // parts of S and P
     static constexpr int NW = 3;                                                   // parts of W
-    static constexpr int kStages = kBf16 ? 2 : 1;   // of Q and K, and of W
-    static constexpr int kStagesV = kBf16 ? 3 : 1;  // (V is read a chunk ahead, for W)
     static constexpr int kWarpsW = 8, kWarpsO = kBf16 ? 8 : 4;
     static constexpr int kFirstW = kLtWarpsS, kFirstO = kFirstW + kWarpsW, kFirstP = kFirstO + kWarpsO, kThreads = 32 * (kFirstP + kLtWarpsP);
     static_assert(kFirstO % 4 == 0 && kFirstP % 4 == 0, "a warp's TMEM lanes go by its number");
     static constexpr int kTileK = kLtChunk * DK * 2, kTileV = kLtChunk * DV * 2, kPartP = kLtChunk * kLtChunk * 2;
     static constexpr int kStage = 2 * NX * kTileK, oK = NX * kTileK;  // Q, and K behind it
+    // stages of Q and K, and of W: two where they fit; of V in bf16 three (it is read a chunk ahead, for W)
+    static constexpr int kStages = 2 * (kStage + (NX + NW) * kTileV) + NS * kPartP <= 222 * 1024 ? 2 : 1;
+    static constexpr int kStagesV = kBf16 ? 3 : kStages;
     static constexpr int oV = kStages * kStage, oW = oV + kStagesV * NX * kTileV, oP = oW + kStages * NW * kTileV, oMisc = oP + NS * kPartP;
     static constexpr uint32_t kParts = NS == 3 ? kLtS : kLtS + 128;  // TMEM columns of the parts of S^T
 };
@@ -493,6 +495,14 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
                     *reinterpret_cast<uint4*>(st + C::oK + lt_swizzled(i % (DK / 8), n + i / (DK / 8))) = make_uint4(0, 0, 0, 0);
             } else {
                 if (c >= C::kStages && !lt_wait(m, &m.empty[stage], turn ^ 1u)) break;
+                // the next chunk's rows, into L2
+                for (int i = id; i < 3 * kLtChunk; i += threads) {
+                    const int t = t0 + kLtChunk + (i & (kLtChunk - 1));
+                    if (t >= seg_end - seg0) continue;
+                    const char* row = reinterpret_cast<const char*>(i < kLtChunk ? k + t * a.k_stride[1] : i < 2 * kLtChunk ? v + t * a.v_stride[1] : q + t * a.q_stride[1]);
+                    const int bytes = (i < kLtChunk || i >= 2 * kLtChunk ? a.dk : dv) * static_cast<int>(sizeof(T));
+                    for (int at = 0; at < bytes; at += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + at));
+                }
                 static_assert(TMA || kLtChunk * DK / 8 / threads % 2 == 0, "pieces");
 #pragma unroll 1
                 for (int i0 = 0; i0 < kLtChunk * DK / 8 / threads; i0 += 2) {
@@ -550,23 +560,31 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
                     }
                 }
             } else {
+                const int t = rank * 8 + (lane & 7);
+                const float weight = m.power[t < n ? n - 1 - t : 0];
 #pragma unroll 1
-                for (int i = rank; i < 8 * kGroups; i += kWarpsW) {
-                    const int t = (i & 7) * 8 + (lane & 7), g = (i >> 3) * 4 + (lane >> 3);
-                    float x[8], y[8];
-                    lt_load8(v + (t0 + t) * a.v_stride[1] + g * 8, t < n ? max(0, min(8, dv - g * 8)) : 0, plan.aligned, x);
-                    const float w = m.power[t < n ? n - 1 - t : 0];
+                for (int g0 = 0; g0 < kGroups; g0 += 2) {  // two pieces on their way together
+                    float x[2][8], y[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = x[e] * w;
-                    lt_store_parts<C::NW>(wt + lt_plain(g, t), C::kTileV, y);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        if (lt_finite(x[e])) continue;
-                        atomicMin(&m.bad, t0 + t);
-                        atomicMin(&m.first_bad[g * 8 + e], t0 + t);
-                        x[e] = 0.0f;
+                    for (int j = 0; j < 2; ++j) {
+                        const int g = (g0 + j) * 4 + (lane >> 3);
+                        lt_load8(v + (t0 + t) * a.v_stride[1] + g * 8, t < n ? max(0, min(8, dv - g * 8)) : 0, plan.aligned, x[j]);
                     }
-                    lt_store_parts<C::NX>(vt + lt_swizzled(g, t), C::kTileV, x);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int g = (g0 + j) * 4 + (lane >> 3);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) y[e] = x[j][e] * weight;
+                        lt_store_parts<C::NW>(wt + lt_plain(g, t), C::kTileV, y);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            if (lt_finite(x[j][e])) continue;
+                            atomicMin(&m.bad, t0 + t);
+                            atomicMin(&m.first_bad[g * 8 + e], t0 + t);
+                            x[j][e] = 0.0f;
+                        }
+                        lt_store_parts<C::NX>(vt + lt_swizzled(g, t), C::kTileV, x[j]);
+                    }
                 }
             }
             fence_proxy_async();
@@ -879,9 +897,16 @@ int64_t linattn_chunk_scratch_bytes(const LinArgs& a) {
     return segs == 1 ? 0 : static_cast<int64_t>(a.batch) * a.heads * segs * a.dk * a.dv * 4;
 }
 
-template <class K>
-static int launch_chunk(K* kernel, dim3 grid, int threads, int bytes, cudaStream_t st, const LinArgs& a, LtPlan plan, const CUtensorMap* maps) {
-    FB_TRY(check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "linear_attention"));
+template <auto kernel>
+static int launch_chunk(dim3 grid, int threads, int bytes, cudaStream_t st, const LinArgs& a, LtPlan plan, const CUtensorMap* maps) {
+    static std::atomic<uint64_t> ready{0};  // devices whose attribute is set (of this instantiation's kernel)
+    int device = 0;
+    FB_TRY(check_cuda(cudaGetDevice(&device), "linear_attention"));
+    const uint64_t bit = 1ull << (device & 63);
+    if (device >= 64 || (ready.load(std::memory_order_relaxed) & bit) == 0) {
+        FB_TRY(check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "linear_attention"));
+        ready.fetch_or(bit, std::memory_order_relaxed);
+    }
     if (plan.segs == 1) return launch_after(kernel, grid, dim3(threads), bytes, st, false, "linear_attention", a, plan, maps[0], maps[1], maps[2]);
     plan.mode = 1;
     FB_TRY(launch_after(kernel, grid, dim3(threads), bytes, st, false, "linear_attention", a, plan, maps[0], maps[1], maps[2]));
@@ -922,9 +947,9 @@ static int launch_chunk(const LinArgs& a, void* scratch, cudaStream_t st) {
                lt_encode(&maps[2], a.v, a.v_stride, a.dv, a.tokens, a.kv_heads, a.batch);
     const dim3 grid(static_cast<unsigned>(ctas));
     if constexpr (C::kBf16) {
-        if (tma) return launch_chunk(linattn_chunk_kernel<T, DK, DV, true>, grid, C::kThreads, bytes, st, a, plan, maps);
+        if (tma) return launch_chunk<linattn_chunk_kernel<T, DK, DV, true>>(grid, C::kThreads, bytes, st, a, plan, maps);
     }
-    return launch_chunk(linattn_chunk_kernel<T, DK, DV, false>, grid, C::kThreads, bytes, st, a, plan, maps);
+    return launch_chunk<linattn_chunk_kernel<T, DK, DV, false>>(grid, C::kThreads, bytes, st, a, plan, maps);
 }
 
 template <typename T>
