@@ -11,7 +11,7 @@
 // finite logits, a constant row), taken by one ordered scan that stops as soon as it has enough.  More candidates than the list holds
 // (rows whose large values sit in few threads) select the bound again by radix, exactly.
 //
-// A row is one CTA, or a cluster of up to eight whose parts meet in the first one's shared memory.
+// A row is one CTA, or a cluster of up to eight whose parts meet in the first one's shared memory; a short row is a warp.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -95,7 +95,7 @@ struct LpVec<__half> {
 };
 
 // sums of one thread, one warp, one part of a row
-struct LpSums {
+struct __align__(16) LpSums {
     float most;  // the largest element (NaN if there is one)
     float ref;   // reference, in powers of two
     float s, t;
@@ -140,18 +140,20 @@ struct LpThread {
     }
 };
 
+template <bool TOP>
 struct LpShared {
     LpSums sums[kLpMaxThreads / 32];
-    LpSums part;                              // of this CTA
-    uint64_t most[kLpMaxThreads];             // maxima of the threads that may have candidates
-    uint64_t above[kLpList], equal[kLpList];  // candidates
+    LpSums part[kLpMaxParts];                 // of the row's CTAs (in the first one)
+    uint64_t most[TOP ? 2 * kLpMaxTop : 1];   // the largest of the threads' maxima, warp by warp
+    uint64_t above[TOP ? kLpList : 1], equal[TOP ? kLpList : 1];  // candidates
     uint64_t best[kLpMaxTop];                 // this CTA's, in order
+    uint64_t parts_best[TOP ? kLpMaxParts * kLpMaxTop : 1];  // of the row's CTAs (in the first one)
     uint64_t row_best[kLpMaxTop];             // the row's
     double log_sum;
     uint32_t hist[256];
     uint32_t warp_count[kLpMaxThreads / 32];
     int busy[kLpBusy];                        // threads that have candidates
-    int num_threads, num_most, num_above, num_equal;
+    int num_threads, num_above, num_equal;
     uint32_t bound, digit, wanted;
     bool empty;
 };
@@ -161,23 +163,33 @@ __device__ __forceinline__ uint32_t lp_cluster_rank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
-__device__ __forceinline__ void lp_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t lp_map(const void* p, uint32_t rank) {
+__device__ __forceinline__ void lp_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void lp_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t lp_first(const void* p) {  // the same place in the row's first CTA
     uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
     return r;
 }
-__device__ __forceinline__ float lp_remote_f32(uint32_t at) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-    return v;
+__device__ __forceinline__ void lp_put(uint32_t at, float x, float y, float z, float w) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
 }
-__device__ __forceinline__ uint64_t lp_remote_u64(uint32_t at) {
-    uint64_t v;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
-    return v;
+__device__ __forceinline__ void lp_put(uint32_t at, uint64_t v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory"); }
+
+// Writes a row's two numbers; returns log sum exp.
+__device__ __forceinline__ double lp_finish(const LpArgs& a, int64_t r, const LpSums& sums, int64_t token, float token_logit, bool& empty) {
+    // (the exponents were x log2e with log2e in 32 bits: the reference goes back by the same number)
+    const double ref = static_cast<double>(sums.ref) / static_cast<double>(kLpLog2e);
+    const double log_s = log(static_cast<double>(sums.s)), log_sum = ref + log_s;
+    empty = sums.most == __int_as_float(0xff800000);
+    float lp = empty ? __int_as_float(0xff800000) : static_cast<float>(static_cast<double>(token_logit) - log_sum);
+    if (token < 0) lp = 0.0f;
+    if (token >= a.vocab) {
+        lp = __int_as_float(0x7fffffff);
+        if (a.status != nullptr) atomicOr(a.status, FB_STATUS_INDEX_RANGE);
+    }
+    a.logprobs[r] = lp;
+    a.entropy[r] = empty ? 0.0f : static_cast<float>(log_s - static_cast<double>(sums.t) / (static_cast<double>(sums.s) * static_cast<double>(kLpLog2e)));
+    return log_sum;
 }
 
 // The elements of a part of a row: vectors, and single ones in front of (first part) and behind (last part) the row's 16-byte boundaries.
@@ -196,59 +208,68 @@ struct LpPart {
     __device__ __forceinline__ uint32_t order(int id) const { return lp_order(LpVec<T>::one(row + id)); }
 };
 
-// number of entries of a list that is in descending order that are above `key`
-__device__ __forceinline__ int lp_above(uint32_t at, int n, uint64_t key) {
+// number of entries of a list in descending order that are above `key`
+__device__ __forceinline__ int lp_above(const uint64_t* list, int n, uint64_t key) {
     int lo = 0, hi = n;
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (lp_remote_u64(at + mid * 8) > key) lo = mid + 1;
+        if (list[mid] > key) lo = mid + 1;
         else hi = mid;
     }
     return lo;
 }
+// the sums of `count` lanes (a power of two) together, in all of them
+__device__ __forceinline__ void lp_join_lanes(LpSums& sums, int count) {
+    for (int d = count / 2; d > 0; d /= 2) {
+        LpSums o;
+        o.most = __shfl_xor_sync(kFullMask, sums.most, d);
+        o.ref = __shfl_xor_sync(kFullMask, sums.ref, d);
+        o.s = __shfl_xor_sync(kFullMask, sums.s, d);
+        o.t = __shfl_xor_sync(kFullMask, sums.t, d);
+        lp_join(sums, o);
+    }
+}
 
-// calls f(order, id) for the elements that thread `who` of the block has, lane `lane` of `lanes` its share of them
+// calls f(order, id) for the elements that this thread has
 template <typename T, class F>
-__device__ __forceinline__ void lp_each(const LpPart<T>& p, int who, int lane, int lanes, F f) {
+__device__ __forceinline__ void lp_each(const LpPart<T>& p, F f) {
     constexpr int N = LpVec<T>::N;
-    const int threads = blockDim.x;
-    for (int v = who + lane * threads; v < p.num_vec; v += lanes * threads) {
+    const int who = threadIdx.x, threads = blockDim.x;
+    for (int v = who; v < p.num_vec; v += threads) {
         float x[N];
         LpVec<T>::get(p.vec(v), x);
 #pragma unroll
         for (int i = 0; i < N; ++i) f(lp_order(x[i]), p.id_of(v) + i);
     }
-    if (lane == 0 && who < p.head) f(p.order(who), who);
-    if (lane == 0 && who < p.tail) f(p.order(p.tail_id + who), p.tail_id + who);
+    if (who < p.head) f(p.order(who), who);
+    if (who < p.tail) f(p.order(p.tail_id + who), p.tail_id + who);
 }
 
 // The `top` best of the part (keys 0 behind them if it has fewer), best first, in sh.best.  most: of this thread's elements.
 template <typename T>
-__device__ void lp_select(LpShared& sh, const LpPart<T>& p, int top, float most) {
+__device__ void lp_select(LpShared<true>& sh, const LpPart<T>& p, int top, float most) {
     constexpr int N = LpVec<T>::N;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
     const uint32_t mine = tid < p.num_vec || tid < p.head || tid < p.tail ? lp_order(most) : 0u;
     if (tid < top) sh.best[tid] = 0;
-    if (tid == 0) sh.num_threads = sh.num_above = sh.num_equal = sh.num_most = 0, sh.bound = 0;
-    // a first bound: the smallest, over the warps, of their (top / warps)-th largest lane
-    uint32_t left = mine, least = 0;
-    for (int i = 0; i < top; i += warps) {
-        least = __reduce_max_sync(kFullMask, left);
-        if (lane == __ffs(__ballot_sync(kFullMask, left == least)) - 1) left = 0;
+    if (tid == 0) sh.num_threads = sh.num_above = sh.num_equal = 0, sh.bound = 0;
+    // a bound: the top-th largest of the warps' (top / warps) largest lanes, by counting
+    const int having = (min(threads, max(p.num_vec, max(p.head, p.tail))) + 31) / 32;  // warps that have elements
+    const int share = having > 0 ? min(32, (top + having - 1) / having) : 0, listed = share * having;
+    uint32_t left = mine;
+    for (int i = 0; i < share && warp < having; ++i) {
+        const uint32_t largest = __reduce_max_sync(kFullMask, left);
+        if (lane == __ffs(__ballot_sync(kFullMask, left == largest)) - 1) {
+            sh.most[warp * share + i] = lp_key(largest, tid);
+            left = 0;
+        }
     }
-    if (lane == 0) sh.warp_count[warp] = least;
     __syncthreads();
-    uint32_t first = sh.warp_count[0];
-    for (int w = 1; w < warps; ++w) first = min(first, sh.warp_count[w]);
-    // the top-th largest of the threads' maxima: among those that reach the first bound, by counting
-    if (mine >= first && mine != 0) sh.most[atomicAdd(&sh.num_most, 1)] = lp_key(mine, tid);
-    __syncthreads();
-    const int reach = sh.num_most;
-    for (int i = tid; i < reach; i += threads) {
-        const uint64_t key = sh.most[i];
+    if (tid < listed) {
+        const uint64_t key = sh.most[tid];
         int rank = 0;
-        for (int j = 0; j < reach; ++j) rank += sh.most[j] > key;
-        if (rank == top - 1) sh.bound = static_cast<uint32_t>(key >> 32);  // (nobody: fewer threads than that have elements, all count)
+        for (int j = 0; j < listed; ++j) rank += sh.most[j] > key;
+        if (rank == top - 1) sh.bound = static_cast<uint32_t>(key >> 32);  // (0 where fewer threads than that have elements: all count)
     }
     __syncthreads();
     uint32_t bound = sh.bound;
@@ -269,9 +290,23 @@ __device__ void lp_select(LpShared& sh, const LpPart<T>& p, int top, float most)
     };
     const int busy = sh.num_threads;
     if (busy <= kLpBusy) {
-        for (int c = warp; c < busy; c += warps) lp_each(p, sh.busy[c], lane, 32, list);
+        // (every piece of theirs on its way at once: one wait for L2)
+        const int each = (p.num_vec + threads - 1) / threads + 1;
+        for (int i = tid; i < busy * each; i += threads) {
+            const int who = sh.busy[i / each], k = i % each, v = who + k * threads;
+            if (k + 1 < each) {
+                if (v >= p.num_vec) continue;
+                float x[N];
+                LpVec<T>::get(p.vec(v), x);
+#pragma unroll
+                for (int e = 0; e < N; ++e) list(lp_order(x[e]), p.id_of(v) + e);
+            } else {
+                if (who < p.head) list(p.order(who), who);
+                if (who < p.tail) list(p.order(p.tail_id + who), p.tail_id + who);
+            }
+        }
     } else {
-        lp_each(p, tid, 0, 1, list);
+        lp_each(p, list);
     }
     __syncthreads();
     if (sh.num_above > kLpList) {
@@ -280,7 +315,7 @@ __device__ void lp_select(LpShared& sh, const LpPart<T>& p, int top, float most)
         for (int shift = 24; shift >= 0; shift -= 8) {
             for (int i = tid; i < 256; i += threads) sh.hist[i] = 0;
             __syncthreads();
-            lp_each(p, tid, 0, 1, [&](uint32_t order, int) {
+            lp_each(p, [&](uint32_t order, int) {
                 if ((order & mask) == prefix) atomicAdd(&sh.hist[(order >> shift) & 255u], 1u);
             });
             __syncthreads();
@@ -300,7 +335,7 @@ __device__ void lp_select(LpShared& sh, const LpPart<T>& p, int top, float most)
         bound = prefix;
         if (tid == 0) sh.num_above = sh.num_equal = 0;
         __syncthreads();
-        lp_each(p, tid, 0, 1, list);
+        lp_each(p, list);
         __syncthreads();
     }
     const int above = sh.num_above, equal = sh.num_equal;
@@ -359,7 +394,7 @@ __device__ void lp_select(LpShared& sh, const LpPart<T>& p, int top, float most)
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kLpMaxThreads) logprobs_kernel(const LpArgs a, int parts) {
     constexpr int N = LpVec<T>::N;
-    __shared__ LpShared sh;
+    __shared__ LpShared<TOP> sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
     const int rank = parts > 1 ? static_cast<int>(lp_cluster_rank()) : 0;
     const int64_t r = blockIdx.x / parts;
@@ -380,6 +415,7 @@ __global__ void __launch_bounds__(kLpMaxThreads) logprobs_kernel(const LpArgs a,
         if (token >= 0 && token < a.vocab) token_logit = LpVec<T>::one(p.row + token);
     }
 
+    if (parts > 1) lp_cluster_arrive();  // (waited for before the first CTA is written to)
     LpThread th;
     th.start();
     if (tid < p.head) th.take({LpVec<T>::one(p.row + tid)});
@@ -401,79 +437,126 @@ __global__ void __launch_bounds__(kLpMaxThreads) logprobs_kernel(const LpArgs a,
         LpVec<T>::get(p.vec(v), x);
         th.take(x);
     }
+    const float most = th.sums.most;
     // the block's sums
-    LpSums sums = th.sums;
-#pragma unroll
-    for (int d = 16; d > 0; d /= 2) {
-        LpSums o;
-        o.most = __shfl_xor_sync(kFullMask, sums.most, d);
-        o.ref = __shfl_xor_sync(kFullMask, sums.ref, d);
-        o.s = __shfl_xor_sync(kFullMask, sums.s, d);
-        o.t = __shfl_xor_sync(kFullMask, sums.t, d);
-        lp_join(sums, o);
-    }
-    if (lane == 0) sh.sums[warp] = sums;
+    lp_join_lanes(th.sums, 32);
+    if (lane == 0) sh.sums[warp] = th.sums;
     __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < warps; ++w) lp_join(sums, sh.sums[w]);
-        sh.part = sums;
+    LpSums sums = {__int_as_float(0xff800000), kLpFloor, 0.0f, 0.0f};
+    if (warp == 0) {
+        if (lane < warps) sums = sh.sums[lane];
+        lp_join_lanes(sums, 16);
     }
-    if (TOP) lp_select<T>(sh, p, a.top, th.sums.most);
-    if (parts > 1) lp_cluster_sync();
-    else __syncthreads();
-    // the row's first CTA finishes it
-    if (rank == 0) {
-        if (tid == 0) {
-            for (int c = 1; c < parts; ++c) {
-                const uint32_t at = lp_map(&sh.part, c);
-                const LpSums o = {lp_remote_f32(at), lp_remote_f32(at + 4), lp_remote_f32(at + 8), lp_remote_f32(at + 12)};
-                lp_join(sums, o);
-            }
-            // (the exponents were x log2e with log2e in 32 bits: the reference goes back by the same number)
-            const double ref = static_cast<double>(sums.ref) / static_cast<double>(kLpLog2e);
-            const double log_s = log(static_cast<double>(sums.s));
-            const bool empty = sums.most == __int_as_float(0xff800000);
-            sh.log_sum = ref + log_s;
-            sh.empty = empty;
-            const double x = static_cast<double>(token_logit);
-            float lp = static_cast<float>(x - sh.log_sum);
-            if (empty) lp = __int_as_float(0xff800000);
-            if (token < 0) lp = 0.0f;
-            if (token >= a.vocab) {
-                lp = __int_as_float(0x7fffffff);
-                if (a.status != nullptr) atomicOr(a.status, FB_STATUS_INDEX_RANGE);
-            }
-            a.logprobs[r] = lp;
-            a.entropy[r] = empty ? 0.0f : static_cast<float>(log_s - static_cast<double>(sums.t) / (static_cast<double>(sums.s) * static_cast<double>(kLpLog2e)));
+    if constexpr (TOP) lp_select<T>(sh, p, a.top, most);
+    if (parts > 1) {
+        // what the parts have meets in the first one's shared memory
+        lp_cluster_wait();  // (it runs)
+        if (tid == 0) lp_put(lp_first(&sh.part[rank]), sums.most, sums.ref, sums.s, sums.t);
+        if (TOP && tid < a.top) lp_put(lp_first(&sh.parts_best[rank * a.top + tid]), sh.best[tid]);
+        lp_cluster_arrive();
+        lp_cluster_wait();
+        if (rank != 0) return;
+        if (warp == 0) {
+            sums = sh.part[lane & (parts - 1)];
+            lp_join_lanes(sums, parts);
         }
-        if (TOP) {
+    }
+    if (tid == 0) {
+        sh.log_sum = lp_finish(a, r, sums, token, token_logit, sh.empty);
+    }
+    if (TOP) {
+        const uint64_t* best = sh.best;
+        if (parts > 1) {
             // every part's list is in order: a candidate's place is the number of larger ones, found by halving
             for (int i = tid; i < parts * a.top; i += threads) {
                 const int c = i / a.top;
-                const uint64_t key = lp_remote_u64(lp_map(&sh.best[i - c * a.top], c));
+                const uint64_t key = sh.parts_best[i];
                 int place = 0;
-                for (int o = 0; o < parts; ++o) place += o == c ? i - c * a.top : lp_above(lp_map(sh.best, o), a.top, key);
+                for (int o = 0; o < parts; ++o) place += o == c ? i - c * a.top : lp_above(sh.parts_best + o * a.top, a.top, key);
                 if (key != 0 && place < a.top) sh.row_best[place] = key;
             }
-            __syncthreads();
-            for (int i = tid; i < a.top; i += threads) {
-                const uint64_t key = sh.row_best[i];
-                const float x = lp_value(static_cast<uint32_t>(key >> 32));
-                a.top_logprobs[r * a.top + i] = sh.empty ? __int_as_float(0xff800000) : static_cast<float>(static_cast<double>(x) - sh.log_sum);
-                a.top_ids[r * a.top + i] = static_cast<int64_t>(0xFFFFFFFFu - static_cast<uint32_t>(key));
-            }
+            best = sh.row_best;
+        }
+        __syncthreads();
+        for (int i = tid; i < a.top; i += threads) {
+            const uint64_t key = best[i];
+            const float x = lp_value(static_cast<uint32_t>(key >> 32));
+            a.top_logprobs[r * a.top + i] = sh.empty ? __int_as_float(0xff800000) : static_cast<float>(static_cast<double>(x) - sh.log_sum);
+            a.top_ids[r * a.top + i] = static_cast<int64_t>(0xFFFFFFFFu - static_cast<uint32_t>(key));
         }
     }
-    if (parts > 1) lp_cluster_sync();  // nobody leaves while the first CTA reads
+}
+
+// Rows of up to 1024 logits: a warp each, its elements in registers, the best taken one by one.
+constexpr int kLpShort = 1024, kLpShortRows = 4;
+template <typename T, int COUNT>
+__global__ void __launch_bounds__(32 * kLpShortRows) logprobs_short_kernel(const LpArgs a, int rows) {
+    const int lane = threadIdx.x & 31;
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * kLpShortRows + (threadIdx.x >> 5);
+    if (r >= rows) return;
+    const T* row = static_cast<const T*>(a.logits) + r * a.row_stride;
+    const int64_t token = a.tokens[r];
+    const float token_logit = token >= 0 && token < a.vocab ? LpVec<T>::one(row + token) : 0.0f;
+    float x[COUNT];  // element i * 32 + lane; -inf where there is none
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) x[i] = i * 32 + lane < a.vocab ? LpVec<T>::one(row + i * 32 + lane) : __int_as_float(0xff800000);
+    LpThread th;
+    th.start();
+    th.take(x);
+    lp_join_lanes(th.sums, 32);
+    double log_sum = 0.0;
+    bool empty = false;
+    if (lane == 0) log_sum = lp_finish(a, r, th.sums, token, token_logit, empty);
+    if (a.top == 0) return;
+    log_sum = __shfl_sync(kFullMask, log_sum, 0);
+    empty = __shfl_sync(kFullMask, empty ? 1 : 0, 0) != 0;
+    uint32_t order[COUNT], most = 0;
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+        order[i] = i * 32 + lane < a.vocab ? lp_order(x[i]) : 0u;
+        most = max(most, order[i]);
+    }
+    for (int k = 0; k < a.top; ++k) {
+        const uint32_t best = __reduce_max_sync(kFullMask, most);
+        uint32_t id = 0xFFFFFFFFu;
+        if (most == best) {
+#pragma unroll
+            for (int i = COUNT - 1; i >= 0; --i)
+                if (order[i] == best) id = i * 32 + lane;
+        }
+        id = __reduce_min_sync(kFullMask, id);
+        if (lane == static_cast<int>(id & 31u)) {  // taken
+            most = 0;
+#pragma unroll
+            for (int i = 0; i < COUNT; ++i) {
+                if (i == static_cast<int>(id >> 5)) order[i] = 0;
+                most = max(most, order[i]);
+            }
+        }
+        if (lane == 0) {
+            a.top_logprobs[r * a.top + k] = empty ? __int_as_float(0xff800000) : static_cast<float>(static_cast<double>(lp_value(best)) - log_sum);
+            a.top_ids[r * a.top + k] = id;
+        }
+    }
+}
+
+template <typename T>
+static int launch_logprobs_short(const LpArgs& a, int rows, cudaStream_t st) {
+    const dim3 grid((rows + kLpShortRows - 1) / kLpShortRows), block(32 * kLpShortRows);
+    if (a.vocab <= 256) return launch_after(logprobs_short_kernel<T, 8>, grid, block, 0, st, false, "token_logprobs", a, rows);
+    return launch_after(logprobs_short_kernel<T, kLpShort / 32>, grid, block, 0, st, false, "token_logprobs", a, rows);
 }
 
 template <typename T, bool TOP>
 static int launch_logprobs(const LpArgs& a, int rows, cudaStream_t st) {
     const int vecs = a.vocab / LpVec<T>::N;
+    // One CTA per row, and per SM, unless rows are few; a part of 512 vectors at least (one row of 32000 fp32 logits: 8.9 us in eight parts,
+    // 12.6 in one).  With several rows per SM 256 threads a row (4096 rows of 32000: 54 us, with 512 threads 62), else 512 (256 rows of
+    // 131072: 25 and 35).
     int parts = 1;
-    while (parts < kLpMaxParts && static_cast<int64_t>(rows) * parts * 2 <= 2 * kNumSMs && vecs / (parts * 2) >= 256) parts *= 2;
+    while (parts < kLpMaxParts && static_cast<int64_t>(rows) * parts * 2 <= kNumSMs && vecs / (parts * 2) >= 512) parts *= 2;
     const int each = vecs / parts;
-    const int threads = each >= 1024 ? 512 : each >= 512 ? 256 : each >= 128 ? 128 : 64;
+    const int threads = each >= 1024 ? (rows >= 4 * kNumSMs ? 256 : 512) : each >= 512 ? 256 : each >= 128 ? 128 : 64;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(rows) * parts);
     cfg.blockDim = dim3(threads);
@@ -491,6 +574,7 @@ static int launch_logprobs(const LpArgs& a, int rows, cudaStream_t st) {
 
 template <typename T>
 static int launch_logprobs(const LpArgs& a, int rows, cudaStream_t st) {
+    if (a.vocab <= kLpShort) return launch_logprobs_short<T>(a, rows, st);
     return a.top > 0 ? launch_logprobs<T, true>(a, rows, st) : launch_logprobs<T, false>(a, rows, st);
 }
 
