@@ -1,13 +1,13 @@
 // Attention with a decaying state, token by token:  S = decay * S + k v^T,  out = scale * S^T q.
 //
-// Serves single tokens (a pass over the states) and, so far, prompts of any length.
+// Serves single tokens, which are a pass over the states (bound by their traffic: 8 bytes per cell), and prompts of few tokens (bound by the
+// latency of a token: its sums over the rows of S).  Longer prompts go chunk by chunk.  A state never leaves registers between tokens.
 #include <type_traits>
 
 #include "linattn.cuh"
 
 namespace fb {
 
-constexpr int kLinFewTokens = 32;  // up to here token by token
 constexpr int kRecurThreads = 256;
 constexpr int kRecurTokens = 8;  // tokens staged at a time
 
@@ -121,12 +121,93 @@ __global__ void __launch_bounds__(kRecurThreads) linattn_recurrent_kernel(const 
     }
 }
 
+// One token, many states: a CTA has a whole state, LANES lanes a row of it, so that 64 KB are on their way at once and one slot is looked up.
+constexpr int kStepThreads = 256;
+template <typename T, int LANES>
+__global__ void __launch_bounds__(kStepThreads) linattn_step_kernel(const LinArgs a) {
+    constexpr int WARPS = kStepThreads / 32, PER = 32 / LANES, STEP = WARPS * PER, ROWS = kLinMaxDim / STEP;
+    __shared__ float s_q[kLinMaxDim], s_k[kLinMaxDim];
+    __shared__ __align__(16) float s_part[WARPS][LANES * 4];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int h = blockIdx.x % a.heads, b = blockIdx.x / a.heads, hk = h / (a.heads / a.kv_heads);
+    const int row = warp * PER + lane / LANES, col = (lane % LANES) * 4;
+    const bool has_col = col < a.dv;
+    const int named = a.slots == nullptr ? b : a.slots[b];
+    const bool inside = named >= 0 && named < a.num_slots;
+    const int64_t state = (static_cast<int64_t>(inside ? named : 0) * a.heads + h) * a.dk * a.dv;
+    // the state first: it may be read whether the slot is this sequence's or an earlier one's
+    float4 s[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const int r = row + i * STEP;
+        s[i] = inside && has_col && r < a.dk && a.state_in != nullptr ? *reinterpret_cast<const float4*>(a.state_in + state + static_cast<int64_t>(r) * a.dv + col)
+                                                                      : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    const T* q = static_cast<const T*>(a.q) + b * a.q_stride[0] + h * a.q_stride[2];
+    const T* k = static_cast<const T*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2];
+    const T* v = static_cast<const T*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2];
+    T* out = static_cast<T*>(a.out) + b * a.out_stride[0] + h * a.out_stride[2];
+    if (tid < kLinMaxDim) s_q[tid] = tid < a.dk ? lin_float(q[tid]) : 0.0f;
+    else s_k[tid - kLinMaxDim] = tid - kLinMaxDim < a.dk ? lin_float(k[tid - kLinMaxDim]) : 0.0f;
+    float x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = has_col ? lin_float(v[col + j]) : 0.0f;
+    int bits;
+    const int slot = lin_slot(a, b, lane, bits);
+    if (bits != 0 && a.status != nullptr && tid == 0) atomicOr(a.status, bits);
+    const double exact = exp(static_cast<double>(a.log_decay[h]));  // (a sum of two floats: see above)
+    const float decay = static_cast<float>(exact), decay_lo = static_cast<float>(exact - static_cast<double>(decay));
+    __syncthreads();
+    float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const float kr = s_k[row + i * STEP], qr = s_q[row + i * STEP];
+        s[i].x = fmaf(kr, x[0], fmaf(decay, s[i].x, decay_lo * s[i].x));
+        s[i].y = fmaf(kr, x[1], fmaf(decay, s[i].y, decay_lo * s[i].y));
+        s[i].z = fmaf(kr, x[2], fmaf(decay, s[i].z, decay_lo * s[i].z));
+        s[i].w = fmaf(kr, x[3], fmaf(decay, s[i].w, decay_lo * s[i].w));
+        o[0] = fmaf(qr, s[i].x, o[0]), o[1] = fmaf(qr, s[i].y, o[1]), o[2] = fmaf(qr, s[i].z, o[2]), o[3] = fmaf(qr, s[i].w, o[3]);
+        const int r = row + i * STEP;
+        if (slot >= 0 && has_col && r < a.dk) *reinterpret_cast<float4*>(a.state_out + state + static_cast<int64_t>(r) * a.dv + col) = s[i];
+    }
+#pragma unroll
+    for (int d = LANES; d < 32; d *= 2) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] += __shfl_xor_sync(kFullMask, o[j], d);
+    }
+    if (lane < LANES) *reinterpret_cast<float4*>(&s_part[warp][col]) = make_float4(o[0], o[1], o[2], o[3]);
+    __syncthreads();
+    if (tid < a.dv) {
+        float y = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) y += s_part[w][tid];
+        out[tid] = lin_from<T>(slot >= 0 ? y * a.scale : 0.0f);
+    }
+}
+
+// Whether a prompt goes chunk by chunk (kernels_linattn_tc.cu) or token by token.  A chunk takes 11.6 us per wave of heads however few tokens it
+// has.  Token by token it is 3.5 us and 0.3 per token while the column tiles are on an SM each, 0.25 per token and tile of an SM beyond
+// that: 8 heads of 64, 24 tokens 10.8 (11.6 as a chunk); 128 heads of 128, 8 tokens 11.0 (11.7), 24 tokens 24.8; 1024 heads, 8 tokens 73 (83).
+static bool lin_by_chunks(const LinArgs& a) {
+    const int64_t heads = static_cast<int64_t>(a.batch) * a.heads, tiles = heads * ((a.dv + 31) / 32);
+    const double chunk = 11.6 * static_cast<double>((heads + kNumSMs - 1) / kNumSMs);
+    const double token = 0.25 * static_cast<double>(tiles) / kNumSMs;
+    return a.tokens > 1 && 3.5 + a.tokens * (token > 0.3 ? token : 0.3) > chunk;
+}
+
 template <typename T>
 static int launch_recurrent(const LinArgs& a, cudaStream_t st) {
     const bool vec = a.dv % 4 == 0 && reinterpret_cast<uintptr_t>(a.state_in) % 16 == 0 && reinterpret_cast<uintptr_t>(a.state_out) % 16 == 0;
     const int64_t bh = static_cast<int64_t>(a.batch) * a.heads;
     const int tiles = (a.dv + 31) / 32;
     FB_REQUIRE(bh * tiles < (1ll << 31), "linear_attention: batch * heads is too large");
+    // (from two states per SM on: 96 x 16 states of 128 x 128 52 us in column tiles, 41 in whole ones; 16 states alone 4.3 and 5.1)
+    if (vec && a.tokens == 1 && a.lengths == nullptr && bh >= 2 * kNumSMs) {
+        const dim3 whole(static_cast<unsigned>(bh)), block(kStepThreads);
+        if (a.dv <= 32) return launch_after(linattn_step_kernel<T, 8>, whole, block, 0, st, false, "linear_attention", a);
+        if (a.dv <= 64) return launch_after(linattn_step_kernel<T, 16>, whole, block, 0, st, false, "linear_attention", a);
+        return launch_after(linattn_step_kernel<T, 32>, whole, block, 0, st, false, "linear_attention", a);
+    }
     const dim3 grid(static_cast<unsigned>(bh * tiles));
     if (vec) return launch_after(linattn_recurrent_kernel<T, 8, true>, grid, dim3(kRecurThreads), 0, st, false, "linear_attention", a, tiles);
     return launch_after(linattn_recurrent_kernel<T, 8, false>, grid, dim3(kRecurThreads), 0, st, false, "linear_attention", a, tiles);
@@ -136,7 +217,7 @@ static int launch_recurrent(const LinArgs& a, cudaStream_t st) {
 
 extern "C" int64_t functs_b200_linear_attention_scratch_bytes(const functs_b200_linear_attention_args* a) {
     using namespace fb;
-    if (a == nullptr || a->batch <= 0 || a->heads <= 0 || a->dk <= 0 || a->dv <= 0 || a->tokens <= kLinFewTokens) return 0;
+    if (a == nullptr || a->batch <= 0 || a->heads <= 0 || a->dk <= 0 || a->dv <= 0 || !lin_by_chunks(*a)) return 0;
     return linattn_chunk_scratch_bytes(*a);
 }
 
@@ -155,7 +236,7 @@ extern "C" int functs_b200_linear_attention(const functs_b200_linear_attention_a
     FB_REQUIRE(a.log_decay != nullptr && a.state_out != nullptr, "linear_attention: null pointer");
     FB_REQUIRE(a.tokens == 0 || (a.q != nullptr && a.k != nullptr && a.v != nullptr && a.out != nullptr), "linear_attention: null pointer");
     const cudaStream_t st = as_stream(stream);
-    if (a.tokens > kLinFewTokens) return launch_linattn_chunk(a, scratch, st);
+    if (lin_by_chunks(a)) return launch_linattn_chunk(a, scratch, st);
     if (a.dtype == FB_DTYPE_F32) return launch_recurrent<float>(a, st);
     if (a.dtype == FB_DTYPE_F16) return launch_recurrent<__half>(a, st);
     return launch_recurrent<__nv_bfloat16>(a, st);
