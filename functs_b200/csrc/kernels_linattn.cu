@@ -101,10 +101,7 @@ __global__ void __launch_bounds__(kRecurThreads) linattn_recurrent_kernel(const 
             if (d < cols) out[(t0 + t) * a.out_stride[1] + d] = lin_from<T>(o * a.scale);
         }
     }
-    for (int i = tid; i < (a.tokens - length) * cols; i += kRecurThreads) {
-        const int t = i / cols, d = i - t * cols;
-        out[(length + t) * a.out_stride[1] + d] = lin_from<T>(0.0f);
-    }
+    lin_clear(out, a.out_stride[1], length, a.tokens, cols);
     if (slot < 0) return;
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {

@@ -303,10 +303,7 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
     T* out = static_cast<T*>(a.out) + b * a.out_stride[0] + h * a.out_stride[2] + col0;
     if (outputs) {  // rows behind the sequence, those that fall in this part
         const int z0 = max(length, seg0), z1 = plan.segs > 1 && seg + 1 < plan.segs ? min(a.tokens, seg0 + plan.seg_tokens) : a.tokens;
-        for (int64_t i = tid; i < static_cast<int64_t>(max(0, z1 - z0)) * dv; i += C::kThreads) {
-            const int64_t t = i / dv;
-            out[(z0 + t) * a.out_stride[1] + (i - t * dv)] = lin_from<T>(0.0f);
-        }
+        lin_clear(out, a.out_stride[1], z0, z1, dv);
     }
     if (slot < 0 || (plan.mode == 2 && seg_end <= seg0)) return;
     const int chunks = max(0, seg_end - seg0 + kLtChunk - 1) / kLtChunk;

@@ -37,6 +37,23 @@ __device__ __forceinline__ int lin_length(const LinArgs& a, int b) {
     return a.lengths == nullptr ? a.tokens : min(max(a.lengths[b], 0), a.tokens);
 }
 
+// Zeros in rows [first, last) of a head's output, `cols` of them adjacent; the whole block, a warp's lanes along a row (or along several,
+// 16 bytes each, where they lie on such boundaries).
+template <typename T>
+__device__ __forceinline__ void lin_clear(T* out, int64_t stride, int first, int last, int cols) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    constexpr int N = 16 / sizeof(T);
+    if (cols % N == 0 && stride % N == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0) {
+        const int pieces = cols / N, rows = 32 / pieces, row = lane / pieces;  // (up to 32 pieces: 128 channels of 4 bytes)
+        if (row >= rows) return;
+        for (int t = first + warp * rows + row; t < last; t += warps * rows)
+            *reinterpret_cast<uint4*>(out + t * stride + (lane - row * pieces) * N) = make_uint4(0, 0, 0, 0);
+    } else {
+        for (int t = first + warp; t < last; t += warps)
+            for (int c = lane; c < cols; c += 32) out[t * stride + c] = lin_from<T>(0.0f);
+    }
+}
+
 // The state that sequence b uses, or -1 for none; `bits` gets the status bit that says why.  Called by a whole warp.
 __device__ __forceinline__ int lin_slot(const LinArgs& a, int b, int lane, int& bits) {
     bits = 0;
