@@ -55,7 +55,7 @@ struct LtCfg {
     static constexpr int kTileK = kLtChunk * DK * 2, kTileV = kLtChunk * DV * 2, kPartP = kLtChunk * kLtChunk * 2;
     static constexpr int kStage = 2 * NX * kTileK, oK = NX * kTileK;  // Q, and K behind it
     // stages of Q and K, and of W: two where they fit; of V in bf16 three (it is read a chunk ahead, for W)
-    static constexpr int kStages = 2 * (kStage + (NX + NW) * kTileV) + NS * kPartP <= 222 * 1024 ? 2 : 1;
+    static constexpr int kStages = 2 * (kStage + (NX + NW) * kTileV) + NS * kPartP <= 224 * 1024 ? 2 : 1;
     static constexpr int kStagesV = kBf16 ? 3 : kStages;
     static constexpr int oV = kStages * kStage, oW = oV + kStagesV * NX * kTileV, oP = oW + kStages * NW * kTileV, oMisc = oP + NS * kPartP;
     static constexpr uint32_t kParts = NS == 3 ? kLtS : kLtS + 128;  // TMEM columns of the parts of S^T
@@ -869,17 +869,19 @@ __global__ void __launch_bounds__(256) linattn_carry_kernel(const LinArgs a, flo
 }
 
 // How many parts a sequence is cut into.  Cutting costs a second reading of K and V for the states of the parts (about 0.4 of a chunk's time
-// for each of its chunks) and two more launches, so it pays where whole sequences leave SMs without work.
+// for each of its chunks) and two more launches (9 us; a chunk is 2.8 us in bf16, 6 and more in the other types), so it pays where whole
+// sequences leave SMs without work: 8192 tokens of 16 heads 408 us whole, 119 in nine parts.
 static void lt_cut(const LinArgs& a, int64_t rows, int& segs, int& seg_tokens) {
     const int chunks = (a.tokens + kLtChunk - 1) / kLtChunk;
     segs = 1;
     seg_tokens = 0;
-    const double whole = static_cast<double>((rows + kNumSMs - 1) / kNumSMs) * chunks;
-    double best = whole;
-    for (int n = 2; n <= 64 && n * 4 <= chunks; ++n) {
+    if (rows > 65535) return;
+    const double launches = a.dtype == FB_DTYPE_BF16 ? 3.2 : 1.5;
+    double best = static_cast<double>((rows + kNumSMs - 1) / kNumSMs) * chunks;
+    for (int n = 2; n <= 64 && n * 2 <= chunks; ++n) {
         const int each = (chunks + n - 1) / n;
         const int parts = (chunks + each - 1) / each;
-        const double cost = static_cast<double>((rows * parts + kNumSMs - 1) / kNumSMs) * (each * 1.4 + 1.0) + 4.0;
+        const double cost = static_cast<double>((rows * parts + kNumSMs - 1) / kNumSMs) * (each * 1.4 + 1.0) + launches;
         if (cost < best) {
             best = cost;
             segs = parts;
@@ -922,7 +924,6 @@ static int launch_chunk(const LinArgs& a, void* scratch, cudaStream_t st) {
     plan.tiles = (a.dv + DV - 1) / DV;
     const int64_t rows = static_cast<int64_t>(a.batch) * a.heads;
     lt_cut(a, rows, plan.segs, plan.seg_tokens);
-    if (rows > 65535) plan.segs = 1;
     FB_REQUIRE(plan.segs == 1 || (scratch != nullptr && reinterpret_cast<uintptr_t>(scratch) % 16 == 0), "linear_attention: scratch must be given, 16-byte aligned");
     plan.states = static_cast<float*>(scratch);
     const int64_t ctas = static_cast<int64_t>(a.batch) * a.heads * plan.tiles * plan.segs;
