@@ -82,7 +82,7 @@ struct LtPlan {
     int segs;        // parts of a sequence
     int seg_tokens;  // a multiple of the chunk
     int mode;        // 0: whole sequences; 1: the state that each part adds, 2: outputs of the parts
-    bool aligned;
+    int boundary;    // of which all rows lie: 16, 8, 4 or 2 bytes
     float* states;   // [batch * heads][segs][dk][dv]
 };
 
@@ -218,20 +218,23 @@ __device__ __forceinline__ void lt_store_parts(unsigned char* at, int stride, fl
     }
 }
 
-// Eight channels of one row in fp32, zeros behind `valid`.
-template <typename T>
-__device__ __forceinline__ void lt_load8(const T* p, int valid, bool aligned, float (&x)[8]) {
-    if (aligned && valid == 8) {
-        if (sizeof(T) == 4) {
-            const float4 a = *reinterpret_cast<const float4*>(p), b = *(reinterpret_cast<const float4*>(p) + 1);
-            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-        } else {
-            const uint4 u = *reinterpret_cast<const uint4*>(p);
-            const T* e = reinterpret_cast<const T*>(&u);
+// Eight channels of one row in fp32, zeros behind `valid`; in the largest loads that the rows' boundary allows.
+template <typename T, typename P>
+__device__ __forceinline__ void lt_load8_as(const T* p, float (&x)[8]) {
+    constexpr int N = sizeof(P) / sizeof(T);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = lin_float(e[i]);
-        }
-    } else {
+    for (int i = 0; i < 8; i += N) {
+        const P u = reinterpret_cast<const P*>(p)[i / N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[i + j] = lin_float(reinterpret_cast<const T*>(&u)[j]);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void lt_load8(const T* p, int valid, int boundary, float (&x)[8]) {
+    if (valid == 8 && boundary == 16) lt_load8_as<T, uint4>(p, x);
+    else if (valid == 8 && boundary == 8) lt_load8_as<T, uint2>(p, x);
+    else if (sizeof(T) == 2 && valid == 8 && boundary == 4) lt_load8_as<T, uint32_t>(p, x);
+    else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = i < valid ? lin_float(p[i]) : 0.0f;
     }
@@ -508,8 +511,8 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
                     for (int j = 0; j < 2; ++j) {
                         const int i = id + (i0 + j) * threads, g = i % (DK / 8), t = i / (DK / 8);
                         const int valid = t < n ? max(0, min(8, a.dk - g * 8)) : 0;
-                        lt_load8(k + (t0 + t) * a.k_stride[1] + g * 8, valid, plan.aligned, y[j]);
-                        if (outputs) lt_load8(q + (t0 + t) * a.q_stride[1] + g * 8, valid, plan.aligned, x[j]);
+                        lt_load8(k + (t0 + t) * a.k_stride[1] + g * 8, valid, plan.boundary, y[j]);
+                        if (outputs) lt_load8(q + (t0 + t) * a.q_stride[1] + g * 8, valid, plan.boundary, x[j]);
                     }
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
@@ -565,7 +568,7 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         const int g = (g0 + j) * 4 + (lane >> 3);
-                        lt_load8(v + (t0 + t) * a.v_stride[1] + g * 8, t < n ? max(0, min(8, dv - g * 8)) : 0, plan.aligned, x[j]);
+                        lt_load8(v + (t0 + t) * a.v_stride[1] + g * 8, t < n ? max(0, min(8, dv - g * 8)) : 0, plan.boundary, x[j]);
                     }
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
@@ -928,19 +931,17 @@ static int launch_chunk(const LinArgs& a, void* scratch, cudaStream_t st) {
     plan.states = static_cast<float*>(scratch);
     const int64_t ctas = static_cast<int64_t>(a.batch) * a.heads * plan.tiles * plan.segs;
     FB_REQUIRE(ctas < (1ll << 31), "linear_attention: batch * heads is too large");
-    plan.aligned = true;
     const void* base[3] = {a.q, a.k, a.v};
     const int64_t* stride[3] = {a.q_stride, a.k_stride, a.v_stride};
-    const int64_t sizes[3] = {a.batch, a.tokens, 0};
+    uint64_t lies = 16;
     for (int i = 0; i < 3; ++i) {
-        plan.aligned = plan.aligned && reinterpret_cast<uintptr_t>(base[i]) % 16 == 0;
-        for (int j = 0; j < 3; ++j) {
-            const int64_t size = j < 2 ? sizes[j] : i == 0 ? a.heads : a.kv_heads;
-            plan.aligned = plan.aligned && (size == 1 || stride[i][j] * static_cast<int64_t>(sizeof(T)) % 16 == 0);
-        }
+        const int64_t sizes[3] = {a.batch, a.tokens, i == 0 ? a.heads : a.kv_heads};
+        lies |= reinterpret_cast<uintptr_t>(base[i]);
+        for (int j = 0; j < 3; ++j) lies |= sizes[j] == 1 ? 0 : static_cast<uint64_t>(stride[i][j]) * sizeof(T);
     }
+    plan.boundary = static_cast<int>(lies & (~lies + 1));
     CUtensorMap maps[3] = {};
-    const bool tma = C::kBf16 && plan.aligned && lt_encode(&maps[0], a.q, a.q_stride, a.dk, a.tokens, a.heads, a.batch) &&
+    const bool tma = C::kBf16 && plan.boundary == 16 && lt_encode(&maps[0], a.q, a.q_stride, a.dk, a.tokens, a.heads, a.batch) &&
                lt_encode(&maps[1], a.k, a.k_stride, a.dk, a.tokens, a.kv_heads, a.batch) &&
                lt_encode(&maps[2], a.v, a.v_stride, a.dv, a.tokens, a.kv_heads, a.batch);
     const dim3 grid(static_cast<unsigned>(ctas));

@@ -32,8 +32,31 @@ void checkSizes(const at::Tensor& t, at::IntArrayRef sizes, const char* name) {
     TORCH_CHECK_VALUE(t.sizes() == sizes, name, " must be of sizes ", sizes, ", not ", t.sizes());
 }
 
-int32_t* statusWord(const MaybeTensor& status, const at::Device& device) {
-    if (!status.has_value()) return nullptr;
+// Where a kernel says that a wait of its own ran out, for callers that give no status word: in pinned host memory, asked at the next call.
+// (Slots and tokens that are out of range are the caller's; without a status word they are skipped as documented, and not reported.)
+int32_t* ownStatusWord() {
+    static int32_t* const word = [] {
+        void* p = nullptr;
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // (the first call may be one that is captured)
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        const cudaError_t rc = cudaHostAlloc(&p, 64, cudaHostAllocPortable | cudaHostAllocMapped);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (rc != cudaSuccess) {
+            cudaGetLastError();
+            return static_cast<int32_t*>(nullptr);
+        }
+        *static_cast<int32_t*>(p) = 0;
+        return static_cast<int32_t*>(p);
+    }();
+    if (word != nullptr && (*static_cast<volatile int32_t*>(word) & FB_STATUS_WAIT_TIMEOUT) != 0) {
+        *static_cast<volatile int32_t*>(word) = 0;
+        TORCH_CHECK(false, "linear_attention: a bounded device-side wait ran out in an earlier call; its outputs mean nothing");
+    }
+    return word;
+}
+
+int32_t* statusWord(const MaybeTensor& status, const at::Device& device, bool own) {
+    if (!status.has_value()) return own ? ownStatusWord() : nullptr;
     TORCH_CHECK_VALUE(status->scalar_type() == at::kInt && status->numel() >= 1 && (status->device() == device || status->is_pinned()),
                       "status must be an int32 tensor on ", device, " or in pinned memory");
     return status->data_ptr<int32_t>();
@@ -87,7 +110,7 @@ void run(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at
         lengths_c = lengths->contiguous();
         a.lengths = lengths_c.data_ptr<int32_t>();
     }
-    a.status = statusWord(status, device);
+    a.status = statusWord(status, device, /*own=*/tokens > 1);
     a.scale = static_cast<float>(scale);
     at::Tensor scratch;
     const int64_t bytes = functs_b200_linear_attention_scratch_bytes(&a);
@@ -188,7 +211,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> tokenLogprobs(const a
                top_ids = at::empty({R, top}, f32.dtype(at::kLong));
     checkRc(functs_b200_token_logprobs(x.data_ptr(), dtype, x.stride(0), ids.data_ptr<int64_t>(), narrow(R, "rows"), narrow(V, "vocab"),
                                        static_cast<int32_t>(top), lp.data_ptr<float>(), entropy.data_ptr<float>(), top_lp.data_ptr<float>(),
-                                       top_ids.data_ptr<int64_t>(), statusWord(status, device), at::cuda::getCurrentCUDAStream().stream()),
+                                       top_ids.data_ptr<int64_t>(), statusWord(status, device, /*own=*/false), at::cuda::getCurrentCUDAStream().stream()),
             "token_logprobs");
     return {lp, entropy, top_lp, top_ids};
 }

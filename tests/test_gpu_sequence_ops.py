@@ -453,3 +453,59 @@ def test_logprobs_refuses(ops):
             f()
     lp, entropy, top_lp, top_ids = ops.token_logprobs(x[:0], t[:0], top=2)
     assert lp.shape == (0,) and top_ids.shape == (0, 2)
+
+
+@pytest.mark.parametrize("vocab", [200, 1000])
+@pytest.mark.parametrize("kind", ["constant", "two values", "few finite", "zeros", "rising"])
+def test_logprobs_of_short_rows(ops, kind, vocab):
+    x = torch.randn(37, vocab, device="cuda")
+    if kind == "constant":
+        x = torch.full((37, vocab), 2.0, device="cuda")
+    elif kind == "two values":
+        x = torch.where(x > 1.5, 1.0, 0.25)
+    elif kind == "few finite":
+        x[:, 3:] = -math.inf
+    elif kind == "zeros":
+        x = torch.where(x > 0, 0.0, -0.0)
+    elif kind == "rising":
+        x = torch.arange(vocab, device="cuda", dtype=F32).repeat(37, 1)
+    for dtype in (F32, F16, BF16):
+        for top in (0, 1, 20, 64):
+            check_logprobs(ops, x.to(dtype).contiguous(), torch.randint(0, vocab, (37,), device="cuda"), top)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("dk,dv,front", [(100, 100, 0), (60, 36, 0), (64, 64, 4), (64, 64, 2), (128, 128, 1)])
+def test_prompt_rows_on_other_boundaries(ops, dk, dv, front, dtype):
+    """Rows on boundaries of 8, 4 and 2 bytes take other loads than those of 16."""
+    b, t, h = 2, 150, 2
+    x = torch.randn(b, t, h, 2 * dk + dv + 8, device="cuda").to(dtype)
+    q, k, v = x[..., front:front + dk], x[..., front + dk:front + 2 * dk], x[..., front + 2 * dk:front + 2 * dk + dv]
+    out, state = ops.linear_attention(q, k, v, decays(h), scale=dk ** -0.5)
+    check_attention(out, state, recurrence(q, k, v, decays(h), dk ** -0.5, None, torch.full((b,), t, device="cuda")), dtype, t, dk)
+
+
+def test_first_call_in_a_capture(cuda_device):
+    """A process whose first prompt is captured into a graph."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from functs_b200 import ops
+q, k, v = (torch.randn(1, 200, 2, 64, device="cuda", dtype=torch.bfloat16) for _ in range(3))
+g = torch.tensor([-0.1, -0.5], device="cuda")
+x, ids = torch.randn(2, 5000, device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out, state = ops.linear_attention(q, k, v, g)
+    lp = ops.token_logprobs(x, ids, top=3)
+for _ in range(2):
+    graph.replay()
+torch.cuda.synchronize()
+want = ops.linear_attention(q, k, v, g)
+assert torch.equal(out, want[0]) and torch.equal(state, want[1])
+assert all(torch.equal(a, b) for a, b in zip(lp, ops.token_logprobs(x, ids, top=3)))
+print("same")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
