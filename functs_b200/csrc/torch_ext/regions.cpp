@@ -16,14 +16,16 @@
 //                         top level; on equality the window is replaced by ONE tssa::ParallelFunctor node that carries
 //                         the pattern's name (attribute `region`), the free constants as named attributes, the tensor
 //                         constants (attribute `tparams`) and, as Subgraph, a copy of the window it replaced.
-//   operator              a region functor never interprets its subgraph: it allocates outputs and scratch with torch and
+//   operator              a region functor never interprets its subgraph (one does, see there): it allocates outputs and scratch with torch and
 //                         launches on the current stream (functs_b200_group_launch; the detection programs through
 //                         detect.cpp, which watches the images' counts in host memory and makes the ragged lists).
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <ATen/core/grad_mode.h>
 #include <torch/csrc/jit/ir/constants.h>
 #include <torch/csrc/jit/ir/ir.h>
+#include <torch/csrc/jit/runtime/graph_executor.h>
 #include <torch/csrc/jit/runtime/operator.h>
 
 #include <cmath>
@@ -36,6 +38,7 @@
 #include "../../../include/functs_b200.h"
 #include "detect.h"
 #include "fusion.h"
+#include "sequence.h"
 
 namespace functs_b200 {
 
@@ -494,6 +497,51 @@ Operation makeLstm(const Node* node) {
     };
 }
 
+// ---- attention with a decaying state ----------------------------------------------------------------------------------
+// Pattern inputs: q, v, k; outputs: the last state [B, H, Dk, Dv], outs [T, B, H, Dv].  Tensor constant: decay [H, 1, 1].
+// Unlike the other regions this one does interpret its subgraph where the kernels do not fit the call (other types or devices, channels
+// beyond 128, decays outside [0, 1], inputs that require gradients): such a program ran before there was a kernel for it.
+Operation makeDecayAttention(const Node* node) {
+    const std::vector<at::Tensor> tc = node->ts(kAttrTParams);
+    TORCH_CHECK(tc.size() == 1, "decay attention region: expected the decay constant, got ", tc.size());
+    const at::Tensor decay = tc[0].to(at::kCPU);
+    bool fits = decay.scalar_type() == at::kFloat && decay.dim() == 3 && decay.size(1) == 1 && decay.size(2) == 1 && decay.size(0) >= 1;
+    fits = fits && decay.ge(0).logical_and(decay.le(1)).all().item<bool>();
+    const at::Tensor log_decay = fits ? decay.reshape({-1}).to(at::kDouble).log().to(at::kFloat) : at::Tensor();
+    auto consts = std::make_shared<DeviceConstants>();
+    auto exec = std::make_shared<GraphExecutor>(node->g(attr::Subgraph)->copy(), "functs_b200_decay_attention");
+    return [=](Stack& stack) {
+        const at::Tensor q = peek(stack, 0, 3).toTensor(), v = peek(stack, 1, 3).toTensor(), k = peek(stack, 2, 3).toTensor();
+        bool here = fits;
+        for (const at::Tensor* t : {&q, &k, &v})
+            here = here && t->is_cuda() && t->device() == q.device() && t->scalar_type() == at::kFloat && t->dim() == 4 &&
+                   !(t->requires_grad() && at::GradMode::is_enabled());
+        here = here && q.size(2) == log_decay.size(0) && k.sizes() == q.sizes() && v.size(0) == q.size(0) && v.size(1) == q.size(1) &&
+               v.size(2) == q.size(2) && q.size(3) >= 1 && q.size(3) <= 128 && v.size(3) >= 1 && v.size(3) <= 128;
+        if (!here) {
+            countInterpretedRun();
+            Stack own{q, v, k};
+            drop(stack, 3);
+            exec->run(own);
+            for (auto& value : own) stack.push_back(std::move(value));
+            return;
+        }
+        drop(stack, 3);
+        c10::cuda::CUDAGuard guard(q.device());
+        at::Tensor log_d;
+        {
+            std::lock_guard<std::mutex> lock(consts->m);
+            auto& c = consts->per_device[q.get_device()];
+            if (c.empty()) c.push_back(log_decay.to(q.device()));
+            log_d = c[0];
+        }
+        at::Tensor outs = at::empty({q.size(0), q.size(1), q.size(2), v.size(3)}, q.options());
+        at::Tensor last = std::get<1>(linearAttention(q.transpose(0, 1), k.transpose(0, 1), v.transpose(0, 1), log_d, 1.0, std::nullopt,
+                                                      std::nullopt, std::nullopt, outs.transpose(0, 1), std::nullopt));
+        push(stack, std::move(last), std::move(outs));
+    };
+}
+
 // ---- C5: YOLACT-style mask assembly ----------------------------------------------------------------------------------
 // Pattern outputs (loop results in order): logits [B, H, W, N], masks [B, N, H, W]   (with_logits = 1)   or: masks.
 Operation makeYolact(const Node* node, bool with_logits) {
@@ -530,6 +578,7 @@ const std::unordered_map<std::string, Adapter>& adapters() {
         {"yolov3_post", [](const Node* n) { return makeYolo(n, false); }},
         {"ssd_post", [](const Node* n) { return makeSsd(n); }},
         {"lstm_seq", [](const Node* n) { return makeLstm(n); }},
+        {"decay_attention_seq", [](const Node* n) { return makeDecayAttention(n); }},
         {"yolact_masks_logits", [](const Node* n) { return makeYolact(n, true); }},
         {"yolact_masks", [](const Node* n) { return makeYolact(n, false); }},
     };

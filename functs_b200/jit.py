@@ -119,6 +119,7 @@ def build(fn, example_inputs=(), add_clone: bool = False):
         hints = [None] + hints  # self
     from . import patterns
     patterns.register_all()  # the programs that the precompiled kernel sequences stand for (once per process)
+    patterns.register_sequence()
     fait_pipeline(g, hints)
     return jit_fn
 

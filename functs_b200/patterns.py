@@ -9,6 +9,10 @@ reference's benchmark modules are written (views + in-place slice / select assig
   LSTMSeq      functs/benchmark/ai_model/lstm/lstm.py:79-133
   YolactMasks  functs/benchmark/ai_model/yolact/yolact_mask.py:250-264, 306-333
 
+and, in the same style as the LSTM, of the sequence operator beside it:
+
+  DecayAttentionSeq  per head a state that decays and takes in k[t] v[t]^T; outs[t] = q[t]^T state
+
 ``register_all()`` scripts every pattern, runs it through the same functionalization as a user's program
 (``_C._jit_pass_prepare_for_matching``) and registers its canonical signature with the kernel adapter that executes it.
 A user's program whose functionalized graph contains a region with the same signature — same operations, same structural
@@ -236,6 +240,27 @@ class LSTMSeq(torch.nn.Module):
         return hs, cs
 
 
+# ---- attention with a decaying state -----------------------------------------------------------------------------------
+
+
+class DecayAttentionSeq(torch.nn.Module):
+    """forward(q [T,B,H,Dk], k [T,B,H,Dk], v [T,B,H,Dv]) -> (outs [T,B,H,Dv], last state [B,H,Dk,Dv]); decay [H,1,1] in [0, 1]."""
+
+    def __init__(self, decay: Tensor):
+        super().__init__()
+        self.decay = decay
+
+    def forward(self, q: Tensor, k: Tensor, v: Tensor) -> Tuple[Tensor, Tensor]:
+        seq_len, batch, heads, dk = q.shape
+        dv = v.size(3)
+        outs = torch.zeros(seq_len, batch, heads, dv, dtype=q.dtype, device=q.device)
+        s = torch.zeros(batch, heads, dk, dv, dtype=q.dtype, device=q.device)
+        for t in range(seq_len):
+            s = s * self.decay + k[t].unsqueeze(3) * v[t].unsqueeze(2)
+            outs[t] = torch.matmul(q[t].unsqueeze(2), s).squeeze(2)
+        return outs, s
+
+
 # ---- YOLACT ----------------------------------------------------------------------------------------------------------
 
 
@@ -364,3 +389,14 @@ def register_all() -> dict:
         _registered["yolact_masks_logits"] = _register("yolact_masks_logits", YolactMasks(_F["thr"]), ("thr",))
         _registered["yolact_masks"] = _register("yolact_masks", YolactMasksOnly(_F["thr"]), ("thr",))
         return _registered
+
+
+_sequence = {}
+
+
+def register_sequence() -> dict:
+    """The same for the sequence operators' programs."""
+    with _lock:
+        if not _sequence:
+            _sequence["decay_attention_seq"] = _register("decay_attention_seq", DecayAttentionSeq(torch.full((3, 1, 1), 0.5)))
+        return _sequence

@@ -509,3 +509,40 @@ print("same")
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("steps,batch,heads,dk,dv", [(1, 1, 1, 4, 4), (20, 2, 3, 16, 24), (300, 2, 4, 64, 64), (0, 2, 2, 8, 8)])
+def test_decaying_state_program_through_the_graph(ops, steps, batch, heads, dk, dv):
+    """The imperative program, built, against its own loop in 64 bits; time-major tensors, one functor, no interpreted run."""
+    from functs_b200 import jit, launch_count, patterns
+    decay = (1 - torch.exp2(-torch.arange(heads, dtype=F32) - 1)).reshape(heads, 1, 1)
+    decay[0] = 0.0 if heads == 3 else decay[0]
+    program = patterns.DecayAttentionSeq(decay)
+    fn = jit.build(program)
+    assert jit.functor_regions(fn.graph) == ["decay_attention_seq"]
+    q, k, v = (torch.randn(steps, batch, heads, d, device="cuda") for d in (dk, dk, dv))
+    before = jit.interpreted_functor_runs()
+    outs, s = fn(q, k, v)
+    launches = launch_count()
+    outs, s = fn(q, k, v)
+    assert jit.interpreted_functor_runs() == before and launch_count() - launches <= 3
+    want, want_s = patterns.DecayAttentionSeq(decay.double())(*(x.double().cpu() for x in (q, k, v)))
+    mag, mag_s = patterns.DecayAttentionSeq(decay.double())(*(x.double().cpu().abs() for x in (q, k, v)))
+    # (as above; the decay goes through its logarithm, which costs it another 2^-24 per token)
+    tol = (5 * steps + dk + 8) * 2.0 ** -24
+    assert outs.shape == want.shape and bool(((outs.cpu().double() - want).abs() <= tol * mag).all())
+    assert bool(((s.cpu().double() - want_s).abs() <= tol * mag_s).all())
+
+
+def test_decaying_state_program_that_does_not_fit_the_kernels(ops):
+    """Other types, wide heads and decays above one run as before there was a kernel: step by step."""
+    from functs_b200 import jit, patterns
+    for decay, dtype, d in ((0.5, torch.float64, 16), (0.5, F32, 144), (1.5, F32, 16)):
+        decay = torch.full((2, 1, 1), decay, device="cuda", dtype=dtype if dtype == torch.float64 else F32)
+        fn = jit.build(patterns.DecayAttentionSeq(decay))
+        q, k, v = (torch.randn(5, 1, 2, d, device="cuda", dtype=dtype) for _ in range(3))
+        before = jit.interpreted_functor_runs()
+        outs, s = fn(q, k, v)
+        assert jit.interpreted_functor_runs() > before
+        want, want_s = patterns.DecayAttentionSeq(decay)(q, k, v)
+        assert torch.allclose(outs, want) and torch.allclose(s, want_s)

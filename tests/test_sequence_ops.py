@@ -63,3 +63,33 @@ def test_there_is_no_cpu_path():
         ops.linear_attention_step(x[0], x[0], x[0], torch.zeros(3), torch.zeros(2, 3, 4, 4))
     with pytest.raises(ValueError, match="CUDA"):
         ops.token_logprobs(torch.zeros(2, 3), torch.zeros(2, dtype=torch.int64))
+
+
+def test_decaying_state_program_reaches_its_kernel():
+    """The imperative loop (a state that decays, outputs assigned by step) is one functor bound to the attention kernels."""
+    from functs_b200 import jit, patterns
+    f = jit.build(patterns.DecayAttentionSeq(torch.rand(4, 1, 1)))
+    assert jit.functor_regions(f.graph) == ["decay_attention_seq"]
+    assert "prim::Loop" not in {n.kind() for n in f.graph.nodes()}
+
+
+class OtherUpdate(torch.nn.Module):
+    """The same loop with the state's halves added the other way round: another program."""
+
+    def __init__(self, decay: torch.Tensor):
+        super().__init__()
+        self.decay = decay
+
+    def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
+        outs = torch.zeros(q.size(0), q.size(1), q.size(2), v.size(3), dtype=q.dtype, device=q.device)
+        s = torch.zeros(q.size(1), q.size(2), q.size(3), v.size(3), dtype=q.dtype, device=q.device)
+        for t in range(q.size(0)):
+            s = s * self.decay - k[t].unsqueeze(3) * v[t].unsqueeze(2)
+            outs[t] = torch.matmul(q[t].unsqueeze(2), s).squeeze(2)
+        return outs, s
+
+
+def test_another_update_does_not_match():
+    from functs_b200 import jit
+    f = jit.build(OtherUpdate(torch.rand(4, 1, 1)))
+    assert "decay_attention_seq" not in jit.functor_regions(f.graph)
