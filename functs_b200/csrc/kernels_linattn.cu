@@ -9,7 +9,7 @@
 namespace fb {
 
 constexpr int kRecurThreads = 256;
-constexpr int kRecurTokens = 8;  // tokens staged at a time
+constexpr int kRecurTokens = 16;  // tokens staged at a time
 
 // A CTA owns COLS = 4 * CG columns of one state: thread -> (column group tid % CG, rows tid / CG + i * RG), so a warp reads whole
 // sectors of 32 / CG rows, and every thread keeps its part of S in registers over all tokens.
@@ -57,8 +57,13 @@ __global__ void __launch_bounds__(kRecurThreads) linattn_recurrent_kernel(const 
     const T* v = static_cast<const T*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2] + col0;
     T* out = static_cast<T*>(a.out) + b * a.out_stride[0] + h * a.out_stride[2] + col0;
     // rows that nothing reads stay zero
-    for (int i = tid; i < kRecurTokens * kLinMaxDim; i += kRecurThreads) (&s_q[0][0])[i] = (&s_k[0][0])[i] = 0.0f;
-    for (int i = tid; i < kRecurTokens * COLS; i += kRecurThreads) (&s_v[0][0])[i] = 0.0f;
+    const int staged = min(kRecurTokens, length);
+    if (a.dk < kLinMaxDim) {
+        for (int i = tid; i < staged * kLinMaxDim; i += kRecurThreads) (&s_q[0][0])[i] = (&s_k[0][0])[i] = 0.0f;
+    }
+    if (cols < COLS) {
+        for (int i = tid; i < staged * COLS; i += kRecurThreads) (&s_v[0][0])[i] = 0.0f;
+    }
     __syncthreads();
     for (int t0 = 0; t0 < length; t0 += kRecurTokens) {
         const int n = min(kRecurTokens, length - t0);
@@ -72,7 +77,8 @@ __global__ void __launch_bounds__(kRecurThreads) linattn_recurrent_kernel(const 
             s_v[t][d] = lin_float(v[(t0 + t) * a.v_stride[1] + d]);
         }
         __syncthreads();
-        for (int t = 0; t < n; ++t) {
+#pragma unroll 4
+        for (int t = 0; t < n; ++t) {  // (tokens overlap: only S ties one to the next)
             const float4 vv = *reinterpret_cast<const float4*>(&s_v[t][cg * 4]);
             float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
