@@ -11,6 +11,8 @@ namespace fb {
 constexpr int kRecurThreads = 256;
 constexpr int kRecurTokens = 16;  // tokens staged at a time
 
+// One token of 16 states of 128 x 128 3.6 us, of 1536 41 (4.9 TB/s), of 8192 187 (5.75 TB/s).
+//
 // A CTA owns COLS = 4 * CG columns of one state: thread -> (column group tid % CG, rows tid / CG + i * RG), so a warp reads whole
 // sectors of 32 / CG rows, and every thread keeps its part of S in registers over all tokens.
 template <typename T, int CG, bool VEC>
@@ -190,7 +192,7 @@ __global__ void __launch_bounds__(kStepThreads) linattn_step_kernel(const LinArg
 
 // Whether a prompt goes chunk by chunk (kernels_linattn_tc.cu) or token by token.  A chunk takes 11.6 us per wave of heads however few tokens it
 // has.  Token by token it is 3.5 us and 0.3 per token while the column tiles are on an SM each, 0.25 per token and tile of an SM beyond
-// that: 8 heads of 64, 24 tokens 10.8 (11.6 as a chunk); 128 heads of 128, 8 tokens 11.0 (11.7), 24 tokens 24.8; 1024 heads, 8 tokens 73 (83).
+// that: 8 heads of 64, 24 tokens 9.3 (12.0 as a chunk); 128 heads of 128, 8 tokens 11.4 (11.9), 24 tokens 24.8; 1024 heads, 8 tokens 71 (83).
 static bool lin_by_chunks(const LinArgs& a) {
     const int64_t heads = static_cast<int64_t>(a.batch) * a.heads, tiles = heads * ((a.dv + 31) / 32);
     const double chunk = 11.6 * static_cast<double>((heads + kNumSMs - 1) / kNumSMs);

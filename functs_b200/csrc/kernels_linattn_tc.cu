@@ -3,12 +3,12 @@
 // Within a chunk whose first token follows the state S (l = decay, i and j count from 0, n = its tokens):
 //   out_i = scale * ( l^(i+1) S^T q_i  +  sum_{j <= i} l^(i-j) (q_i . k_j) v_j )          S' = l^n S + sum_j l^(n-1-j) k_j v_j^T
 // which is four products:  G = Q K^T,  X = S^T Q^T,  Y = V^T P^T with P = G masked and decayed,  U = K^T W with W = decayed V.
-// S is decayed and added to in fp32 outside the tensor core (which truncates when it adds); the decay is a sum of two floats, because
-// its rounding would be the same for every chunk.
+// S is decayed and added to in fp32 outside the tensor core (which truncates when it adds).
 //
-// Operands have 8 bits, so what has more is a sum of parts: S and P of two (what they make is rounded to 16 bits at once, 2^-16 apart),
-// W of three (it makes the state, which is fp32).  Q, K and V are their own part in bf16, two in fp16 (exact), three in fp32; products of
-// parts that are below the result's precision are left out, and the small ones are added first.
+// Operands have 8 bits, so what has more is a sum of parts: S and P of two (what they make is rounded to 16 bits at once, 2^-16 apart;
+// three where the outputs are fp32), W of three (it makes the state, which is fp32: with two it was 3e-6 off, now 2e-7).  Q, K and V are
+// their own part in bf16, two in fp16 (exact), three in fp32; products of parts that are below the result's precision are left out, and the
+// small ones are added first.
 //
 // X, Y and U are formed transposed, with the channels of V as rows, so that S^T is an operand in TMEM (in shared memory it cost 128 KB of
 // writes and reads per chunk, and shared memory's bandwidth was the bound), and stores of S and of the outputs are coalesced.  All products
@@ -23,6 +23,15 @@
 //   P   P from G: four warps (there are 64 rows)
 //   beside these, one warp issues U and G, one X and Y, so that the tensor core has work while either waits, and one issues the copies.
 // G of the next chunk is formed in U's columns as soon as they have been read, so P is ready long before its product's turn.
+//
+// What bounds it: 128 x 128 heads in bf16 take 2.8 us per chunk and SM, where HBM would let 64 tokens pass in 1.5.  The chunk's 44 products
+// take 2100 cycles alone and about 3000 beside the other warps, whose reads and writes of shared memory they share; the 14 000 instructions
+// of a chunk issue at 2.9 per cycle, so issue is the bound, not one role's chain.  16 x 2048 tokens of 16 heads 190 us (2.85 TB/s),
+// 8192 tokens of 16 heads 97, 16 uneven prompts of up to 2048 tokens 121.  In fp16 and fp32 the threads split every tile into parts:
+// 4 to 5 us per chunk of 64 x 64 heads, 10 of 128 x 128, which shared memory holds once.
+// Tried and slower: G in columns of its own behind X, so that it does not wait for U to be read (2.95 and 3.3 us per chunk against 2.75);
+// S read eight columns at a time with the next eight on their way (2.82); the roles' loops unrolled (4.5: instruction cache); one lane of a
+// warp waiting for all (6.5); all of a chunk's phases by all warps between block barriers (6.8).
 //
 // NaN and infinities: a masked entry of P is 0 by selection, but 0 * V is not 0 for a V that is not finite, so such entries are taken as 0 in
 // Y (not in W) and the outputs of their channel, from their token on, are set to NaN.

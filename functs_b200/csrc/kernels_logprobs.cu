@@ -5,13 +5,16 @@
 // Every thread takes the maximum of its first elements as its reference and changes it only where an element lies 2^80 above it, so that
 // the loop is a fused multiply-add, an exponential and two sums per element; partial sums meet at the row's maximum at the end.
 //
-// Alternatives: each thread also keeps the maximum of its elements.  The top-th largest of those maxima bounds the top-th largest element
-// from below, so only the few threads whose maximum reaches it have candidates: their elements are read again (from L2), what reaches
-// the bound is ordered by rank counting.  Elements equal to the bound are listed too, or, where there are many (a masked row with few
+// Alternatives: each thread also keeps the maximum of its elements.  The top-th largest of some of those maxima (the largest of every warp)
+// bounds the top-th largest element from below, so only the few threads whose maximum reaches it have candidates: their elements are read
+// again (from L2), and what reaches the bound is ordered by rank counting.  Elements equal to the bound are listed too, or, where there are many (a masked row with few
 // finite logits, a constant row), taken by one ordered scan that stops as soon as it has enough.  More candidates than the list holds
 // (rows whose large values sit in few threads) select the bound again by radix, exactly.
 //
 // A row is one CTA, or a cluster of up to eight whose parts meet in the first one's shared memory; a short row is a warp.
+//
+// Bound by HBM where rows are many (4096 rows of 32000 in bf16: 54 us, 4.8 TB/s; exponentials and issue take half of the time beside it)
+// and by latency where they are few (one row of 32000 in fp32 4.1 us, with five alternatives 8.2: the choice is eight block barriers).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -485,6 +485,40 @@ def test_prompt_rows_on_other_boundaries(ops, dk, dv, front, dtype):
     check_attention(out, state, recurrence(q, k, v, decays(h), dk ** -0.5, None, torch.full((b,), t, device="cuda")), dtype, t, dk)
 
 
+@pytest.mark.parametrize("dk,dv", [(8, 16), (16, 8), (24, 40), (8, 128)])
+def test_prompt_heads_narrower_than_a_tile(ops, dk, dv):
+    """Boxes that reach past the channels, sequences and heads of the tensor; batches and heads of one."""
+    for b, h in ((1, 1), (2, 3)):
+        q, k, v = make(b, 100, h, h, dk, dv, BF16)
+        out, state = ops.linear_attention(q, k, v, decays(h))
+        check_attention(out, state, recurrence(q, k, v, decays(h), 1.0, None, torch.full((b,), 100, device="cuda")), BF16, 100, dk)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_prompt_of_shared_and_expanded_tensors(ops, dtype):
+    """Keys and values of one sequence for all (stride 0), queries that share memory with them."""
+    b, t, h, d = 3, 130, 2, 64
+    x = torch.randn(1, t, h, d, device="cuda").to(dtype)
+    q = k = v = x.expand(b, t, h, d)
+    out, state = ops.linear_attention(q, k, v, decays(h), scale=0.1)
+    check_attention(out, state, recurrence(q, k, v, decays(h), 0.1, None, torch.full((b,), t, device="cuda")), dtype, t, d)
+    assert torch.equal(out[0], out[2])
+
+
+def test_many_sequences_of_which_few_have_tokens(ops):
+    b, t, h, d = 300, 70, 2, 64
+    q, k, v = make(b, t, h, h, d, d, BF16)
+    lengths = torch.zeros(b, device="cuda", dtype=torch.int32)
+    lengths[[3, 299]] = torch.tensor([70, 5], device="cuda", dtype=torch.int32)
+    out, state = ops.linear_attention(q, k, v, decays(h), lengths=lengths)
+    for i in (3, 299):
+        n = int(lengths[i])
+        want = recurrence(q[i:i + 1], k[i:i + 1], v[i:i + 1], decays(h), 1.0, None, lengths[i:i + 1])
+        check_attention(out[i:i + 1], state[i:i + 1], want, BF16, n, d)
+    others = lengths == 0
+    assert bool((out[others] == 0).all()) and bool((state[others] == 0).all())
+
+
 def test_first_call_in_a_capture(cuda_device):
     """A process whose first prompt is captured into a graph."""
     import subprocess
