@@ -402,14 +402,21 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
             for (int e = 0; e < 16; ++e, at += a.dv)
                 if (k0 + g + e < a.dk) *at = s[e];
         };
+        if (from == nullptr && chunks > 0) {  // (little code: fetched cold, the loop below takes 2 us)
+            const uint32_t zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            const uint32_t columns = lane_base + kLtS + (warp >> 2) * (kLtTmemCols - kLtS) / 2;  // S and its parts are the columns from kLtS on
 #pragma unroll 1
-        for (int g = 0; g < kHalf; g += 16) {
-            float s[16];
+            for (uint32_t g = 0; g < (kLtTmemCols - kLtS) / 2; g += 8) lt_st(columns + g, zero);
+        } else {
+#pragma unroll 1
+            for (int g = 0; g < kHalf; g += 16) {
+                float s[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = from != nullptr && has_row && k0 + g + e < a.dk ? from[static_cast<int64_t>(g + e) * a.dv] : 0.0f;
-            if (chunks == 0) at_end(g, s);
-            if (C::NS == 2) lt_st(lane_base + kLtS + k0 + g, s);
-            keep_parts(g, s);
+                for (int e = 0; e < 16; ++e) s[e] = from != nullptr && has_row && k0 + g + e < a.dk ? from[static_cast<int64_t>(g + e) * a.dv] : 0.0f;
+                if (chunks == 0) at_end(g, s);
+                if (C::NS == 2) lt_st(lane_base + kLtS + k0 + g, s);
+                keep_parts(g, s);
+            }
         }
         lt_st_wait();
         lt_arrive_read(&m.s_full, lane);
