@@ -11,7 +11,7 @@ namespace fb {
 constexpr int kRecurThreads = 256;
 constexpr int kRecurTokens = 16;  // tokens staged at a time
 
-// One token of 16 states of 128 x 128 3.6 us, of 1536 41 (4.9 TB/s), of 8192 187 (5.75 TB/s).
+// One token of 16 states of 128 x 128 3.9 us, of 1536 42 (4.8 TB/s), of 8192 187 (5.75 TB/s).
 //
 // A CTA owns COLS = 4 * CG columns of one state: thread -> (column group tid % CG, rows tid / CG + i * RG), so a warp reads whole
 // sectors of 32 / CG rows, and every thread keeps its part of S in registers over all tokens.
@@ -206,8 +206,9 @@ static int launch_recurrent(const LinArgs& a, cudaStream_t st) {
     const int64_t bh = static_cast<int64_t>(a.batch) * a.heads;
     const int tiles = (a.dv + 31) / 32;
     FB_REQUIRE(bh * tiles < (1ll << 31), "linear_attention: batch * heads is too large");
-    // (from two states per SM on: 96 x 16 states of 128 x 128 52 us in column tiles, 41 in whole ones; 16 states alone 4.3 and 5.1)
-    if (vec && a.tokens == 1 && a.lengths == nullptr && bh >= 2 * kNumSMs) {
+    // Whole states where they are small (48 of 64 x 64 3.2 us, in column tiles 4.1) or fill half of the SMs (128 x 128: 16 states 4.6, in
+    // tiles 3.9; 64 4.8 and 4.7; 112 5.1 and 6.1; 256 7.1 and 9.7; 1536 42 and 53)
+    if (vec && a.tokens == 1 && a.lengths == nullptr && (a.dk * a.dv <= 64 * 64 || bh >= kNumSMs / 2)) {
         const dim3 whole(static_cast<unsigned>(bh)), block(kStepThreads);
         if (a.dv <= 32) return launch_after(linattn_step_kernel<T, 8>, whole, block, 0, st, false, "linear_attention", a);
         if (a.dv <= 64) return launch_after(linattn_step_kernel<T, 16>, whole, block, 0, st, false, "linear_attention", a);

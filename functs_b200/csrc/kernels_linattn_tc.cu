@@ -6,7 +6,7 @@
 // S is decayed and added to in fp32 outside the tensor core (which truncates when it adds).
 //
 // Operands have 8 bits, so what has more is a sum of parts: S and P of two (what they make is rounded to 16 bits at once, 2^-16 apart;
-// three where the outputs are fp32), W of three (it makes the state, which is fp32: with two it was 3e-6 off, now 2e-7).  Q, K and V are
+// three where the outputs are fp32), W of three (it makes the state, which is fp32: two would leave 2^-16 of each term, with three it is 2e-7 off).  Q, K and V are
 // their own part in bf16, two in fp16 (exact), three in fp32; products of parts that are below the result's precision are left out, and the
 // small ones are added first.
 //
@@ -25,8 +25,9 @@
 // G of the next chunk is formed in U's columns as soon as they have been read, so P is ready long before its product's turn.
 //
 // What bounds it: 128 x 128 heads in bf16 take 2.8 us per chunk and SM, where HBM would let 64 tokens pass in 1.5.  The chunk's 44 products
-// take 2100 cycles alone and about 3000 beside the other warps, whose reads and writes of shared memory they share; the 14 000 instructions
-// of a chunk issue at 2.9 per cycle, so issue is the bound, not one role's chain.  16 x 2048 tokens of 16 heads 190 us (2.85 TB/s),
+// alone take 2100 cycles (2700 where a lane is chosen by comparison instead of election), and more beside the other warps, whose reads and
+// writes of shared memory they share; the warps issue about 2.1 instructions per cycle and SM.  No single role is the bound: when a chunk
+// took 4.2 us, leaving out the work of one role saved 3 to 13 %, of four together 34 %.  16 x 2048 tokens of 16 heads 190 us (2.85 TB/s),
 // 8192 tokens of 16 heads 97, 16 uneven prompts of up to 2048 tokens 121.  In fp16 and fp32 the threads split every tile into parts:
 // 4 to 5 us per chunk of 64 x 64 heads, 10 of 128 x 128, which shared memory holds once.
 // Tried and slower: G in columns of its own behind X, so that it does not wait for U to be read (2.95 and 3.3 us per chunk against 2.75);
@@ -889,7 +890,7 @@ __global__ void __launch_bounds__(256) linattn_carry_kernel(const LinArgs a, flo
 
 // How many parts a sequence is cut into.  Cutting costs a second reading of K and V for the states of the parts (about 0.4 of a chunk's time
 // for each of its chunks) and two more launches (9 us; a chunk is 2.8 us in bf16, 6 and more in the other types), so it pays where whole
-// sequences leave SMs without work: 8192 tokens of 16 heads 408 us whole, 119 in nine parts.
+// sequences leave SMs without work: 8192 tokens of 16 heads 408 us whole and 119 in nine parts when both were timed, in parts 97 now.
 static void lt_cut(const LinArgs& a, int64_t rows, int& segs, int& seg_tokens) {
     const int chunks = (a.tokens + kLtChunk - 1) / kLtChunk;
     segs = 1;

@@ -14,7 +14,7 @@
 // A row is one CTA, or a cluster of up to eight whose parts meet in the first one's shared memory; a short row is a warp.
 //
 // Bound by HBM where rows are many (4096 rows of 32000 in bf16: 54 us, 4.8 TB/s; exponentials and issue take half of the time beside it)
-// and by latency where they are few (one row of 32000 in fp32 4.1 us, with five alternatives 8.2: the choice is eight block barriers).
+// and by latency where they are few (one row of 32000 in fp32 4.3 us, with five alternatives 7.1: the choice is eight block barriers).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -25,6 +25,7 @@ namespace fb {
 constexpr int kLpMaxThreads = 512;
 constexpr int kLpMaxTop = FB_LOGPROBS_MAX_TOP;
 constexpr int kLpMaxParts = 8;               // CTAs per row
+constexpr int kLpTopParts = 4;               // the same with alternatives
 constexpr int kLpList = 1024;                // candidates above the bound; as many equal to it
 constexpr int kLpBusy = 128;                 // threads whose elements are looked through one by one
 constexpr float kLpLog2e = 1.44269504088896340736f;
@@ -150,7 +151,7 @@ struct LpShared {
     uint64_t most[TOP ? 2 * kLpMaxTop : 1];   // the largest of the threads' maxima, warp by warp
     uint64_t above[TOP ? kLpList : 1], equal[TOP ? kLpList : 1];  // candidates
     uint64_t best[kLpMaxTop];                 // this CTA's, in order
-    uint64_t parts_best[TOP ? kLpMaxParts * kLpMaxTop : 1];  // of the row's CTAs (in the first one)
+    uint64_t parts_best[TOP ? kLpTopParts * kLpMaxTop : 1];  // of the row's CTAs (in the first one)
     uint64_t row_best[kLpMaxTop];             // the row's
     double log_sum;
     uint32_t hist[256];
@@ -553,11 +554,13 @@ static int launch_logprobs_short(const LpArgs& a, int rows, cudaStream_t st) {
 template <typename T, bool TOP>
 static int launch_logprobs(const LpArgs& a, int rows, cudaStream_t st) {
     const int vecs = a.vocab / LpVec<T>::N;
-    // One CTA per row, and per SM, unless rows are few; a part of 512 vectors at least (one row of 32000 fp32 logits: 8.9 us in eight parts,
-    // 12.6 in one).  With several rows per SM 256 threads a row (4096 rows of 32000: 54 us, with 512 threads 62), else 512 (256 rows of
-    // 131072: 25 and 35).
+    // One CTA per row, unless rows are few and long.  Without alternatives a part of 512 vectors at least (one row of 32000 fp32 logits 4.3 us
+    // in eight parts, 4.5 in four, 5.2 in one).  With alternatives the parts' lists have to meet: four parts from 8192 vectors on (8 rows of
+    // 65536 in bf16 8.9 us in one, 7.6 in four, 7.7 in eight), fewer vectors in one (one row of 32000 in fp32 7.1, in eight 8.2).  With several
+    // rows per SM 256 threads a row (4096 rows of 32000: 54 us, with 512 threads 62), else 512 (256 rows of 131072: 24 and 37).
+    const int most = !TOP ? kLpMaxParts : vecs >= 8192 ? kLpTopParts : 1;
     int parts = 1;
-    while (parts < kLpMaxParts && static_cast<int64_t>(rows) * parts * 2 <= kNumSMs && vecs / (parts * 2) >= 512) parts *= 2;
+    while (parts < most && static_cast<int64_t>(rows) * parts * 2 <= kNumSMs && vecs / (parts * 2) >= 512) parts *= 2;
     const int each = vecs / parts;
     const int threads = each >= 1024 ? (rows >= 4 * kNumSMs ? 256 : 512) : each >= 512 ? 256 : each >= 128 ? 128 : 64;
     cudaLaunchConfig_t cfg = {};

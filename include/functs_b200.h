@@ -261,7 +261,7 @@ int functs_b200_lstm_forward_mode(const float* x, const float* w_ih, const float
  * num_slots = batch.  A negative slot is no sequence: its rows of out are zero, and no state is touched.  So is, with a status bit, one
  * of num_slots or above (FB_STATUS_INDEX_RANGE) and one that an earlier sequence has (FB_STATUS_INDEX_TWICE).
  * lengths (optional, int32 [batch], taken as 0 .. tokens): sequence b ends there; its later rows are not read, and zero in out.
- * status: optional.  One launch for a few tokens, for longer prompts one, or two and three where sequences are cut into parts.
+ * status: optional.  One launch for a few tokens, for longer prompts one, or three where sequences are cut into parts.
  * scratch: functs_b200_linear_attention_scratch_bytes, 16-byte aligned (may be NULL where that is 0). */
 typedef struct {
     int32_t dtype, batch, tokens, heads, kv_heads, dk, dv, num_slots;

@@ -138,6 +138,27 @@ def test_step(ops, shape, dtype):
     assert torch.equal(pool[others], before[others])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", [(73, 1, 1, 128, 128), (74, 1, 1, 128, 128), (1, 1, 1, 128, 32), (1, 2, 1, 128, 36), (3, 2, 2, 33, 124), (2, 3, 1, 3, 4),
+                                   (5, 2, 2, 64, 64), (5, 2, 2, 65, 64)], ids=str)
+def test_step_of_whole_states_and_of_tiles(ops, shape, dtype):
+    """Sizes on either side of those where a block takes a whole state; some slots name no sequence."""
+    b, h, hk, dk, dv = shape
+    q, k, v = (x[:, 0] for x in make(b, 1, h, hk, dk, dv, dtype, "fused"))
+    pool = torch.randn(b + 2, h, dk, dv, device="cuda")
+    slots = torch.randperm(b + 2, device="cuda")[:b].to(torch.int32)
+    slots[1::3] = -1
+    live = slots >= 0
+    before = pool.clone()
+    want = recurrence(q[:, None], k[:, None], v[:, None], decays(h), 0.5, pool[slots.clamp(min=0).long()], torch.ones(b, device="cuda"))
+    out = ops.linear_attention_step(q, k, v, decays(h), pool, scale=0.5, slots=slots)
+    check_attention(out[live][:, None], pool[slots[live].long()], tuple(x[live] for x in want), dtype, 1, dk)
+    assert bool((out[~live] == 0).all())
+    others = torch.ones(b + 2, dtype=torch.bool, device="cuda")
+    others[slots[live].long()] = False
+    assert torch.equal(pool[others], before[others])
+
+
 @pytest.mark.parametrize("tokens", [1, 5, 200])
 def test_slots_that_are_none_out_of_range_or_named_twice(ops, tokens):
     import functs_b200
@@ -363,6 +384,38 @@ def test_logprobs(ops, rows, vocab, top, dtype):
     g = torch.Generator(device="cuda").manual_seed(vocab)
     logits = (torch.randn(rows, vocab, generator=g, device="cuda") * 3).to(dtype)
     check_logprobs(ops, logits, torch.randint(0, vocab, (rows,), generator=g, device="cuda"), top)
+
+
+@pytest.mark.parametrize("top", [0, 1, 64])
+@pytest.mark.parametrize("rows,vecs", [(1, 8191), (1, 8192), (37, 8193), (38, 8192), (74, 8200), (75, 8192), (3, 16385), (148, 600)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_logprobs_of_rows_around_those_that_are_shared(ops, rows, vecs, top, dtype):
+    """Rows as long as those that several blocks share, a little shorter and longer, on every boundary (the row before them is longer)."""
+    vocab = vecs * 16 // dtype.itemsize
+    g = torch.Generator(device="cuda").manual_seed(vecs)
+    for less in (0, 3):
+        x = (torch.randn(rows, vocab + 1, generator=g, device="cuda") * 3).to(dtype)[:, :vocab - less]
+        check_logprobs(ops, x, torch.randint(0, vocab - less, (rows,), generator=g, device="cuda"), top)
+
+
+@pytest.mark.parametrize("kind", ["constant", "one part", "last part", "few finite", "none but one"])
+@pytest.mark.parametrize("rows", [2, 60])
+def test_logprobs_of_shared_rows_that_are_hard_to_select_from(ops, kind, rows):
+    vocab, top = 70003, 64
+    at = torch.arange(vocab, device="cuda")
+    x = torch.randn(rows, vocab, device="cuda")
+    if kind == "constant":
+        x = torch.full((rows, vocab), 1.25, device="cuda")
+    elif kind == "one part":  # all alternatives lie in one of the parts
+        x = torch.where((at > 18000) & (at < 18100), x + 50, x)
+    elif kind == "last part":
+        x = torch.where(at >= vocab - 64, x + 50, x)
+    elif kind == "few finite":  # fewer than asked for, in two parts
+        x[:, 5:vocab - 5] = -math.inf
+    elif kind == "none but one":
+        x = torch.full((rows, vocab), -math.inf, device="cuda")
+        x[:, 69999] = -4.0
+    check_logprobs(ops, x.to(BF16).contiguous(), torch.randint(0, vocab, (rows,), device="cuda"), top)
 
 
 @pytest.mark.parametrize("rows", [2, 300])
