@@ -276,10 +276,14 @@ __device__ __forceinline__ bool lt_finite(float x) { return fabsf(x) <= 3.402823
 
 // ---- the kernel -----------------------------------------------------------------------------------------------------
 
-template <typename T, int DK, int DV, bool TMA>
+// LOADS: how the rows are read.  By TMA; by loads of 16 bytes; or by those that plan.boundary allows (a kernel of its own: their code beside
+// the others' costs: 16 x 2048 tokens of 16 heads of 64 in fp32 297 us, with it 317).
+enum LtLoads { kLtTma, kLtWide, kLtAny };
+template <typename T, int DK, int DV, LtLoads LOADS>
 __global__ void __launch_bounds__(LtCfg<T, DK, DV>::kThreads, 1)
 linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                      const __grid_constant__ CUtensorMap map_v) {
+    constexpr bool TMA = LOADS == kLtTma;
     using C = LtCfg<T, DK, DV>;
     constexpr int kWarpsW = C::kWarpsW;
     extern __shared__ __align__(1024) unsigned char smem[];
@@ -528,8 +532,8 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
                     for (int j = 0; j < 2; ++j) {
                         const int i = id + (i0 + j) * threads, g = i % (DK / 8), t = i / (DK / 8);
                         const int valid = t < n ? max(0, min(8, a.dk - g * 8)) : 0;
-                        lt_load8(k + (t0 + t) * a.k_stride[1] + g * 8, valid, plan.boundary, y[j]);
-                        if (outputs) lt_load8(q + (t0 + t) * a.q_stride[1] + g * 8, valid, plan.boundary, x[j]);
+                        lt_load8(k + (t0 + t) * a.k_stride[1] + g * 8, valid, LOADS == kLtWide ? 16 : plan.boundary, y[j]);
+                        if (outputs) lt_load8(q + (t0 + t) * a.q_stride[1] + g * 8, valid, LOADS == kLtWide ? 16 : plan.boundary, x[j]);
                     }
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
@@ -585,7 +589,7 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         const int g = (g0 + j) * 4 + (lane >> 3);
-                        lt_load8(v + (t0 + t) * a.v_stride[1] + g * 8, t < n ? max(0, min(8, dv - g * 8)) : 0, plan.boundary, x[j]);
+                        lt_load8(v + (t0 + t) * a.v_stride[1] + g * 8, t < n ? max(0, min(8, dv - g * 8)) : 0, LOADS == kLtWide ? 16 : plan.boundary, x[j]);
                     }
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
@@ -888,20 +892,24 @@ __global__ void __launch_bounds__(256) linattn_carry_kernel(const LinArgs a, flo
     a.state_out[own] = s;
 }
 
-// How many parts a sequence is cut into.  Cutting costs a second reading of K and V for the states of the parts (about 0.4 of a chunk's time
-// for each of its chunks) and two more launches (9 us; a chunk is 2.8 us in bf16, 6 and more in the other types), so it pays where whole
-// sequences leave SMs without work: 8192 tokens of 16 heads 408 us whole and 119 in nine parts when both were timed, in parts 97 now.
+// How many parts a sequence is cut into, by the time that it would take (in us; fitted to 66 sizes with 1 to 32 parts, and within a tenth of the
+// best of those).  Cutting costs a second reading of K and V, a start of both kernels for every wave of parts, and the states in between; it
+// pays where whole sequences leave SMs without work.  128 x 128 heads in bf16: 8192 tokens of 16 heads 354 whole and 92 in nine parts, 1024
+// tokens 46 and 33 in eight; but 8 x 1024 tokens of 8 heads 50 and 65 in two, 3 x 640 tokens of 16 heads 33 and 54 in three.
 static void lt_cut(const LinArgs& a, int64_t rows, int& segs, int& seg_tokens) {
     const int chunks = (a.tokens + kLtChunk - 1) / kLtChunk;
     segs = 1;
     seg_tokens = 0;
     if (rows > 65535) return;
-    const double launches = a.dtype == FB_DTYPE_BF16 ? 3.2 : 1.5;
-    double best = static_cast<double>((rows + kNumSMs - 1) / kNumSMs) * chunks;
-    for (int n = 2; n <= 64 && n * 2 <= chunks; ++n) {
+    const bool bf16 = a.dtype == FB_DTYPE_BF16;
+    const double chunk = bf16 ? 2.6 : a.dk <= 64 && a.dv <= 64 ? 4.2 : 10.0, again = chunk * (bf16 ? 1.4 : 1.65);
+    const double start = 12.0 + 6.0 * a.dk * a.dv / (kLinMaxDim * kLinMaxDim);
+    const auto waves = [](int64_t ctas) { return ctas <= kNumSMs ? 1.0 : 1.1 * static_cast<double>((ctas + kNumSMs - 1) / kNumSMs); };
+    double best = waves(rows) * (chunks * chunk + 5.0);
+    for (int n = 2; n <= 64 && n <= chunks; ++n) {
         const int each = (chunks + n - 1) / n;
         const int parts = (chunks + each - 1) / each;
-        const double cost = static_cast<double>((rows * parts + kNumSMs - 1) / kNumSMs) * (each * 1.4 + 1.0) + launches;
+        const double cost = waves(rows * parts) * (each * again + start) + 6.0;
         if (cost < best) {
             best = cost;
             segs = parts;
@@ -963,9 +971,11 @@ static int launch_chunk(const LinArgs& a, void* scratch, cudaStream_t st) {
                lt_encode(&maps[2], a.v, a.v_stride, a.dv, a.tokens, a.kv_heads, a.batch);
     const dim3 grid(static_cast<unsigned>(ctas));
     if constexpr (C::kBf16) {
-        if (tma) return launch_chunk<linattn_chunk_kernel<T, DK, DV, true>>(grid, C::kThreads, bytes, st, a, plan, maps);
+        if (tma) return launch_chunk<linattn_chunk_kernel<T, DK, DV, kLtTma>>(grid, C::kThreads, bytes, st, a, plan, maps);
+    } else {
+        if (plan.boundary == 16) return launch_chunk<linattn_chunk_kernel<T, DK, DV, kLtWide>>(grid, C::kThreads, bytes, st, a, plan, maps);
     }
-    return launch_chunk<linattn_chunk_kernel<T, DK, DV, false>>(grid, C::kThreads, bytes, st, a, plan, maps);
+    return launch_chunk<linattn_chunk_kernel<T, DK, DV, kLtAny>>(grid, C::kThreads, bytes, st, a, plan, maps);
 }
 
 template <typename T>

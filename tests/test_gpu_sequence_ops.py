@@ -123,6 +123,26 @@ def test_prompt_lengths_pool_and_layouts(ops, shape, layout, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("shape", [(1, 512, 16, 8, 64, 64), (1, 513, 16, 16, 128, 128), (2, 256, 4, 4, 128, 128), (3, 320, 5, 5, 100, 36), (1, 1024, 16, 2, 64, 128)],
+                         ids=str)
+def test_prompts_in_parts_of_one_or_two_chunks(ops, shape, dtype):
+    """Long prompts of few heads are cut into parts, some of one chunk: lengths that end in one, at its end, and before most of them."""
+    b, t, h, hk, dk, dv = shape
+    q, k, v = make(*shape, dtype)
+    for first in (t, 64, 65, 1, t - 1):
+        lengths = torch.tensor([first, 0, 200][:b], device="cuda", dtype=torch.int32)
+        pool = torch.randn(b + 1, h, dk, dv, device="cuda")
+        slots = torch.arange(b, 0, -1, device="cuda", dtype=torch.int32)
+        want = recurrence(q, k, v, decays(h), 0.2, pool[slots.long()].clone(), lengths)
+        before = pool[0].clone()
+        out, _ = ops.linear_attention(q, k, v, decays(h), scale=0.2, state=pool, slots=slots, lengths=lengths)
+        check_attention(out, pool[slots.long()], want, dtype, t, dk)
+        assert torch.equal(pool[0], before)
+        for i in range(b):
+            assert bool((out[i, int(lengths[i]):] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("shape", [(1, 1, 1, 1, 1), (1, 16, 16, 128, 128), (33, 12, 4, 72, 40), (7, 4, 2, 128, 17), (70, 8, 8, 64, 64)], ids=str)
 def test_step(ops, shape, dtype):
     b, h, hk, dk, dv = shape
