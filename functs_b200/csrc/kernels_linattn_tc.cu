@@ -26,9 +26,9 @@
 //
 // What bounds it: 128 x 128 heads in bf16 take 2.8 us per chunk and SM, where HBM would let 64 tokens pass in 1.5.  The chunk's 44 products
 // alone take 2100 cycles (2700 where a lane is chosen by comparison instead of election), and more beside the other warps, whose reads and
-// writes of shared memory they share; the warps issue about 2.1 instructions per cycle and SM.  No single role is the bound: when a chunk
-// took 4.2 us, leaving out the work of one role saved 3 to 13 %, of four together 34 %.  16 x 2048 tokens of 16 heads 190 us (2.85 TB/s),
-// 8192 tokens of 16 heads 97, 16 uneven prompts of up to 2048 tokens 121.  In fp16 and fp32 the threads split every tile into parts:
+// writes of shared memory they share; the warps' 13 600 instructions of a chunk issue at 2.4 of 4 per cycle.  No single role or pipe is the
+// bound: when a chunk took 4.2 us, leaving out the work of one role saved 3 to 13 %, of four together 34 %.  16 x 2048 tokens of 16 heads 187 us (2.9 TB/s),
+// 8192 tokens of 16 heads 97, 16 uneven prompts of up to 2048 tokens 117.  In fp16 and fp32 the threads split every tile into parts:
 // 4 to 5 us per chunk of 64 x 64 heads, 10 of 128 x 128, which shared memory holds once.
 // Tried and slower: G in columns of its own behind X, so that it does not wait for U to be read (2.95 and 3.3 us per chunk against 2.75);
 // S read eight columns at a time with the next eight on their way (2.82); the roles' loops unrolled (4.5: instruction cache); one lane of a
