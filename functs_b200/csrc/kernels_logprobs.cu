@@ -29,7 +29,8 @@ constexpr int kLpTopParts = 4;               // the same with alternatives
 constexpr int kLpList = 1024;                // candidates above the bound; as many equal to it
 constexpr int kLpBusy = 128;                 // threads whose elements are looked through one by one
 constexpr float kLpLog2e = 1.44269504088896340736f;
-constexpr float kLpFloor = -1e30f;           // reference of threads that saw nothing finite
+constexpr float kLpFloor = -5e8f;            // the lowest reference: what lies more below it than a power can say counts as nothing there
+constexpr float kLpFarValue = 268435456.0f;  // 2^28: where x log2e is rounded by 16 and more, see lp_again
 constexpr float kLpFar = 80.0f;              // how far above its reference, in powers of two, a thread's sums may grow
 
 struct LpArgs {
@@ -117,6 +118,32 @@ __device__ __forceinline__ void lp_join(LpSums& a, const LpSums& o) {
     a.most = max_nan(a.most, o.most);
 }
 
+// Whether sums against a rounded x log2e do not do for this largest element (finite, and far from 0).
+__device__ __forceinline__ bool lp_far(float most) { return fabsf(most) >= kLpFarValue && fabsf(most) <= 3.402823466e38f; }
+// what `ref` stands for, in powers of two; far from 0 sums are taken against the largest element itself (both factors exact in 64 bits)
+__device__ __forceinline__ double lp_ref(const LpSums& sums) {
+    return lp_far(sums.most) ? static_cast<double>(sums.most) * static_cast<double>(kLpLog2e) : static_cast<double>(sums.ref);
+}
+// elements against the largest one, by a difference that is exact where it matters
+template <int N>
+__device__ __forceinline__ void lp_take_near(const float (&x)[N], float most, float& s, float& t) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float d = fmaxf((x[i] - most) * kLpLog2e, -1000.0f), e = lp_ex2(d);
+        s += e;
+        t = fmaf(e, d, t);
+    }
+}
+
+// a row: log sum exp = base + log_s
+struct LpRow {
+    double base, log_s;
+    bool empty;
+    __device__ __forceinline__ float logprob(float x) const {
+        return empty ? __int_as_float(0xff800000) : static_cast<float>((static_cast<double>(x) - base) - log_s);
+    }
+};
+
 struct LpThread {
     LpSums sums;
 
@@ -153,13 +180,12 @@ struct LpShared {
     uint64_t best[kLpMaxTop];                 // this CTA's, in order
     uint64_t parts_best[TOP ? kLpTopParts * kLpMaxTop : 1];  // of the row's CTAs (in the first one)
     uint64_t row_best[kLpMaxTop];             // the row's
-    double log_sum;
+    LpRow whole;
     uint32_t hist[256];
     uint32_t warp_count[kLpMaxThreads / 32];
     int busy[kLpBusy];                        // threads that have candidates
     int num_threads, num_above, num_equal;
     uint32_t bound, digit, wanted;
-    bool empty;
 };
 
 __device__ __forceinline__ uint32_t lp_cluster_rank() {
@@ -179,21 +205,41 @@ __device__ __forceinline__ void lp_put(uint32_t at, float x, float y, float z, f
 }
 __device__ __forceinline__ void lp_put(uint32_t at, uint64_t v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory"); }
 
-// Writes a row's two numbers; returns log sum exp.
-__device__ __forceinline__ double lp_finish(const LpArgs& a, int64_t r, const LpSums& sums, int64_t token, float token_logit, bool& empty) {
+// Writes a row's two numbers, from sums against `ref` (in powers of two).
+__device__ __forceinline__ LpRow lp_finish(const LpArgs& a, int64_t r, const LpSums& sums, double ref, int64_t token, float token_logit) {
+    LpRow row;
     // (the exponents were x log2e with log2e in 32 bits: the reference goes back by the same number)
-    const double ref = static_cast<double>(sums.ref) / static_cast<double>(kLpLog2e);
-    const double log_s = log(static_cast<double>(sums.s)), log_sum = ref + log_s;
-    empty = sums.most == __int_as_float(0xff800000);
-    float lp = empty ? __int_as_float(0xff800000) : static_cast<float>(static_cast<double>(token_logit) - log_sum);
+    row.base = lp_far(sums.most) ? static_cast<double>(sums.most) : ref / static_cast<double>(kLpLog2e);
+    row.log_s = log(static_cast<double>(sums.s));
+    row.empty = sums.most == __int_as_float(0xff800000);
+    float lp = row.logprob(token_logit);
     if (token < 0) lp = 0.0f;
     if (token >= a.vocab) {
         lp = __int_as_float(0x7fffffff);
         if (a.status != nullptr) atomicOr(a.status, FB_STATUS_INDEX_RANGE);
     }
     a.logprobs[r] = lp;
-    a.entropy[r] = empty ? 0.0f : static_cast<float>(log_s - static_cast<double>(sums.t) / (static_cast<double>(sums.s) * static_cast<double>(kLpLog2e)));
-    return log_sum;
+    a.entropy[r] = row.empty ? 0.0f : static_cast<float>(row.log_s - static_cast<double>(sums.t) / (static_cast<double>(sums.s) * static_cast<double>(kLpLog2e)));
+    return row;
+}
+
+// The sums of a row's parts (one in each of `count` lanes), in all lanes; returns their reference.
+__device__ __forceinline__ double lp_join_parts(LpSums& sums, int count) {
+    const double own = sums.s == 0.0f ? -1e300 : lp_ref(sums);
+    double ref = own;
+    for (int d = count / 2; d > 0; d /= 2) {
+        ref = fmax(ref, __shfl_xor_sync(kFullMask, ref, d));
+        sums.most = max_nan(sums.most, __shfl_xor_sync(kFullMask, sums.most, d));
+    }
+    if (lp_far(sums.most)) ref = static_cast<double>(sums.most) * static_cast<double>(kLpLog2e);
+    const float below = static_cast<float>(fmax(own - ref, -1000.0)), f = lp_ex2(below);
+    sums.t = f * fmaf(below, sums.s, sums.t);
+    sums.s = f * sums.s;
+    for (int d = count / 2; d > 0; d /= 2) {
+        sums.s += __shfl_xor_sync(kFullMask, sums.s, d);
+        sums.t += __shfl_xor_sync(kFullMask, sums.t, d);
+    }
+    return ref;
 }
 
 // The elements of a part of a row: vectors, and single ones in front of (first part) and behind (last part) the row's 16-byte boundaries.
@@ -247,6 +293,32 @@ __device__ __forceinline__ void lp_each(const LpPart<T>& p, F f) {
     }
     if (who < p.head) f(p.order(who), who);
     if (who < p.tail) f(p.order(p.tail_id + who), p.tail_id + who);
+}
+
+// A part whose largest element is 2^28 or more from 0, once more: there x log2e is rounded by so much that powers of the remainder overflow
+// (and -inf, where a mask is the type's lowest value).  Nothing else comes here: masked elements below a row of usual ones count as nothing.
+template <typename T, bool TOP>
+__device__ __noinline__ void lp_again(LpShared<TOP>& sh, const LpPart<T>& p) {
+    constexpr int N = LpVec<T>::N;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
+    float most = sh.sums[0].most;
+    for (int w = 1; w < warps; ++w) most = max_nan(most, sh.sums[w].most);
+    if (!lp_far(most)) return;
+    __syncthreads();
+    float s = 0.0f, t = 0.0f;
+    for (int v = tid; v < p.num_vec; v += threads) {
+        float x[N];
+        LpVec<T>::get(p.vec(v), x);
+        lp_take_near(x, most, s, t);
+    }
+    if (tid < p.head) lp_take_near({LpVec<T>::one(p.row + tid)}, most, s, t);
+    if (tid < p.tail) lp_take_near({LpVec<T>::one(p.row + p.tail_id + tid)}, most, s, t);
+    for (int d = 16; d > 0; d /= 2) {
+        s += __shfl_xor_sync(kFullMask, s, d);
+        t += __shfl_xor_sync(kFullMask, t, d);
+    }
+    if (lane == 0) sh.sums[warp] = {most, 0.0f, s, t};  // (one reference for all)
+    __syncthreads();
 }
 
 // The `top` best of the part (keys 0 behind them if it has fewer), best first, in sh.best.  most: of this thread's elements.
@@ -445,13 +517,14 @@ __global__ void __launch_bounds__(kLpMaxThreads) logprobs_kernel(const LpArgs a,
     // the block's sums
     lp_join_lanes(th.sums, 32);
     if (lane == 0) sh.sums[warp] = th.sums;
-    __syncthreads();
+    if (__syncthreads_or(lane == 0 && lp_far(th.sums.most))) lp_again<T, TOP>(sh, p);
     LpSums sums = {__int_as_float(0xff800000), kLpFloor, 0.0f, 0.0f};
     if (warp == 0) {
         if (lane < warps) sums = sh.sums[lane];
         lp_join_lanes(sums, 16);
     }
     if constexpr (TOP) lp_select<T>(sh, p, a.top, most);
+    double ref = 0.0;
     if (parts > 1) {
         // what the parts have meets in the first one's shared memory
         lp_cluster_wait();  // (it runs)
@@ -462,12 +535,12 @@ __global__ void __launch_bounds__(kLpMaxThreads) logprobs_kernel(const LpArgs a,
         if (rank != 0) return;
         if (warp == 0) {
             sums = sh.part[lane & (parts - 1)];
-            lp_join_lanes(sums, parts);
+            ref = lp_join_parts(sums, parts);
         }
+    } else {
+        ref = lp_ref(sums);
     }
-    if (tid == 0) {
-        sh.log_sum = lp_finish(a, r, sums, token, token_logit, sh.empty);
-    }
+    if (tid == 0) sh.whole = lp_finish(a, r, sums, ref, token, token_logit);
     if (TOP) {
         const uint64_t* best = sh.best;
         if (parts > 1) {
@@ -484,8 +557,7 @@ __global__ void __launch_bounds__(kLpMaxThreads) logprobs_kernel(const LpArgs a,
         __syncthreads();
         for (int i = tid; i < a.top; i += threads) {
             const uint64_t key = best[i];
-            const float x = lp_value(static_cast<uint32_t>(key >> 32));
-            a.top_logprobs[r * a.top + i] = sh.empty ? __int_as_float(0xff800000) : static_cast<float>(static_cast<double>(x) - sh.log_sum);
+            a.top_logprobs[r * a.top + i] = sh.whole.logprob(lp_value(static_cast<uint32_t>(key >> 32)));
             a.top_ids[r * a.top + i] = static_cast<int64_t>(0xFFFFFFFFu - static_cast<uint32_t>(key));
         }
     }
@@ -508,12 +580,17 @@ __global__ void __launch_bounds__(32 * kLpShortRows) logprobs_short_kernel(const
     th.start();
     th.take(x);
     lp_join_lanes(th.sums, 32);
-    double log_sum = 0.0;
-    bool empty = false;
-    if (lane == 0) log_sum = lp_finish(a, r, th.sums, token, token_logit, empty);
-    if (a.top == 0) return;
-    log_sum = __shfl_sync(kFullMask, log_sum, 0);
-    empty = __shfl_sync(kFullMask, empty ? 1 : 0, 0) != 0;
+    if (lp_far(th.sums.most)) {  // (see lp_again)
+        float s = 0.0f, t = 0.0f;
+        lp_take_near(x, th.sums.most, s, t);
+        for (int d = 16; d > 0; d /= 2) {
+            s += __shfl_xor_sync(kFullMask, s, d);
+            t += __shfl_xor_sync(kFullMask, t, d);
+        }
+        th.sums.s = s, th.sums.t = t;
+    }
+    LpRow whole = {};
+    if (lane == 0) whole = lp_finish(a, r, th.sums, lp_ref(th.sums), token, token_logit);
     uint32_t order[COUNT], most = 0;
 #pragma unroll
     for (int i = 0; i < COUNT; ++i) {
@@ -538,7 +615,7 @@ __global__ void __launch_bounds__(32 * kLpShortRows) logprobs_short_kernel(const
             }
         }
         if (lane == 0) {
-            a.top_logprobs[r * a.top + k] = empty ? __int_as_float(0xff800000) : static_cast<float>(static_cast<double>(lp_value(best)) - log_sum);
+            a.top_logprobs[r * a.top + k] = whole.logprob(lp_value(best));
             a.top_ids[r * a.top + k] = id;
         }
     }

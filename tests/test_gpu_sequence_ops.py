@@ -484,6 +484,40 @@ def test_logprobs_of_rows_without_a_distribution(ops, vocab):
     check_logprobs(ops, x[4:], tokens[4:], 4)
 
 
+@pytest.mark.parametrize("vocab,rows", [(50, 9), (1000, 40), (9001, 3), (70001, 2), (140000, 60)])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("kind", ["all lowest", "few left", "one left at the lowest", "two masks", "masked and -inf", "highest", "steps"])
+def test_logprobs_of_logits_masked_with_large_values(ops, kind, dtype, vocab, rows):
+    """Masks of the type's lowest value and of other large ones: rows that they leave something of, and nothing; and the same far above 0."""
+    lowest, highest = torch.finfo(dtype).min, torch.finfo(dtype).max
+    for value in (-1e9, -1e10, -3.3e20, -1e30, lowest):
+        value = max(value, lowest)
+        x = torch.randn(rows, vocab, device="cuda") * 3
+        if kind == "all lowest":
+            x[:] = value
+        elif kind == "few left":
+            x[:, 3:-3] = value
+        elif kind == "one left at the lowest":  # the row's largest is itself a large negative number
+            x[:] = lowest
+            x[:, vocab // 2] = value / 2
+        elif kind == "two masks":
+            x[:] = value
+            x[:, ::7] = lowest
+        elif kind == "masked and -inf":
+            x[:] = -math.inf
+            x[:, 5::11] = value
+        elif kind == "highest":
+            x[:, 1::5] = -value  # (and none far below 0: their log probabilities would not be numbers of 32 bits)
+        elif kind == "steps":  # neighbours of 2^28, 16 and 32 apart in fp32
+            x[:] = -(2.0 ** 28)
+            x[:, 1::3] = -(2.0 ** 28) - 32
+            x[:, 2::3] = -(2.0 ** 28) + 16
+            if value == lowest:
+                x = -x
+        x = x.clamp(lowest, highest) if kind != "masked and -inf" else x
+        check_logprobs(ops, x.to(dtype).contiguous(), torch.randint(0, vocab, (rows,), device="cuda"), min(20, vocab))
+
+
 def test_logprobs_tokens_that_are_none_or_out_of_range(ops):
     x = torch.randn(4, 100, device="cuda")
     status = ops.new_status("cuda")
