@@ -408,10 +408,17 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
                 if (k0 + g + e < a.dk) *at = s[e];
         };
         if (from == nullptr && chunks > 0) {  // (little code: fetched cold, the loop below takes 2 us)
+            // the columns that this warp itself reads: U does not wait for S, so nothing orders other warps' columns before its first reading
             const uint32_t zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            const uint32_t columns = lane_base + kLtS + (warp >> 2) * (kLtTmemCols - kLtS) / 2;  // S and its parts are the columns from kLtS on
+            if (C::NS == 2) {
 #pragma unroll 1
-            for (uint32_t g = 0; g < (kLtTmemCols - kLtS) / 2; g += 8) lt_st(columns + g, zero);
+                for (int g = 0; g < kHalf; g += 8) lt_st(lane_base + kLtS + k0 + g, zero);
+            }
+#pragma unroll 1
+            for (int p = 0; p < C::NS; ++p) {
+#pragma unroll 1
+                for (int g = 0; g < kHalf / 2; g += 8) lt_st(lane_base + C::kParts + p * kHalf + k0 / 2 + g, zero);
+            }
         } else {
 #pragma unroll 1
             for (int g = 0; g < kHalf; g += 16) {

@@ -13,8 +13,8 @@
 //
 // A row is one CTA, or a cluster of up to eight whose parts meet in the first one's shared memory; a short row is a warp.
 //
-// Bound by HBM where rows are many (4096 rows of 32000 in bf16: 54 us, 4.8 TB/s; exponentials and issue take half of the time beside it)
-// and by latency where they are few (one row of 32000 in fp32 4.3 us, with five alternatives 7.1: the choice is eight block barriers).
+// Bound by HBM where rows are many (4096 rows of 32000 in bf16: 57 us, 4.6 TB/s; exponentials and issue take half of the time beside it)
+// and by latency where they are few (one row of 32000 in fp32 4.8 us, with five alternatives 7.6: the choice is eight block barriers).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -297,6 +297,7 @@ __device__ __forceinline__ void lp_each(const LpPart<T>& p, F f) {
 
 // A part whose largest element is 2^28 or more from 0, once more: there x log2e is rounded by so much that powers of the remainder overflow
 // (and -inf, where a mask is the type's lowest value).  Nothing else comes here: masked elements below a row of usual ones count as nothing.
+// (A call: inlined, the loop over usual rows came out slower, 4096 rows of 32000 in bf16 65 us and 57.)
 template <typename T, bool TOP>
 __device__ __noinline__ void lp_again(LpShared<TOP>& sh, const LpPart<T>& p) {
     constexpr int N = LpVec<T>::N;
@@ -631,7 +632,7 @@ static int launch_logprobs_short(const LpArgs& a, int rows, cudaStream_t st) {
 template <typename T, bool TOP>
 static int launch_logprobs(const LpArgs& a, int rows, cudaStream_t st) {
     const int vecs = a.vocab / LpVec<T>::N;
-    // One CTA per row, unless rows are few and long.  Without alternatives a part of 512 vectors at least (one row of 32000 fp32 logits 4.3 us
+    // (figures that were timed together)  One CTA per row, unless rows are few and long.  Without alternatives a part of 512 vectors at least (one row of 32000 fp32 logits 4.3 us
     // in eight parts, 4.5 in four, 5.2 in one).  With alternatives the parts' lists have to meet: four parts from 8192 vectors on (8 rows of
     // 65536 in bf16 8.9 us in one, 7.6 in four, 7.7 in eight), fewer vectors in one (one row of 32000 in fp32 7.1, in eight 8.2).  With several
     // rows per SM 256 threads a row (4096 rows of 32000: 54 us, with 512 threads 62), else 512 (256 rows of 131072: 24 and 37).
