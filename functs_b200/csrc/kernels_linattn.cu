@@ -128,14 +128,16 @@ __global__ void __launch_bounds__(kRecurThreads) linattn_recurrent_kernel(const 
 
 // One token, many states: a CTA has a whole state, LANES lanes a row of it, so that 64 KB are on their way at once and one slot is looked up.
 constexpr int kStepThreads = 256;
-template <typename T, int LANES>
+// A lane has four columns of a row, beside one another (VEC: rows of whole 16 bytes) or LANES apart.
+template <typename T, int LANES, bool VEC>
 __global__ void __launch_bounds__(kStepThreads) linattn_step_kernel(const LinArgs a) {
     constexpr int WARPS = kStepThreads / 32, PER = 32 / LANES, STEP = WARPS * PER, ROWS = kLinMaxDim / STEP;
     __shared__ float s_q[kLinMaxDim], s_k[kLinMaxDim];
     __shared__ __align__(16) float s_part[WARPS][LANES * 4];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int h = blockIdx.x % a.heads, b = blockIdx.x / a.heads, hk = h / (a.heads / a.kv_heads);
-    const int row = warp * PER + lane / LANES, col = (lane % LANES) * 4;
+    const int row = warp * PER + lane / LANES, col = (lane % LANES) * (VEC ? 4 : 1);
+    constexpr int kNext = VEC ? 1 : LANES;  // columns between two of a lane's
     const bool has_col = col < a.dv;
     const int named = a.slots == nullptr ? b : a.slots[b];
     const bool inside = named >= 0 && named < a.num_slots;
@@ -145,8 +147,17 @@ __global__ void __launch_bounds__(kStepThreads) linattn_step_kernel(const LinArg
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
         const int r = row + i * STEP;
-        s[i] = inside && has_col && r < a.dk && a.state_in != nullptr ? *reinterpret_cast<const float4*>(a.state_in + state + static_cast<int64_t>(r) * a.dv + col)
-                                                                      : make_float4(0.f, 0.f, 0.f, 0.f);
+        s[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (inside && has_col && r < a.dk && a.state_in != nullptr) {
+            const float* at = a.state_in + state + static_cast<int64_t>(r) * a.dv + col;
+            if (VEC) s[i] = *reinterpret_cast<const float4*>(at);
+            else {
+                s[i].x = at[0];
+                if (col + kNext < a.dv) s[i].y = at[kNext];
+                if (col + 2 * kNext < a.dv) s[i].z = at[2 * kNext];
+                if (col + 3 * kNext < a.dv) s[i].w = at[3 * kNext];
+            }
+        }
     }
     const T* q = static_cast<const T*>(a.q) + b * a.q_stride[0] + h * a.q_stride[2];
     const T* k = static_cast<const T*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2];
@@ -156,7 +167,7 @@ __global__ void __launch_bounds__(kStepThreads) linattn_step_kernel(const LinArg
     else s_k[tid - kLinMaxDim] = tid - kLinMaxDim < a.dk ? lin_float(k[tid - kLinMaxDim]) : 0.0f;
     float x[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = has_col ? lin_float(v[col + j]) : 0.0f;
+    for (int j = 0; j < 4; ++j) x[j] = col + j * kNext < a.dv ? lin_float(v[col + j * kNext]) : 0.0f;
     int bits;
     const int slot = lin_slot(a, b, lane, bits);
     if (bits != 0 && a.status != nullptr && tid == 0) atomicOr(a.status, bits);
@@ -173,14 +184,26 @@ __global__ void __launch_bounds__(kStepThreads) linattn_step_kernel(const LinArg
         s[i].w = fmaf(kr, x[3], fmaf(decay, s[i].w, decay_lo * s[i].w));
         o[0] = fmaf(qr, s[i].x, o[0]), o[1] = fmaf(qr, s[i].y, o[1]), o[2] = fmaf(qr, s[i].z, o[2]), o[3] = fmaf(qr, s[i].w, o[3]);
         const int r = row + i * STEP;
-        if (slot >= 0 && has_col && r < a.dk) *reinterpret_cast<float4*>(a.state_out + state + static_cast<int64_t>(r) * a.dv + col) = s[i];
+        if (slot >= 0 && has_col && r < a.dk) {
+            float* at = a.state_out + state + static_cast<int64_t>(r) * a.dv + col;
+            if (VEC) *reinterpret_cast<float4*>(at) = s[i];
+            else {
+                at[0] = s[i].x;
+                if (col + kNext < a.dv) at[kNext] = s[i].y;
+                if (col + 2 * kNext < a.dv) at[2 * kNext] = s[i].z;
+                if (col + 3 * kNext < a.dv) at[3 * kNext] = s[i].w;
+            }
+        }
     }
 #pragma unroll
     for (int d = LANES; d < 32; d *= 2) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[j] += __shfl_xor_sync(kFullMask, o[j], d);
     }
-    if (lane < LANES) *reinterpret_cast<float4*>(&s_part[warp][col]) = make_float4(o[0], o[1], o[2], o[3]);
+    if (lane < LANES) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s_part[warp][col + j * kNext] = o[j];
+    }
     __syncthreads();
     if (tid < a.dv) {
         float y = 0.0f;
@@ -200,6 +223,14 @@ static bool lin_by_chunks(const LinArgs& a) {
     return a.tokens > 1 && 3.5 + a.tokens * (token > 0.3 ? token : 0.3) > chunk;
 }
 
+template <typename T, bool VEC>
+static int launch_step(const LinArgs& a, cudaStream_t st) {
+    const dim3 grid(static_cast<unsigned>(a.batch) * a.heads), block(kStepThreads);
+    if (a.dv <= 32) return launch_after(linattn_step_kernel<T, 8, VEC>, grid, block, 0, st, false, "linear_attention", a);
+    if (a.dv <= 64) return launch_after(linattn_step_kernel<T, 16, VEC>, grid, block, 0, st, false, "linear_attention", a);
+    return launch_after(linattn_step_kernel<T, 32, VEC>, grid, block, 0, st, false, "linear_attention", a);
+}
+
 template <typename T>
 static int launch_recurrent(const LinArgs& a, cudaStream_t st) {
     const bool vec = a.dv % 4 == 0 && reinterpret_cast<uintptr_t>(a.state_in) % 16 == 0 && reinterpret_cast<uintptr_t>(a.state_out) % 16 == 0;
@@ -207,13 +238,9 @@ static int launch_recurrent(const LinArgs& a, cudaStream_t st) {
     const int tiles = (a.dv + 31) / 32;
     FB_REQUIRE(bh * tiles < (1ll << 31), "linear_attention: batch * heads is too large");
     // Whole states where they are small (48 of 64 x 64 3.2 us, in column tiles 4.1) or fill half of the SMs (128 x 128: 16 states 4.6, in
-    // tiles 3.9; 64 4.8 and 4.7; 112 5.1 and 6.1; 256 7.1 and 9.7; 1536 42 and 53)
-    if (vec && a.tokens == 1 && a.lengths == nullptr && (a.dk * a.dv <= 64 * 64 || bh >= kNumSMs / 2)) {
-        const dim3 whole(static_cast<unsigned>(bh)), block(kStepThreads);
-        if (a.dv <= 32) return launch_after(linattn_step_kernel<T, 8>, whole, block, 0, st, false, "linear_attention", a);
-        if (a.dv <= 64) return launch_after(linattn_step_kernel<T, 16>, whole, block, 0, st, false, "linear_attention", a);
-        return launch_after(linattn_step_kernel<T, 32>, whole, block, 0, st, false, "linear_attention", a);
-    }
+    // tiles 3.9; 64 4.8 and 4.7; 112 5.1 and 6.1; 256 7.1 and 9.7; 1536 42 and 53; of 128 x 39, 2856 31 and 51)
+    if (a.tokens == 1 && a.lengths == nullptr && (a.dk * a.dv <= 64 * 64 || bh >= kNumSMs / 2))
+        return vec ? launch_step<T, true>(a, st) : launch_step<T, false>(a, st);
     const dim3 grid(static_cast<unsigned>(bh * tiles));
     if (vec) return launch_after(linattn_recurrent_kernel<T, 8, true>, grid, dim3(kRecurThreads), 0, st, false, "linear_attention", a, tiles);
     return launch_after(linattn_recurrent_kernel<T, 8, false>, grid, dim3(kRecurThreads), 0, st, false, "linear_attention", a, tiles);

@@ -160,7 +160,8 @@ def test_step(ops, shape, dtype):
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("shape", [(73, 1, 1, 128, 128), (74, 1, 1, 128, 128), (1, 1, 1, 128, 32), (1, 2, 1, 128, 36), (3, 2, 2, 33, 124), (2, 3, 1, 3, 4),
-                                   (5, 2, 2, 64, 64), (5, 2, 2, 65, 64)], ids=str)
+                                   (5, 2, 2, 64, 64), (5, 2, 2, 65, 64), (40, 2, 1, 128, 127), (74, 1, 1, 127, 65), (5, 2, 2, 65, 39), (7, 3, 1, 128, 31),
+                                   (5, 4, 2, 64, 33), (3, 1, 1, 1, 1), (2, 2, 2, 20, 7)], ids=str)
 def test_step_of_whole_states_and_of_tiles(ops, shape, dtype):
     """Sizes on either side of those where a block takes a whole state; some slots name no sequence."""
     b, h, hk, dk, dv = shape
