@@ -517,6 +517,10 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
             unsigned char *st = smem + stage * C::kStage, *vt = smem + C::oV + (c % C::kStagesV) * C::NX * C::kTileV;
             if (TMA) {
                 if (!lt_wait(m, &m.full_v[c % C::kStagesV], (c / C::kStagesV) & 1)) break;
+                // W's place is free when the product before that has it is done.  That product has read its K too, so the wait for K below
+                // is for this chunk's: V alone is two chunks ahead of Q and K, and a barrier that is still in the phase of the chunk
+                // before in this stage lets a wait for the other parity through.
+                if (c >= C::kStages && !lt_wait(m, &m.w_free[stage], turn ^ 1u)) break;
                 // rows behind the sequence are somebody's: K (here) and V (below) must be zero there; Q's make rows that nobody reads
                 if (n < kLtChunk && !lt_wait(m, &m.full[stage], turn)) break;
                 for (int i = id; i < (kLtChunk - n) * (DK / 8); i += threads)
@@ -550,8 +554,8 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
                     }
                 }
             }
-            // V, and W (free when the product before that has it is done)
-            if (c >= C::kStages && !lt_wait(m, &m.w_free[stage], turn ^ 1u)) break;
+            // V, and W
+            if (!TMA && c >= C::kStages && !lt_wait(m, &m.w_free[stage], turn ^ 1u)) break;
             unsigned char* wt = smem + C::oW + stage * C::NW * C::kTileV;
             // a warp's piece: 16 bytes of eight tokens beside one another, four groups of channels.  A thread keeps to its tokens.
             constexpr int kGroups = DV / 32;

@@ -688,3 +688,29 @@ def test_decaying_state_program_that_does_not_fit_the_kernels(ops):
         assert jit.interpreted_functor_runs() > before
         want, want_s = patterns.DecayAttentionSeq(decay)(q, k, v)
         assert torch.allclose(outs, want) and torch.allclose(s, want_s)
+
+
+@pytest.mark.parametrize("b,t,d", [(40, 131, 128), (6, 190, 128), (1, 3 * 64 + 5, 64), (30, 5 * 64 + 33, 64)])
+def test_prompt_whose_last_chunk_is_partial_and_whose_queries_arrive_late(ops, b, t, d):
+    """Three chunks and more, the last one partial: V is at hand, Q and K are not (every token's row in a page of its own, out of the cache),
+    and what lies behind the sequences is NaN."""
+    h = 4
+    far = 2 ** 14 // h
+    room = [torch.full((b, t + 40, h, far // (4 if i else 1)), math.nan, device="cuda", dtype=BF16) for i in range(2)]
+    q, k = (x[:, :, :, 8:8 + d] for x in room)
+    v = torch.full((b, t + 40, h, d), math.nan, device="cuda", dtype=BF16)
+    for x in (q, k, v):
+        x[:, :t] = torch.randn(b, t, h, d, device="cuda").to(BF16)
+    lengths = torch.full((b,), t, device="cuda", dtype=torch.int32)
+    want = recurrence(q[:, :t], k[:, :t], v[:, :t], decays(h), 0.1, None, lengths)
+    flush = torch.empty(2 ** 28, device="cuda", dtype=torch.uint8)
+    first = None
+    for i in range(12):
+        flush.fill_(i)
+        v.sum()
+        out, state = ops.linear_attention(q, k, v, decays(h), scale=0.1, lengths=lengths)
+        if first is None:
+            first = out, state
+            check_attention(out[:, :t], state, want, BF16, t, d)
+        assert torch.equal(out, first[0]) and torch.equal(state, first[1])
+        assert bool((out[:, t:] == 0).all())
