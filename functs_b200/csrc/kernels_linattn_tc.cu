@@ -325,7 +325,7 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
     if (slot < 0 || (plan.mode == 2 && seg_end <= seg0)) return;
     const int chunks = max(0, seg_end - seg0 + kLtChunk - 1) / kLtChunk;
 
-    const double log_decay = static_cast<double>(fmaxf(a.log_decay[h], -1e30f));
+    const double log_decay = static_cast<double>(lin_log_decay(a, h));
     if (tid <= kLtChunk) {
         const double p = exp(log_decay * tid);
         m.power[tid] = static_cast<float>(p);
@@ -893,12 +893,12 @@ __global__ void __launch_bounds__(256) linattn_carry_kernel(const LinArgs a, flo
     const int64_t own = (static_cast<int64_t>(slot) * a.heads + h) * cells + cell;
     float* part = states + (static_cast<int64_t>(b) * a.heads + h) * segs * cells + cell;
     float s = a.state_in != nullptr ? a.state_in[own] : 0.0f;
-    const float log_decay = a.log_decay[h];
+    const float log_decay = lin_log_decay(a, h);
     for (int i = 0; i < segs; ++i) {
         const int n = min(max(length - i * seg_tokens, 0), i + 1 < segs ? seg_tokens : length);
         const float added = part[i * cells];
         part[i * cells] = s;
-        s = fmaf(lin_decay(log_decay, n), s, added);
+        if (n > 0) s = fmaf(lin_decay(log_decay, n), s, added);  // (no tokens, no decay: not even one that is NaN)
     }
     a.state_out[own] = s;
 }

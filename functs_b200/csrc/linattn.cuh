@@ -30,8 +30,10 @@ __device__ __forceinline__ __half lin_from<__half>(float x) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 lin_from<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// exp(log_decay * n): the weight of a token n steps back.  A decay of -inf forgets at once, but not what it just saw: n = 0 is 1.
-__device__ __forceinline__ float lin_decay(float log_decay, int n) { return expf(fmaxf(log_decay, -1e30f) * static_cast<float>(n)); }
+// A head's log decay.  One of -inf forgets at once, but not what it just saw: -1e30 * 0 is 0 where -inf * 0 is not.  A NaN stays one.
+__device__ __forceinline__ float lin_log_decay(const LinArgs& a, int h) { return max_nan(a.log_decay[h], -1e30f); }
+// exp(log_decay * n): the weight of a token n steps back.
+__device__ __forceinline__ float lin_decay(float log_decay, int n) { return expf(log_decay * static_cast<float>(n)); }
 
 __device__ __forceinline__ int lin_length(const LinArgs& a, int b) {
     return a.lengths == nullptr ? a.tokens : min(max(a.lengths[b], 0), a.tokens);

@@ -714,3 +714,23 @@ def test_prompt_whose_last_chunk_is_partial_and_whose_queries_arrive_late(ops, b
             check_attention(out[:, :t], state, want, BF16, t, d)
         assert torch.equal(out, first[0]) and torch.equal(state, first[1])
         assert bool((out[:, t:] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("tokens,d", [(1, 64), (5, 64), (150, 64), (200, 128), (2048, 64)])
+def test_decay_that_is_not_a_number(ops, tokens, d, dtype):
+    """A NaN in one head's decay: that head's outputs and states are NaN however many tokens there are, other heads are as without it, and a
+    sequence without tokens keeps its state."""
+    b, h = 2, 3
+    q, k, v = make(b, tokens, h, h, d, d, dtype)
+    g = decays(h)
+    bad = g.clone()
+    bad[1] = math.nan
+    for lengths in (None, torch.tensor([tokens, 0], device="cuda", dtype=torch.int32)):
+        for start in (None, torch.randn(b, h, d, d, device="cuda")):
+            clean, clean_state = ops.linear_attention(q, k, v, g, state=None if start is None else start.clone(), lengths=lengths)
+            out, state = ops.linear_attention(q, k, v, bad, state=None if start is None else start.clone(), lengths=lengths)
+            live = b if lengths is None else 1
+            assert bool(torch.isnan(out[:live, :, 1]).all()) and bool(torch.isnan(state[:live, 1]).all())
+            assert torch.equal(out[:, :, ::2], clean[:, :, ::2]) and torch.equal(state[:, ::2], clean_state[:, ::2])
+            assert torch.equal(out[live:], clean[live:]) and torch.equal(state[live:], clean_state[live:])
