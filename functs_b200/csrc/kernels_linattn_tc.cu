@@ -893,12 +893,20 @@ __global__ void __launch_bounds__(256) linattn_carry_kernel(const LinArgs a, flo
     const int64_t own = (static_cast<int64_t>(slot) * a.heads + h) * cells + cell;
     float* part = states + (static_cast<int64_t>(b) * a.heads + h) * segs * cells + cell;
     float s = a.state_in != nullptr ? a.state_in[own] : 0.0f;
-    const float log_decay = lin_log_decay(a, h);
+    // The decay of a part as a sum of two floats: rounded to one, it would be off the same way for every part (and expf takes an exponent that
+    // is rounded itself: 2.7e-6 of a state that passed 64 parts).
+    const double log_decay = static_cast<double>(lin_log_decay(a, h));
+    float decay = 1.0f, decay_lo = 0.0f;
+    int of = 0;  // tokens that they are of
     for (int i = 0; i < segs; ++i) {
         const int n = min(max(length - i * seg_tokens, 0), i + 1 < segs ? seg_tokens : length);
+        if (n > 0 && n != of) {
+            const double exact = exp(log_decay * static_cast<double>(n));
+            decay = static_cast<float>(exact), decay_lo = static_cast<float>(exact - static_cast<double>(decay)), of = n;
+        }
         const float added = part[i * cells];
         part[i * cells] = s;
-        if (n > 0) s = fmaf(lin_decay(log_decay, n), s, added);  // (no tokens, no decay: not even one that is NaN)
+        if (n > 0) s = fmaf(decay, s, fmaf(decay_lo, s, added));  // (no tokens, no decay: not even one that is NaN)
     }
     a.state_out[own] = s;
 }

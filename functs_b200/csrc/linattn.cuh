@@ -32,8 +32,6 @@ __device__ __forceinline__ __nv_bfloat16 lin_from<__nv_bfloat16>(float x) { retu
 
 // A head's log decay.  One of -inf forgets at once, but not what it just saw: -1e30 * 0 is 0 where -inf * 0 is not.  A NaN stays one.
 __device__ __forceinline__ float lin_log_decay(const LinArgs& a, int h) { return max_nan(a.log_decay[h], -1e30f); }
-// exp(log_decay * n): the weight of a token n steps back.
-__device__ __forceinline__ float lin_decay(float log_decay, int n) { return expf(log_decay * static_cast<float>(n)); }
 
 __device__ __forceinline__ int lin_length(const LinArgs& a, int b) {
     return a.lengths == nullptr ? a.tokens : min(max(a.lengths[b], 0), a.tokens);

@@ -734,3 +734,23 @@ def test_decay_that_is_not_a_number(ops, tokens, d, dtype):
             assert bool(torch.isnan(out[:live, :, 1]).all()) and bool(torch.isnan(state[:live, 1]).all())
             assert torch.equal(out[:, :, ::2], clean[:, :, ::2]) and torch.equal(state[:, ::2], clean_state[:, ::2])
             assert torch.equal(out[live:], clean[live:]) and torch.equal(state[live:], clean_state[live:])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("t", [8192, 4000])
+def test_slow_decays_over_many_parts(ops, t, dtype):
+    """A state that outlives a long prompt, which is cut into parts.  Its tokens add next to nothing, so that the error is the decay's: of
+    every token's or part's factor at most half a step if it is rounded apart from the others (random, so sqrt(128) * 2^-24 = 6.7e-7 for
+    128 factors), and 2^-25 * 128 = 3.8e-6 if it is the same every time."""
+    h, d = 2, 64
+    g = torch.tensor([-1.59e-7, -1e-4], device="cuda")
+    for g in (g, torch.tensor([0.0, -1e-5], device="cuda"), torch.tensor([-2.3e-6, -3.7e-4], device="cuda")):
+        q, k, v = make(1, t, h, h, d, d, dtype)
+        k, v = k * 2.0 ** -10, v * 2.0 ** -10
+        start = torch.randn(1, h, d, d, device="cuda") * 100
+        state = start.clone()
+        want = recurrence(q, k, v, g, 0.1, start, torch.full((1,), t, device="cuda"))
+        out, _ = ops.linear_attention(q, k, v, g, scale=0.1, state=state)
+        check_attention(out, state, want, dtype, t, d)
+        for i in range(h):
+            assert float((state[:, i].double() - want[1][:, i]).norm()) <= 1e-6 * float(want[1][:, i].norm())
