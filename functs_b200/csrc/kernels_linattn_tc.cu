@@ -48,7 +48,11 @@ namespace fb {
 
 constexpr int kLtChunk = 64;
 constexpr int kLtWarpsS = 8, kLtWarpsP = 8;  // (of the P group four make P, two issue products, one copies)
-constexpr uint32_t kLtWaitLimit = 200000u;
+constexpr uint32_t kLtWaitLimit = 200000u, kLtWaitLimitDropped = 5000u;
+// Development switch (functs_b200_debug_set "linattn_drop_state"): in this thread's calls nobody says that S is there, so that the waits for it,
+// and for what follows from it, run out.
+static thread_local int t_lt_drop = 0;
+void linattn_set_drop_state(int on) { t_lt_drop = on ? 1 : 0; }
 // TMEM columns: U (and, between two of them, G), X, Y, S^T in fp32 and as two operand parts of DK / 2 columns, or as three parts, which are exact
 constexpr uint32_t kLtU = 0, kLtG = 0, kLtX = 128, kLtY = 192, kLtS = 256, kLtTmemCols = 512;
 
@@ -74,8 +78,10 @@ struct LtCfg {
 struct LtMisc {
     uint64_t full[2], full_v[3], v_whole[3], empty[2], w_full[2], w_free[2];  // stages; v_whole: V with zeros where it must have them
     uint64_t g_full, g_read, u_full, u_free, s_full, x_full, p_full, y_full, xy_free;
+    uint64_t none_left[2];                         // of the two warps that issue products: theirs are done
     uint32_t tmem;
     int dead;                                      // a wait ran out
+    uint32_t wait_limit;                           // tries of a wait
     int b;
     float power_next, power_gap, power_off;        // the float beyond power[64] on decay^64's side, how far, and how far decay^64 is (relative)
     float power[kLtChunk + 4];                        // decay^i
@@ -94,6 +100,8 @@ struct LtPlan {
     int mode;        // 0: whole sequences; 1: the state that each part adds, 2: outputs of the parts
     int boundary;    // of which all rows lie: 16, 8, 4 or 2 bytes
     float* states;   // [batch * heads][segs][dk][dv]
+    uint32_t wait_limit;  // tries of a wait
+    int drop_state;       // the switch below
 };
 
 // ---- small pieces ---------------------------------------------------------------------------------------------------
@@ -181,7 +189,7 @@ __device__ __forceinline__ bool lt_try(uint64_t* bar, uint32_t parity) {
     return ok != 0;
 }
 __device__ __forceinline__ bool lt_wait_one(LtMisc& m, uint64_t* bar, uint32_t parity) {
-    for (uint32_t i = 0; i < kLtWaitLimit; ++i) {
+    for (uint32_t i = 0; i < m.wait_limit; ++i) {
         if (lt_try(bar, parity)) return true;
         if ((i & 7u) == 7u && *reinterpret_cast<volatile int*>(&m.dead)) return false;
     }
@@ -361,6 +369,7 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
             mbar_init(&m.w_free[i], 1);
         }
         mbar_init(&m.g_full, 1), mbar_init(&m.u_full, 1), mbar_init(&m.x_full, 1), mbar_init(&m.y_full, 1);
+        mbar_init(&m.none_left[0], 1), mbar_init(&m.none_left[1], 1);
         mbar_init(&m.p_full, 4);
         mbar_init(&m.g_read, 4);
         mbar_init(&m.u_free, kLtWarpsS);
@@ -368,6 +377,7 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
         mbar_init(&m.xy_free, C::kWarpsO);
         fence_barrier_init();
         m.dead = 0;
+        m.wait_limit = plan.wait_limit;
         m.bad = 0x7fffffff;
     }
     if (warp == 0) {
@@ -431,7 +441,7 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
             }
         }
         lt_st_wait();
-        lt_arrive_read(&m.s_full, lane);
+        if (!plan.drop_state) lt_arrive_read(&m.s_full, lane);
         // The decay of a chunk is one of the two floats beside it, by turns, so that their product stays within half a step of the decay's
         // power: rounded the same way every time it would be off by 2^-25 per chunk.
         float drift = 0.0f;
@@ -810,6 +820,11 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
                     __syncwarp();
                 }
             }
+            // none of its products is under way when the CTA ends, not even where somebody gave up (TMEM is freed, and barriers end with it)
+            uint64_t* none_left = &m.none_left[warp == C::kFirstP + 6 ? 0 : 1];
+            if (lt_elect()) tc_commit(none_left);
+            __syncwarp();
+            for (uint32_t i = 0; i < plan.wait_limit && !lt_try(none_left, 0); ++i) {}
         }
     } else if (TMA && warp == C::kFirstP + 3 && lane == 0) {
         // ---- the copies: Q and K of a chunk and V of the next
@@ -834,7 +849,7 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
             issued = c + 1;
             if (c + 1 < chunks) copy_v(c + 1);
         }
-        // nothing is in flight when the CTA ends, not even where somebody gave up
+        // no copy is in flight when the CTA ends, not even where somebody gave up
         for (int c = max(0, issued - C::kStages); c < issued; ++c) mbar_wait_bounded(&m.full[c % C::kStages], (c / C::kStages) & 1, kLtWaitLimit);
         for (int c = max(0, issued_v - C::kStagesV); c < issued_v; ++c)
             mbar_wait_bounded(&m.full_v[c % C::kStagesV], (c / C::kStagesV) & 1, kLtWaitLimit);
@@ -968,6 +983,8 @@ static int launch_chunk(const LinArgs& a, void* scratch, cudaStream_t st) {
     constexpr int bytes = C::oMisc + static_cast<int>(sizeof(LtMisc));
     static_assert(bytes <= 232448, "shared memory");
     LtPlan plan = {};
+    plan.drop_state = t_lt_drop;
+    plan.wait_limit = t_lt_drop ? kLtWaitLimitDropped : kLtWaitLimit;
     plan.tiles = (a.dv + DV - 1) / DV;
     const int64_t rows = static_cast<int64_t>(a.batch) * a.heads;
     lt_cut(a, rows, plan.segs, plan.seg_tokens);

@@ -91,6 +91,7 @@ constexpr int kLstmDefaultMode = 3;
 namespace fb {
 void yolo_set_prune(int on);
 void lstm_set_drop_exchange(int on);
+void linattn_set_drop_state(int on);
 }
 
 extern "C" {
@@ -160,6 +161,10 @@ int functs_b200_debug_set(const char* name, int32_t value) {
     }
     if (name != nullptr && std::strcmp(name, "lstm_drop_exchange") == 0) {
         fb::lstm_set_drop_exchange(value);
+        return FB_OK;
+    }
+    if (name != nullptr && std::strcmp(name, "linattn_drop_state") == 0) {
+        fb::linattn_set_drop_state(value);
         return FB_OK;
     }
     fb::set_error("debug_set: unknown switch");

@@ -294,7 +294,9 @@ int functs_b200_token_logprobs(const void* logits, int32_t dtype, int64_t row_st
  *   "yolo_prune": 0 makes functs_b200_yolo_postprocess keep every candidate above the score threshold instead of
  *                 those that reach the image's score floor (default 1; the outputs are the same either way).
  *   "lstm_drop_exchange": 1 makes the CTAs of the LSTM's cluster recurrence send each other nothing, in the calls of this
- *                 thread: every wait gives up and FB_STATUS_WAIT_TIMEOUT is set (default 0). */
+ *                 thread: every wait gives up and FB_STATUS_WAIT_TIMEOUT is set (default 0).
+ *   "linattn_drop_state": 1 makes prompts that go by chunks, in the calls of this thread, wait in vain for their state: they give up
+ *                 within some tenths of a second and FB_STATUS_WAIT_TIMEOUT is set (default 0). */
 int functs_b200_debug_set(const char* name, int32_t value);
 
 /* ---- C5: YOLACT-style mask assembly ------------------------------------------------------------ */

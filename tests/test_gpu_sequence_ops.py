@@ -754,3 +754,33 @@ def test_slow_decays_over_many_parts(ops, t, dtype):
         check_attention(out, state, want, dtype, t, d)
         for i in range(h):
             assert float((state[:, i].double() - want[1][:, i]).norm()) <= 1e-6 * float(want[1][:, i].norm())
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("b,t,h,d", [(2, 60, 2, 64), (2, 200, 2, 128), (1, 2048, 2, 64)])
+def test_waits_that_run_out(ops, b, t, h, d, dtype):
+    """With the state never announced the waits for it run out: the kernel ends all the same, with no product and no copy under way, says so to
+    the caller's status word, or else to the next call once, and the one after that is as ever."""
+    import functs_b200
+    from functs_b200 import _lib
+    q, k, v = make(b, t, h, h, d, d, dtype)
+    want = ops.linear_attention(q, k, v, decays(h))
+    status = ops.new_status("cuda")
+    drop = lambda on: _lib.check(_lib.lib.functs_b200_debug_set(b"linattn_drop_state", on), "debug_set")  # noqa: E731
+    for given in (status, None):
+        drop(1)
+        try:
+            ops.linear_attention(q, k, v, decays(h), status=given)
+        finally:
+            drop(0)
+        torch.cuda.synchronize()
+        if given is not None:
+            with pytest.raises(functs_b200.FunctsB200Error, match="wait ran out"):
+                ops.raise_on_status(status, "linear_attention")
+        else:
+            with pytest.raises(RuntimeError, match="wait ran out in an earlier call"):
+                ops.linear_attention(q, k, v, decays(h))
+        for _ in range(2):
+            got = ops.linear_attention(q, k, v, decays(h))
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    torch.cuda.synchronize()
