@@ -5,6 +5,8 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <cstring>
+
 #include "../../../include/functs_b200.h"
 
 namespace functs_b200 {
@@ -32,31 +34,35 @@ void checkSizes(const at::Tensor& t, at::IntArrayRef sizes, const char* name) {
     TORCH_CHECK_VALUE(t.sizes() == sizes, name, " must be of sizes ", sizes, ", not ", t.sizes());
 }
 
-// Where a kernel says that a wait of its own ran out, for callers that give no status word: in pinned host memory, asked at the next call.
-// (Slots and tokens that are out of range are the caller's; without a status word they are skipped as documented, and not reported.)
-int32_t* ownStatusWord() {
-    static int32_t* const word = [] {
+// Where a kernel says that a wait of its own ran out, for callers that give no status word: in pinned host memory, a word for each device, asked
+// at that device's next call.  (Slots and tokens that are out of range are the caller's; without a status word they are skipped as documented,
+// and not reported.)
+constexpr int kMostDevices = 64, kWordsApart = 16;  // (a line of 64 bytes each)
+int32_t* ownStatusWord(const at::Device& device) {
+    static int32_t* const words = [] {
         void* p = nullptr;
         cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // (the first call may be one that is captured)
         cudaThreadExchangeStreamCaptureMode(&mode);
-        const cudaError_t rc = cudaHostAlloc(&p, 64, cudaHostAllocPortable | cudaHostAllocMapped);
+        const cudaError_t rc = cudaHostAlloc(&p, kMostDevices * kWordsApart * sizeof(int32_t), cudaHostAllocPortable | cudaHostAllocMapped);
         cudaThreadExchangeStreamCaptureMode(&mode);
         if (rc != cudaSuccess) {
             cudaGetLastError();
             return static_cast<int32_t*>(nullptr);
         }
-        *static_cast<int32_t*>(p) = 0;
+        std::memset(p, 0, kMostDevices * kWordsApart * sizeof(int32_t));
         return static_cast<int32_t*>(p);
     }();
-    if (word != nullptr && (*static_cast<volatile int32_t*>(word) & FB_STATUS_WAIT_TIMEOUT) != 0) {
+    if (words == nullptr || device.index() < 0 || device.index() >= kMostDevices) return nullptr;
+    int32_t* const word = words + device.index() * kWordsApart;
+    if ((*static_cast<volatile int32_t*>(word) & FB_STATUS_WAIT_TIMEOUT) != 0) {
         *static_cast<volatile int32_t*>(word) = 0;
-        TORCH_CHECK(false, "linear_attention: a bounded device-side wait ran out in an earlier call; its outputs mean nothing");
+        TORCH_CHECK(false, "linear_attention: a bounded device-side wait ran out in an earlier call on ", device, "; its outputs mean nothing");
     }
     return word;
 }
 
 int32_t* statusWord(const MaybeTensor& status, const at::Device& device, bool own) {
-    if (!status.has_value()) return own ? ownStatusWord() : nullptr;
+    if (!status.has_value()) return own ? ownStatusWord(device) : nullptr;
     TORCH_CHECK_VALUE(status->scalar_type() == at::kInt && status->numel() >= 1 && (status->device() == device || status->is_pinned()),
                       "status must be an int32 tensor on ", device, " or in pinned memory");
     return status->data_ptr<int32_t>();

@@ -784,3 +784,19 @@ def test_waits_that_run_out(ops, b, t, h, d, dtype):
             got = ops.linear_attention(q, k, v, decays(h))
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     torch.cuda.synchronize()
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="one device")
+def test_a_wait_that_ran_out_is_told_on_its_own_device(ops):
+    from functs_b200 import _lib
+    q, k, v = make(1, 200, 2, 2, 64, 64, BF16)
+    drop = lambda on: _lib.check(_lib.lib.functs_b200_debug_set(b"linattn_drop_state", on), "debug_set")  # noqa: E731
+    drop(1)
+    try:
+        ops.linear_attention(q, k, v, decays(2))
+    finally:
+        drop(0)
+    torch.cuda.synchronize()
+    ops.linear_attention(*(x.to("cuda:1") for x in (q, k, v, decays(2))))
+    with pytest.raises(RuntimeError, match="wait ran out in an earlier call on cuda:0"):
+        ops.linear_attention(q, k, v, decays(2))
