@@ -500,7 +500,7 @@ Operation makeLstm(const Node* node) {
 // ---- attention with a decaying state ----------------------------------------------------------------------------------
 // Pattern inputs: q, v, k; outputs: the last state [B, H, Dk, Dv], outs [T, B, H, Dv].  Tensor constant: decay [H, 1, 1].
 // Unlike the other regions this one does interpret its subgraph where the kernels do not fit the call (other types or devices, channels
-// beyond 128, decays outside [0, 1], inputs that require gradients): such a program ran before there was a kernel for it.
+// beyond 128, decays outside [0, 1], inputs that derivatives are asked of): such a program ran before there was a kernel for it.
 Operation makeDecayAttention(const Node* node) {
     const std::vector<at::Tensor> tc = node->ts(kAttrTParams);
     TORCH_CHECK(tc.size() == 1, "decay attention region: expected the decay constant, got ", tc.size());
@@ -515,7 +515,7 @@ Operation makeDecayAttention(const Node* node) {
         bool here = fits;
         for (const at::Tensor* t : {&q, &k, &v})
             here = here && t->is_cuda() && t->device() == q.device() && t->scalar_type() == at::kFloat && t->dim() == 4 &&
-                   !(t->requires_grad() && at::GradMode::is_enabled());
+                   !wantsDerivative(*t);
         here = here && q.size(2) == log_decay.size(0) && k.sizes() == q.sizes() && v.size(0) == q.size(0) && v.size(1) == q.size(1) &&
                v.size(2) == q.size(2) && q.size(3) >= 1 && q.size(3) <= 128 && v.size(3) >= 1 && v.size(3) <= 128;
         if (!here) {

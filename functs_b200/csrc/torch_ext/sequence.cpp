@@ -3,6 +3,7 @@
 #include <ATen/MemoryOverlap.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <cstring>
@@ -10,6 +11,10 @@
 #include "../../../include/functs_b200.h"
 
 namespace functs_b200 {
+
+bool carriesTangent(const at::Tensor& t) { return c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined(); }
+bool wantsDerivative(const at::Tensor& t) { return (t.requires_grad() && at::GradMode::is_enabled()) || carriesTangent(t) || !t.has_storage(); }
+
 namespace {
 
 int32_t dtypeOf(const at::Tensor& t, const char* name) {
@@ -29,6 +34,8 @@ void checkInput(const at::Tensor& t, const at::Device& device, at::ScalarType dt
     TORCH_CHECK_TYPE(t.scalar_type() == dtype, name, " must be ", dtype, ", got ", t.scalar_type());
     TORCH_CHECK_NOT_IMPLEMENTED(!(t.requires_grad() && at::GradMode::is_enabled()), name,
                                 " requires a gradient, and this operator has none: call it under torch.no_grad()");
+    TORCH_CHECK_NOT_IMPLEMENTED(!carriesTangent(t), name, " carries a tangent, and this operator has no derivative");
+    TORCH_CHECK_NOT_IMPLEMENTED(t.has_storage(), name, " is a tensor of a transform (torch.func), which this operator does not have");
 }
 void checkSizes(const at::Tensor& t, at::IntArrayRef sizes, const char* name) {
     TORCH_CHECK_VALUE(t.sizes() == sizes, name, " must be of sizes ", sizes, ", not ", t.sizes());

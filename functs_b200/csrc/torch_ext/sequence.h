@@ -11,6 +11,10 @@ namespace functs_b200 {
 
 using MaybeTensor = std::optional<at::Tensor>;
 
+// Whether a forward derivative is asked of what is made of `t`; whether any is, or a transform (torch.func) is on its way through.
+bool carriesTangent(const at::Tensor& t);
+bool wantsDerivative(const at::Tensor& t);
+
 // q [B, T, H, Dk], k [B, T, Hk, Dk], v [B, T, Hk, Dv] -> (out [B, T, H, Dv], the states)
 std::tuple<at::Tensor, at::Tensor> linearAttention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& log_decay,
                                                    double scale, const MaybeTensor& state, const MaybeTensor& slots,

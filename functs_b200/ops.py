@@ -296,7 +296,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     are new, [B, H, Dk, Dv].
     lengths int32 [B] (on the device; taken as 0 to T): a sequence ends there; its later rows are not read, and are zero in out.
     A token with a NaN or an infinity leaves the outputs before it alone; from it on they are not finite where the formula's are not
-    (an infinity of the formula may be a NaN).  No gradients: inputs that require one are refused.
+    (an infinity of the formula may be a NaN).  No derivatives: inputs that require a gradient or carry a tangent are refused.
     status (int32, on the device or pinned): also FB_STATUS_WAIT_TIMEOUT, should a wait inside the kernel run out; without it the next
     prompt on that device raises, whoever calls it: callers that share a device and have to know whose it was give a word each."""
     return _native()._linear_attention(q, k, v, log_decay, scale, state, slots, lengths, out, status)

@@ -800,3 +800,33 @@ def test_a_wait_that_ran_out_is_told_on_its_own_device(ops):
     ops.linear_attention(*(x.to("cuda:1") for x in (q, k, v, decays(2))))
     with pytest.raises(RuntimeError, match="wait ran out in an earlier call on cuda:0"):
         ops.linear_attention(q, k, v, decays(2))
+
+
+def test_inputs_that_carry_a_tangent(ops):
+    """Forward derivatives are refused, not lost; a built program runs step by step, so that the state keeps them (the immutable assignment of
+    `outs` has never had any)."""
+    import torch.autograd.forward_ad as fwd
+    from functs_b200 import jit, patterns
+    q, k, v = make(1, 70, 2, 2, 16, 16, F32)
+    g, state = decays(2), torch.zeros(1, 2, 16, 16, device="cuda")
+    x, ids = torch.randn(2, 2000, device="cuda"), torch.zeros(2, device="cuda", dtype=torch.int64)
+    decay = torch.full((2, 1, 1), 0.5, device="cuda")
+    program = patterns.DecayAttentionSeq(decay)
+    fn = jit.build(program)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for f in (lambda: ops.linear_attention(dual(q), k, v, g), lambda: ops.linear_attention(q, dual(k), v, g),
+                  lambda: ops.linear_attention(q, k, dual(v), g), lambda: ops.linear_attention(q, k, v, dual(g)),
+                  lambda: ops.linear_attention(q, k, v, g, state=dual(state)),
+                  lambda: ops.linear_attention_step(dual(q[:, 0]), k[:, 0], v[:, 0], g, state), lambda: ops.token_logprobs(dual(x), ids)):
+            with pytest.raises(NotImplementedError, match="tangent"):
+                f()
+        before = jit.interpreted_functor_runs()
+        q, k, v = q.transpose(0, 1), k.transpose(0, 1), v.transpose(0, 1)
+        outs, s = fn(q, dual(k), v)
+        assert jit.interpreted_functor_runs() > before
+        want = fwd.unpack_dual(program(q, dual(k), v)[1]).tangent
+        got = fwd.unpack_dual(s).tangent
+        assert got is not None and torch.allclose(got, want, atol=1e-4)
+    with pytest.raises(NotImplementedError, match="transform"):
+        torch.func.vmap(lambda y: ops.token_logprobs(y, ids)[0])(x[None])
