@@ -288,7 +288,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
 
     q [B, T, H, Dk], k [B, T, Hk, Dk], v [B, T, Hk, Dv] in float32, float16 or bfloat16, H a multiple of Hk (heads share keys and
     values in groups), up to 128 channels; any strides with adjacent channels (others are copied), so views of one fused
-    projection and time-major tensors go in as they are.  log_decay float32 [H].  Returns (out [B, T, H, Dv], states).
+    projection and time-major tensors go in as they are.  log_decay float32 [H]: 0 keeps,
+    -inf forgets at once, above 0 the state grows; a NaN makes its head NaN.  Returns (out [B, T, H, Dv], states).
 
     state: float32 [N, H, Dk, Dv], contiguous, read and updated in place: sequence b's is state[slots[b]] (slots int32 [B]), or state[b]
     without slots.  A negative slot is no sequence (zero rows in out).  So is one of N or above, or one that an earlier sequence has

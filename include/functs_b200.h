@@ -255,7 +255,7 @@ int functs_b200_lstm_forward_mode(const float* x, const float* w_ih, const float
 /* The loop  for t < tokens: S = exp(log_decay[h]) * S + k[t] v[t]^T;  out[t] = scale * S^T q[t]  for every sequence b and head h, S being a
  * [dk, dv] matrix in fp32.  q [batch, tokens, heads, dk], k [.., kv_heads, dk], v [.., kv_heads, dv], out [.., heads, dv]: elements of
  * `dtype`, channels adjacent, the other strides free; head h reads key and value head h / (heads / kv_heads).  1 <= dk, dv <= 128.
- * log_decay [heads] fp32 (0 or less; -inf forgets at once).
+ * log_decay [heads] fp32 (-inf forgets at once, above 0 the state grows, a NaN makes its head NaN).
  * Sequence b starts from state_in and leaves its last state in state_out, both [num_slots, heads, dk, dv] fp32 (the same memory if the
  * caller likes); state_in = NULL starts from zero.  slots (optional, int32 [batch]) says which of them is sequence b's, else it is b and
  * num_slots = batch.  A negative slot is no sequence: its rows of out are zero, and no state is touched.  So is, with a status bit, one

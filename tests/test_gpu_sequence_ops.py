@@ -830,3 +830,16 @@ def test_inputs_that_carry_a_tangent(ops):
         assert got is not None and torch.allclose(got, want, atol=1e-4)
     with pytest.raises(NotImplementedError, match="transform"):
         torch.func.vmap(lambda y: ops.token_logprobs(y, ids)[0])(x[None])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("tokens,d", [(1, 64), (6, 64), (150, 128), (2048, 64)])
+def test_decays_above_zero(ops, tokens, d, dtype):
+    """States that grow: the same formula, and the same bounds."""
+    g = torch.tensor([2.0 ** -9, 0.02 if tokens < 1000 else 0.004], device="cuda")
+    q, k, v = make(2, tokens, 2, 2, d, d, dtype)
+    q = q * 2.0 ** -8  # (that the outputs stay within fp16)
+    start = torch.randn(2, 2, d, d, device="cuda")
+    want = recurrence(q, k, v, g, 0.1, start, torch.full((2,), tokens, device="cuda"))
+    out, state = ops.linear_attention(q, k, v, g, scale=0.1, state=start)
+    check_attention(out, state, want, dtype, tokens, d)
