@@ -1,12 +1,13 @@
 #include "sequence.h"
 
-#include <ATen/MemoryOverlap.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <algorithm>
 #include <cstring>
+#include <vector>
 
 #include "../../../include/functs_b200.h"
 
@@ -154,8 +155,6 @@ void checkAttention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& 
         TORCH_CHECK_VALUE(state->dim() == 4 && state->size(1) == H && state->size(2) == Dk && state->size(3) == Dv && state->is_contiguous(),
                           "state must be a contiguous [slots, ", H, ", ", Dk, ", ", Dv, "] tensor");
         TORCH_CHECK_VALUE(slots.has_value() || state->size(0) == B, "without slots, state must hold ", B, " states");
-        TORCH_CHECK_VALUE(!state->is_alias_of(q) && !state->is_alias_of(k) && !state->is_alias_of(v) && !state->is_alias_of(log_decay),
-                          "state must not share memory with the inputs");
     } else {
         TORCH_CHECK_VALUE(!slots.has_value(), "slots name rows of a state: give one");
     }
@@ -169,16 +168,52 @@ void checkAttention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& 
     }
 }
 
-at::Tensor output(const MaybeTensor& out, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor* state) {
+// Whether the memory from the first element of one to its last lies apart from the other's.
+bool apart(const at::Tensor& a, const at::Tensor& b) {
+    if (a.numel() == 0 || b.numel() == 0) return true;
+    const auto end = [](const at::Tensor& t) {
+        int64_t last = 0;
+        for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+        return reinterpret_cast<uintptr_t>(t.data_ptr()) + (last + 1) * t.element_size();
+    };
+    return end(a) <= reinterpret_cast<uintptr_t>(b.data_ptr()) || end(b) <= reinterpret_cast<uintptr_t>(a.data_ptr());
+}
+
+// Whether no two elements of `t` can be the same: every stride steps over all that the smaller ones reach.
+bool elementsApart(const at::Tensor& t) {
+    std::vector<std::pair<int64_t, int64_t>> by_stride;
+    for (int64_t d = 0; d < t.dim(); ++d)
+        if (t.size(d) > 1) by_stride.emplace_back(t.stride(d), t.size(d));
+    std::sort(by_stride.begin(), by_stride.end());
+    int64_t reach = 0;
+    for (const auto& [stride, size] : by_stride) {
+        if (stride <= reach) return false;
+        reach += (size - 1) * stride;
+    }
+    return true;
+}
+
+// What is written (the output, a given state) lies apart from all that is read while it is, and from one another.
+void checkWritten(const at::Tensor* out, const at::Tensor* state, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                  const at::Tensor& log_decay, const MaybeTensor& slots, const MaybeTensor& lengths, const MaybeTensor& status) {
+    std::vector<const at::Tensor*> others{&q, &k, &v, &log_decay};
+    for (const MaybeTensor* t : {&slots, &lengths, &status})
+        if (t->has_value()) others.push_back(&**t);
+    for (const at::Tensor* t : others) {
+        TORCH_CHECK_VALUE(state == nullptr || apart(*state, *t), "state must not share memory with the inputs");
+        TORCH_CHECK_VALUE(out == nullptr || apart(*out, *t), "out must not share memory with the inputs (from its first element to its last)");
+    }
+    TORCH_CHECK_VALUE(out == nullptr || state == nullptr || apart(*out, *state), "out must not share memory with the state");
+}
+
+at::Tensor output(const MaybeTensor& out, const at::Tensor& q, const at::Tensor& v) {
     std::vector<int64_t> sizes = q.sizes().vec();
     sizes.back() = v.size(-1);
     if (!out.has_value()) return at::empty(sizes, q.options());
     checkInput(*out, q.device(), q.scalar_type(), "out");
     checkSizes(*out, sizes, "out");
     TORCH_CHECK_VALUE(out->size(-1) == 1 || out->stride(-1) == 1, "out must have adjacent channels");
-    TORCH_CHECK_VALUE(at::has_internal_overlap(*out) != at::MemOverlap::Yes, "out must not overlap itself");
-    TORCH_CHECK_VALUE(!out->is_alias_of(q) && !out->is_alias_of(k) && !out->is_alias_of(v) && (state == nullptr || !out->is_alias_of(*state)),
-                      "out must not share memory with the inputs");
+    TORCH_CHECK_VALUE(elementsApart(*out), "out must not overlap itself");
     return *out;
 }
 
@@ -190,7 +225,8 @@ std::tuple<at::Tensor, at::Tensor> linearAttention(const at::Tensor& q, const at
     const at::Tensor* given = state.has_value() ? &*state : nullptr;
     checkAttention(q, k, v, log_decay, given, slots, lengths, 4);
     c10::cuda::CUDAGuard guard(q.device());
-    const at::Tensor o = output(out, q, k, v, given);
+    const at::Tensor o = output(out, q, v);
+    checkWritten(out.has_value() ? &o : nullptr, given, q, k, v, log_decay, slots, lengths, status);
     const at::Tensor s = given != nullptr ? *given : at::empty({q.size(0), q.size(2), q.size(3), v.size(3)}, q.options().dtype(at::kFloat));
     run(q, k, v, log_decay, scale, s, given == nullptr, slots, lengths, o, status, q.size(1));
     return {o, s};
@@ -201,7 +237,8 @@ at::Tensor linearAttentionStep(const at::Tensor& q, const at::Tensor& k, const a
                                const MaybeTensor& status) {
     checkAttention(q, k, v, log_decay, &state, slots, std::nullopt, 3);
     c10::cuda::CUDAGuard guard(q.device());
-    const at::Tensor o = output(out, q, k, v, &state);
+    const at::Tensor o = output(out, q, v);
+    checkWritten(out.has_value() ? &o : nullptr, &state, q, k, v, log_decay, slots, std::nullopt, status);
     run(q, k, v, log_decay, scale, state, false, slots, std::nullopt, o, status, 1);
     return o;
 }

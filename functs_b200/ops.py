@@ -296,6 +296,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     already, and `status` gets the bit that raise_on_status reports.  Without state, sequences start from zero and the states returned
     are new, [B, H, Dk, Dv].
     lengths int32 [B] (on the device; taken as 0 to T): a sequence ends there; its later rows are not read, and are zero in out.
+    out (with adjacent channels) and state lie apart from all other tensors of the call: a slice of one buffer is fine, rows that take turns
+    with an input's in memory are refused.
     A token with a NaN or an infinity leaves the outputs before it alone; from it on they are not finite where the formula's are not
     (an infinity of the formula may be a NaN).  No derivatives: inputs that require a gradient or carry a tangent are refused.
     status (int32, on the device or pinned): also FB_STATUS_WAIT_TIMEOUT, should a wait inside the kernel run out; without it the next

@@ -843,3 +843,42 @@ def test_decays_above_zero(ops, tokens, d, dtype):
     want = recurrence(q, k, v, g, 0.1, start, torch.full((2,), tokens, device="cuda"))
     out, state = ops.linear_attention(q, k, v, g, scale=0.1, state=start)
     check_attention(out, state, want, dtype, tokens, d)
+
+
+@pytest.mark.parametrize("tokens", [1, 5, 150])
+def test_tensors_that_are_slices_of_one_buffer(ops, tokens):
+    """out and state may lie in one workspace with the inputs, beside them; where they share an element with anything that is read, or out one
+    with itself, the call is refused."""
+    b, h, d = 2, 2, 16
+    n, states = b * tokens * h * d, b * h * d * d
+    room = torch.zeros(4 * n + states + 64, device="cuda")
+    q, k, v, out = (room[i * n:(i + 1) * n].view(b, tokens, h, d) for i in range(4))
+    state = room[4 * n:4 * n + states].view(b, h, d, d)
+    rest = room[4 * n + states:]
+    g, slots, lengths, status = rest[:2], rest[2:4].view(torch.int32), rest[4:6].view(torch.int32), rest[6:7].view(torch.int32)
+    for x in (q, k, v):
+        x.normal_()
+    g.copy_(decays(h))
+    slots.copy_(torch.tensor([1, 0]))
+    lengths.fill_(tokens)
+    want = ops.linear_attention(q.clone(), k.clone(), v.clone(), decays(h), state=state.clone(), slots=slots.clone())
+    got = ops.linear_attention(q, k, v, g, state=state, slots=slots, lengths=lengths, out=out, status=status)
+    assert torch.equal(got[0], want[0]) and torch.equal(state, want[1]) and int(status) == 0
+    whole = torch.zeros(n + 64, device="cuda")
+    front, behind = whole[:n].view(b, tokens, h, d), whole[n - 2:n]
+    with pytest.raises(ValueError, match="out must not share memory with the inputs"):
+        ops.linear_attention(q, k, v, behind, out=front)
+    for name in ("slots", "lengths"):
+        given = {"slots": slots, "lengths": lengths, name: behind.view(torch.int32)}
+        with pytest.raises(ValueError, match="out must not share memory with the inputs"):
+            ops.linear_attention(q, k, v, g, state=state, out=front, **given)
+        given[name] = state.view(-1)[:2].view(torch.int32)
+        with pytest.raises(ValueError, match="state must not share memory with the inputs"):
+            ops.linear_attention(q, k, v, g, state=state, **given)
+    with pytest.raises(ValueError, match="out must not share memory with the state"):
+        both = torch.zeros(n + states, device="cuda")
+        ops.linear_attention(q, k, v, g, state=both[:states].view(b, h, d, d), out=both[states - 1:states - 1 + n].view(b, tokens, h, d))
+    if tokens > 1:
+        with pytest.raises(ValueError, match="overlap itself"):
+            ops.linear_attention(q, k, v, g, out=torch.zeros(2 * n, device="cuda").as_strided((b, tokens, h, d), (tokens * h * d - 1, h * d, d, 1)))
+    torch.cuda.synchronize()
