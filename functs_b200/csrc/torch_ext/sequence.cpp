@@ -76,7 +76,9 @@ int32_t* statusWord(const MaybeTensor& status, const at::Device& device, bool ow
     return status->data_ptr<int32_t>();
 }
 
-at::Tensor channelsAdjacent(const at::Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+// (a view that negates when it is read, as of a conjugate's imaginary part, is written out)
+at::Tensor channelsAdjacent(const at::Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t.resolve_neg() : t.contiguous().resolve_neg(); }
+at::Tensor packed(const at::Tensor& t) { return t.contiguous().resolve_neg(); }
 
 int32_t narrow(int64_t n, const char* what) {
     TORCH_CHECK_VALUE(n <= INT32_MAX, what, " (", n, ") is too large");
@@ -100,7 +102,7 @@ void run(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at
          bool fresh, const MaybeTensor& slots, const MaybeTensor& lengths, const at::Tensor& out, const MaybeTensor& status, int64_t tokens) {
     const int64_t B = q.size(0), H = q.size(-2);
     const at::Device device = q.device();
-    const at::Tensor qc = channelsAdjacent(q), kc = channelsAdjacent(k), vc = channelsAdjacent(v), decay = log_decay.contiguous();
+    const at::Tensor qc = channelsAdjacent(q), kc = channelsAdjacent(k), vc = channelsAdjacent(v), decay = packed(log_decay);
     functs_b200_linear_attention_args a = {};
     a.dtype = dtypeOf(q, "q");
     a.batch = narrow(B, "batch");
@@ -117,11 +119,11 @@ void run(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at
     a.state_out = state.data_ptr<float>();
     at::Tensor slots_c, lengths_c;
     if (slots.has_value()) {
-        slots_c = slots->contiguous();
+        slots_c = packed(*slots);
         a.slots = slots_c.data_ptr<int32_t>();
     }
     if (lengths.has_value()) {
-        lengths_c = lengths->contiguous();
+        lengths_c = packed(*lengths);
         a.lengths = lengths_c.data_ptr<int32_t>();
     }
     a.status = statusWord(status, device, /*own=*/tokens > 1);
@@ -152,6 +154,7 @@ void checkAttention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& 
     checkSizes(log_decay, {H}, "log_decay");
     if (state != nullptr) {
         checkInput(*state, device, at::kFloat, "state");
+        TORCH_CHECK_VALUE(!state->is_neg(), "state must not be a negated view");
         TORCH_CHECK_VALUE(state->dim() == 4 && state->size(1) == H && state->size(2) == Dk && state->size(3) == Dv && state->is_contiguous(),
                           "state must be a contiguous [slots, ", H, ", ", Dk, ", ", Dv, "] tensor");
         TORCH_CHECK_VALUE(slots.has_value() || state->size(0) == B, "without slots, state must hold ", B, " states");
@@ -211,6 +214,7 @@ at::Tensor output(const MaybeTensor& out, const at::Tensor& q, const at::Tensor&
     sizes.back() = v.size(-1);
     if (!out.has_value()) return at::empty(sizes, q.options());
     checkInput(*out, q.device(), q.scalar_type(), "out");
+    TORCH_CHECK_VALUE(!out->is_neg(), "out must not be a negated view");
     checkSizes(*out, sizes, "out");
     TORCH_CHECK_VALUE(out->size(-1) == 1 || out->stride(-1) == 1, "out must have adjacent channels");
     TORCH_CHECK_VALUE(elementsApart(*out), "out must not overlap itself");
@@ -255,7 +259,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> tokenLogprobs(const a
     TORCH_CHECK_VALUE(top >= 0 && top <= FB_LOGPROBS_MAX_TOP && top <= V, "top must be 0 to ", FB_LOGPROBS_MAX_TOP, " and at most the vocabulary (", V,
                       "), got ", top);
     c10::cuda::CUDAGuard guard(device);
-    const at::Tensor x = channelsAdjacent(logits), ids = tokens.contiguous();
+    const at::Tensor x = channelsAdjacent(logits), ids = packed(tokens);
     const auto f32 = logits.options().dtype(at::kFloat);
     at::Tensor lp = at::empty({R}, f32), entropy = at::empty({R}, f32), top_lp = at::empty({R, top}, f32),
                top_ids = at::empty({R, top}, f32.dtype(at::kLong));

@@ -882,3 +882,24 @@ def test_tensors_that_are_slices_of_one_buffer(ops, tokens):
         with pytest.raises(ValueError, match="overlap itself"):
             ops.linear_attention(q, k, v, g, out=torch.zeros(2 * n, device="cuda").as_strided((b, tokens, h, d), (tokens * h * d - 1, h * d, d, 1)))
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("tokens", [1, 100])
+def test_views_that_negate(ops, tokens):
+    """A tensor whose values are the negatives of its memory's (as the imaginary part of a conjugate is)."""
+    q, k, v = make(2, tokens, 2, 2, 16, 16, F32)
+    g, state = decays(2), torch.zeros(2, 2, 16, 16, device="cuda")
+    neg = torch._neg_view
+    want = ops.linear_attention(-q, -k, v, g)
+    got = ops.linear_attention(neg(q), neg(k), v, neg(-g))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    x = torch.complex(torch.randn(3, 3000, device="cuda"), torch.randn(3, 3000, device="cuda"))
+    ids = torch.tensor([5, 1, 2999], device="cuda")
+    for view in (x.conj().imag, neg(x.real.contiguous())):
+        assert view.is_neg()
+        for a, b in zip(ops.token_logprobs(view, neg(-ids), top=3), ops.token_logprobs(view.clone().resolve_neg(), ids, top=3)):
+            assert torch.equal(a, b)
+    with pytest.raises(ValueError, match="state must not be a negated view"):
+        ops.linear_attention(q, k, v, g, state=neg(state))
+    with pytest.raises(ValueError, match="out must not be a negated view"):
+        ops.linear_attention(q, k, v, g, out=neg(torch.zeros_like(q)))
