@@ -171,6 +171,11 @@ void checkAttention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& 
     }
 }
 
+// A kernel has written `t`: autograd, which may have saved it for a backward pass, has to know.
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // Whether the memory from the first element of one to its last lies apart from the other's.
 bool apart(const at::Tensor& a, const at::Tensor& b) {
     if (a.numel() == 0 || b.numel() == 0) return true;
@@ -233,6 +238,8 @@ std::tuple<at::Tensor, at::Tensor> linearAttention(const at::Tensor& q, const at
     checkWritten(out.has_value() ? &o : nullptr, given, q, k, v, log_decay, slots, lengths, status);
     const at::Tensor s = given != nullptr ? *given : at::empty({q.size(0), q.size(2), q.size(3), v.size(3)}, q.options().dtype(at::kFloat));
     run(q, k, v, log_decay, scale, s, given == nullptr, slots, lengths, o, status, q.size(1));
+    if (given != nullptr) written(s);
+    if (out.has_value()) written(o);
     return {o, s};
 }
 
@@ -244,6 +251,8 @@ at::Tensor linearAttentionStep(const at::Tensor& q, const at::Tensor& k, const a
     const at::Tensor o = output(out, q, v);
     checkWritten(out.has_value() ? &o : nullptr, &state, q, k, v, log_decay, slots, std::nullopt, status);
     run(q, k, v, log_decay, scale, state, false, slots, std::nullopt, o, status, 1);
+    written(state);
+    if (out.has_value()) written(o);
     return o;
 }
 

@@ -903,3 +903,24 @@ def test_views_that_negate(ops, tokens):
         ops.linear_attention(q, k, v, g, state=neg(state))
     with pytest.raises(ValueError, match="out must not be a negated view"):
         ops.linear_attention(q, k, v, g, out=neg(torch.zeros_like(q)))
+
+
+def test_tensors_that_autograd_has_saved_and_a_call_writes(ops):
+    """A backward pass through a state or an output that a later call wrote over is refused by autograd, as behind any in-place operator."""
+    q, k, v = make(1, 3, 2, 2, 16, 16, F32)
+    w = torch.ones(1, device="cuda", requires_grad=True)
+    for tokens in (3, 1):
+        for which in ("state", "out"):
+            state, out = torch.ones(1, 2, 16, 16, device="cuda"), torch.ones(1, 3, 2, 16, device="cuda")
+            loss = (w * (state if which == "state" else out)).sum()
+            if tokens == 1:
+                ops.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], decays(2), state, out=out[:, 0])
+            else:
+                ops.linear_attention(q, k, v, decays(2), state=state, out=out)
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                loss.backward()
+    with torch.inference_mode():
+        state = torch.zeros(1, 2, 16, 16, device="cuda")
+    ops.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], decays(2), state)
+    with torch.inference_mode():
+        ops.linear_attention(q, k, v, decays(2), state=state)
