@@ -268,6 +268,11 @@ extern "C" int functs_b200_linear_attention(const functs_b200_linear_attention_a
     if (a.batch == 0) return FB_OK;
     FB_REQUIRE(a.log_decay != nullptr && a.state_out != nullptr, "linear_attention: null pointer");
     FB_REQUIRE(a.tokens == 0 || (a.q != nullptr && a.k != nullptr && a.v != nullptr && a.out != nullptr), "linear_attention: null pointer");
+    const uintptr_t elements = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
+                               reinterpret_cast<uintptr_t>(a.out);
+    const uintptr_t words = reinterpret_cast<uintptr_t>(a.log_decay) | reinterpret_cast<uintptr_t>(a.state_in) | reinterpret_cast<uintptr_t>(a.state_out) |
+                            reinterpret_cast<uintptr_t>(a.slots) | reinterpret_cast<uintptr_t>(a.lengths) | reinterpret_cast<uintptr_t>(a.status);
+    FB_REQUIRE(elements % (a.dtype == FB_DTYPE_F32 ? 4 : 2) == 0 && words % 4 == 0, "linear_attention: pointers must lie on a boundary of their type");
     const cudaStream_t st = as_stream(stream);
     if (lin_by_chunks(a)) return launch_linattn_chunk(a, scratch, st);
     if (a.dtype == FB_DTYPE_F32) return launch_recurrent<float>(a, st);

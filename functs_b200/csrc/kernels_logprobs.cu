@@ -676,6 +676,10 @@ extern "C" int functs_b200_token_logprobs(const void* logits, int32_t dtype, int
     FB_REQUIRE(logits != nullptr && tokens != nullptr && logprobs != nullptr && entropy != nullptr, "token_logprobs: null pointer");
     FB_REQUIRE(top == 0 || (top_logprobs != nullptr && top_ids != nullptr), "token_logprobs: null pointer");
     FB_REQUIRE(reinterpret_cast<uintptr_t>(logits) % (dtype == FB_DTYPE_F32 ? 4 : 2) == 0, "token_logprobs: logits must lie on a boundary of their type");
+    const uintptr_t words = reinterpret_cast<uintptr_t>(logprobs) | reinterpret_cast<uintptr_t>(entropy) | reinterpret_cast<uintptr_t>(top_logprobs) |
+                            reinterpret_cast<uintptr_t>(status);
+    FB_REQUIRE(words % 4 == 0 && (reinterpret_cast<uintptr_t>(tokens) | reinterpret_cast<uintptr_t>(top_ids)) % 8 == 0,
+               "token_logprobs: pointers must lie on a boundary of their type");
     const LpArgs a = {logits, row_stride, tokens, vocab, top, logprobs, entropy, top_logprobs, top_ids, status};
     const cudaStream_t st = as_stream(stream);
     if (dtype == FB_DTYPE_F32) return launch_logprobs<float>(a, rows, st);

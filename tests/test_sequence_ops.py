@@ -93,3 +93,20 @@ def test_another_update_does_not_match():
     from functs_b200 import jit
     f = jit.build(OtherUpdate(torch.rand(4, 1, 1)))
     assert "decay_attention_seq" not in jit.functor_regions(f.graph)
+
+
+@pytest.mark.parametrize("dtype,over", [(2, {n: 4097}) for n in ("q", "k", "v", "out")] + [(0, {n: 4098}) for n in ("q", "k", "v", "out")] +
+                         [(1, {n: 4098}) for n in ("log_decay", "state_in", "state_out", "slots", "lengths", "status")])
+def test_linear_attention_pointers_off_their_boundary(dtype, over):
+    from functs_b200 import _lib
+    assert _lib.lib.functs_b200_linear_attention(ctypes.byref(args(dtype=dtype, **over)), None, None) == -1
+    assert "boundary" in _lib.last_error()
+
+
+@pytest.mark.parametrize("at,value", [(3, 4100), (7, 4098), (8, 4098), (9, 4098), (10, 4100), (11, 4098)])
+def test_token_logprobs_pointers_off_their_boundary(at, value):
+    from functs_b200 import _lib
+    a = [4096, 2, 10, 4096, 1, 10, 5, 4096, 4096, 4096, 4096, None, None]
+    a[at] = value
+    assert _lib.lib.functs_b200_token_logprobs(*a) == -1
+    assert "boundary" in _lib.last_error()
