@@ -1,9 +1,12 @@
 // Log probabilities of given tokens, entropies and the best alternatives: one pass over the logits.
 //
-//   With any reference c_ref near the row's maximum m (in powers of two: y = x log2 e),  s = sum 2^(y - c_ref)  and
-//   t = sum 2^(y - c_ref) (y - c_ref)  give  log sum exp(x) = ln2 c_ref + ln s  and  entropy = ln s - ln2 t / s.
-// Every thread takes the maximum of its first elements as its reference and changes it only where an element lies 2^80 above it, so that
-// the loop is a fused multiply-add, an exponential and two sums per element; partial sums meet at the row's maximum at the end.
+//   With the row's maximum m,  s = sum 2^d  and  t = sum 2^d d  with  d = (x - m) log2 e  give  log sum exp(x) = m + ln s  and
+//   entropy = ln s - ln2 t / s.
+// Every thread takes the largest element that it has met as its reference, so that d is small where 2^d is large (an exponent of 40 is off by
+// 2^-20: a row whose best lies that far above the others and above its thread's reference came out 2.7e-6 off, above 0).  That element itself
+// stays out of the sums: in them it would round the small ones away, and against the row's maximum its own power is exact, 1 where it is
+// the maximum.  So s >= 1 and t <= 0, no log probability is above 0 and no entropy below.  A thread looks for a larger element once in four
+// vectors; the loop is a fused multiply-add, an exponential and two sums per element.
 //
 // Alternatives: each thread also keeps the maximum of its elements.  The top-th largest of some of those maxima (the largest of every warp)
 // bounds the top-th largest element from below, so only the few threads whose maximum reaches it have candidates: their elements are read
@@ -29,9 +32,9 @@ constexpr int kLpTopParts = 4;               // the same with alternatives
 constexpr int kLpList = 1024;                // candidates above the bound; as many equal to it
 constexpr int kLpBusy = 128;                 // threads whose elements are looked through one by one
 constexpr float kLpLog2e = 1.44269504088896340736f;
-constexpr float kLpFloor = -5e8f;            // the lowest reference: what lies more below it than a power can say counts as nothing there
+constexpr double kLpLog2eOff = 1.0 / static_cast<double>(kLpLog2e) - 0.69314718055994530942;  // what rounding log2 e takes from ln 2
+constexpr float kLpFloor = -3.4e8f;          // stands for no element: the sums of what lies below it are taken by lp_again
 constexpr float kLpFarValue = 268435456.0f;  // 2^28: where x log2e is rounded by 16 and more, see lp_again
-constexpr float kLpFar = 80.0f;              // how far above its reference, in powers of two, a thread's sums may grow
 
 struct LpArgs {
     const void* logits;
@@ -55,7 +58,7 @@ __device__ __forceinline__ float lp_value(uint32_t order) {
 }
 __device__ __forceinline__ uint64_t lp_key(uint32_t order, uint32_t id) { return (static_cast<uint64_t>(order) << 32) | (0xFFFFFFFFu - id); }
 
-__device__ __forceinline__ float lp_ex2(float x) {
+__device__ __forceinline__ float lp_ex2(float x) {  // (of 0 exactly 1)
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
@@ -70,6 +73,14 @@ struct LpVec<float> {
         x[0] = __uint_as_float(u.x), x[1] = __uint_as_float(u.y), x[2] = __uint_as_float(u.z), x[3] = __uint_as_float(u.w);
     }
     static __device__ __forceinline__ float one(const float* p) { return *p; }
+    template <int K>
+    static __device__ __forceinline__ float most(const uint4 (&u)[K]) {
+        float m = __uint_as_float(u[0].x);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            m = max_nan(max_nan(m, max_nan(__uint_as_float(u[k].x), __uint_as_float(u[k].y))), max_nan(__uint_as_float(u[k].z), __uint_as_float(u[k].w)));
+        return m;
+    }
 };
 template <>
 struct LpVec<__nv_bfloat16> {
@@ -83,6 +94,14 @@ struct LpVec<__nv_bfloat16> {
         }
     }
     static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+    template <int K>
+    static __device__ __forceinline__ float most(const uint4 (&u)[K]) {
+        const auto two = [](const uint32_t& w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+        __nv_bfloat162 m = two(u[0].x);
+#pragma unroll
+        for (int k = 0; k < K; ++k) m = __hmax2_nan(__hmax2_nan(m, __hmax2_nan(two(u[k].x), two(u[k].y))), __hmax2_nan(two(u[k].z), two(u[k].w)));
+        return max_nan(__low2float(m), __high2float(m));
+    }
 };
 template <>
 struct LpVec<__half> {
@@ -97,33 +116,25 @@ struct LpVec<__half> {
         }
     }
     static __device__ __forceinline__ float one(const __half* p) { return __half2float(*p); }
+    template <int K>
+    static __device__ __forceinline__ float most(const uint4 (&u)[K]) {
+        const auto two = [](const uint32_t& w) { return *reinterpret_cast<const __half2*>(&w); };
+        __half2 m = two(u[0].x);
+#pragma unroll
+        for (int k = 0; k < K; ++k) m = __hmax2_nan(__hmax2_nan(m, __hmax2_nan(two(u[k].x), two(u[k].y))), __hmax2_nan(two(u[k].z), two(u[k].w)));
+        return max_nan(__low2float(m), __high2float(m));
+    }
 };
 
-// sums of one thread, one warp, one part of a row
+// sums of a warp, of a part of a row, of a row: against its own largest element
 struct __align__(16) LpSums {
-    float most;  // the largest element (NaN if there is one)
-    float ref;   // reference, in powers of two
+    float most;  // the largest element (NaN if there is one, -inf if there is none)
     float s, t;
+    __device__ __forceinline__ void none() { most = __int_as_float(0xff800000), s = t = 0.0f; }
 };
-
-// takes `o` into `a`, at the larger of the two references
-__device__ __forceinline__ void lp_join(LpSums& a, const LpSums& o) {
-    const float ref = fmaxf(a.ref, o.ref);
-    const float da = a.ref - ref, db = o.ref - ref;  // one of them is 0
-    const float fa = lp_ex2(da), fb_ = lp_ex2(db);
-    // (a reference at the floor has no sums, and its distance must not meet them)
-    a.t = fa * fmaf(da, fa > 0.0f ? a.s : 0.0f, a.t) + fb_ * fmaf(db, fb_ > 0.0f ? o.s : 0.0f, o.t);
-    a.s = fa * a.s + fb_ * o.s;
-    a.ref = ref;
-    a.most = max_nan(a.most, o.most);
-}
 
 // Whether sums against a rounded x log2e do not do for this largest element (finite, and far from 0).
 __device__ __forceinline__ bool lp_far(float most) { return fabsf(most) >= kLpFarValue && fabsf(most) <= 3.402823466e38f; }
-// what `ref` stands for, in powers of two; far from 0 sums are taken against the largest element itself (both factors exact in 64 bits)
-__device__ __forceinline__ double lp_ref(const LpSums& sums) {
-    return lp_far(sums.most) ? static_cast<double>(sums.most) * static_cast<double>(kLpLog2e) : static_cast<double>(sums.ref);
-}
 // elements against the largest one, by a difference that is exact where it matters
 template <int N>
 __device__ __forceinline__ void lp_take_near(const float (&x)[N], float most, float& s, float& t) {
@@ -145,29 +156,74 @@ struct LpRow {
 };
 
 struct LpThread {
-    LpSums sums;
+    float most;       // the largest element (NaN if there is one)
+    float held, ref;  // the largest above the floor, which is not in the sums, and the reference that they are against: held log2e, rounded
+    float s, t;
 
-    __device__ __forceinline__ void start() { sums = {__int_as_float(0xff800000), kLpFloor, 0.0f, 0.0f}; }
-    __device__ __forceinline__ void raise(float x) {  // the reference, to x
-        const float to = x * kLpLog2e, d = sums.ref - to, f = lp_ex2(d);
-        sums.t = f > 0.0f ? f * fmaf(d, sums.s, sums.t) : 0.0f;
-        sums.s = f * sums.s;
-        sums.ref = to;
+    __device__ __forceinline__ void start() { most = __int_as_float(0xff800000), held = kLpFloor, ref = kLpFloor * kLpLog2e, s = t = 0.0f; }
+    // x is the one to hold, and what was held goes into the sums
+    __device__ __forceinline__ void hold(float x) {
+        const float own = fmaf(held, kLpLog2e, -ref), e = lp_ex2(own), to = x * kLpLog2e, d = ref - to, f = lp_ex2(d);
+        s += e;
+        t = fmaf(e, own, t);
+        t = f > 0.0f ? f * fmaf(d, s, t) : 0.0f;  // (so far below that nothing of them is left: they need not be numbers)
+        s = f > 0.0f ? f * s : 0.0f;
+        held = x, ref = to;
     }
-    template <int N>
-    __device__ __forceinline__ void take(const float (&x)[N]) {
-        float m = x[0];
-#pragma unroll
-        for (int i = 1; i < N; ++i) m = max_nan(m, x[i]);
-        sums.most = max_nan(sums.most, m);
-        if (fmaf(m, kLpLog2e, -sums.ref) > kLpFar) raise(m);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float d = max_nan(fmaf(x[i], kLpLog2e, -sums.ref), -1000.0f);  // (-inf: its power is 0, and 0 * d must be)
-            const float e = lp_ex2(d);
-            sums.s += e;
-            sums.t = fmaf(e, d, sums.t);
+    // The elements of K vectors (get(k, x) gives one), of which `m` is the largest.
+    template <int N, int K, class F>
+    __device__ __forceinline__ void take(float m, F get) {
+        most = max_nan(most, m);
+        float own = 0.0f, own_t = 0.0f;
+        if (m > held) {
+            hold(m);
+            const float d = fmaf(m, kLpLog2e, -ref);
+            own = lp_ex2(d), own_t = own * d;
         }
+        float sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            float x[N];
+            get(k, x);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float d = fmaxf(fmaf(x[i], kLpLog2e, -ref), -1000.0f);  // (-inf: its power is 0, and 0 * d must be; a NaN is in `most`)
+                x[i] = lp_ex2(d);
+                t = fmaf(x[i], d, t);
+            }
+#pragma unroll
+            for (int w = N / 2; w > 0; w /= 2) {  // (by halves: `own` is among them, and rounds the others three times instead of seven)
+#pragma unroll
+                for (int i = 0; i < w; ++i) x[i] += x[i + w];
+            }
+            sum += x[0];
+        }
+        s += sum - own;
+        t -= own_t;
+    }
+    __device__ __forceinline__ void take_one(float x) {
+        take<1, 1>(x, [&](int, float (&y)[1]) { y[0] = x; });
+    }
+    template <class V, int K>
+    __device__ __forceinline__ void take_vectors(const uint4 (&u)[K]) {
+        take<V::N, K>(V::most(u), [&](int k, float (&x)[V::N]) { V::get(u[k], x); });
+    }
+    // The warp's sums, in all lanes.  (Where its largest element is far from 0 they mean nothing: lp_again takes them.)
+    __device__ __forceinline__ LpSums warp_sums() const {
+        LpSums all;
+        all.most = most;
+        for (int d = 16; d > 0; d /= 2) all.most = max_nan(all.most, __shfl_xor_sync(kFullMask, all.most, d));
+        all.s = all.t = 0.0f;
+        if (held > kLpFloor) {
+            const float d = fmaxf((held - all.most) * kLpLog2e, -1000.0f), below = fmaf(-all.most, kLpLog2e, ref), f = lp_ex2(below), rest = fmaxf(s, 0.0f);
+            all.s = lp_ex2(d), all.t = all.s * d;
+            if (f > 0.0f) all.s = fmaf(f, rest, all.s), all.t += fminf(f * fmaf(below, rest, t), 0.0f);
+        }
+        for (int d = 16; d > 0; d /= 2) {
+            all.s += __shfl_xor_sync(kFullMask, all.s, d);
+            all.t += __shfl_xor_sync(kFullMask, all.t, d);
+        }
+        return all;
     }
 };
 
@@ -181,6 +237,8 @@ struct LpShared {
     uint64_t parts_best[TOP ? kLpTopParts * kLpMaxTop : 1];  // of the row's CTAs (in the first one)
     uint64_t row_best[kLpMaxTop];             // the row's
     LpRow whole;
+    int64_t token;                            // the token to score and its logit, fetched at the start (registers that the loop needs)
+    float token_logit;
     uint32_t hist[256];
     uint32_t warp_count[kLpMaxThreads / 32];
     int busy[kLpBusy];                        // threads that have candidates
@@ -200,18 +258,21 @@ __device__ __forceinline__ uint32_t lp_first(const void* p) {  // the same place
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
     return r;
 }
-__device__ __forceinline__ void lp_put(uint32_t at, float x, float y, float z, float w) {
-    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
+__device__ __forceinline__ void lp_put(uint32_t at, float x, float y, float z) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(x), "f"(y), "f"(z), "f"(0.0f) : "memory");
 }
 __device__ __forceinline__ void lp_put(uint32_t at, uint64_t v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory"); }
 
-// Writes a row's two numbers, from sums against `ref` (in powers of two).
-__device__ __forceinline__ LpRow lp_finish(const LpArgs& a, int64_t r, const LpSums& sums, double ref, int64_t token, float token_logit) {
+// Writes a row's two numbers.
+__device__ __forceinline__ LpRow lp_finish(const LpArgs& a, int64_t r, const LpSums& sums, int64_t token, float token_logit) {
     LpRow row;
-    // (the exponents were x log2e with log2e in 32 bits: the reference goes back by the same number)
-    row.base = lp_far(sums.most) ? static_cast<double>(sums.most) : ref / static_cast<double>(kLpLog2e);
-    row.log_s = log(static_cast<double>(sums.s));
     row.empty = sums.most == __int_as_float(0xff800000);
+    row.base = static_cast<double>(sums.most);
+    // (log2 e in 32 bits is 1.3e-8 too small, so every power a little too large: to first order t says how much in all.  The largest element's
+    // own, which is 1, is not: where the others are lost beside it, what t has of them is not to be taken off.)
+    double s = fmax(fma(kLpLog2eOff, static_cast<double>(sums.t), static_cast<double>(sums.s)), 1.0);
+    if (!(sums.most <= 3.402823466e38f)) s = static_cast<double>(__int_as_float(0x7fffffff));  // a NaN or an infinity
+    row.log_s = log(s);
     float lp = row.logprob(token_logit);
     if (token < 0) lp = 0.0f;
     if (token >= a.vocab) {
@@ -219,27 +280,8 @@ __device__ __forceinline__ LpRow lp_finish(const LpArgs& a, int64_t r, const LpS
         if (a.status != nullptr) atomicOr(a.status, FB_STATUS_INDEX_RANGE);
     }
     a.logprobs[r] = lp;
-    a.entropy[r] = row.empty ? 0.0f : static_cast<float>(row.log_s - static_cast<double>(sums.t) / (static_cast<double>(sums.s) * static_cast<double>(kLpLog2e)));
+    a.entropy[r] = row.empty ? 0.0f : static_cast<float>(row.log_s - static_cast<double>(sums.t) / (s * static_cast<double>(kLpLog2e)));
     return row;
-}
-
-// The sums of a row's parts (one in each of `count` lanes), in all lanes; returns their reference.
-__device__ __forceinline__ double lp_join_parts(LpSums& sums, int count) {
-    const double own = sums.s == 0.0f ? -1e300 : lp_ref(sums);
-    double ref = own;
-    for (int d = count / 2; d > 0; d /= 2) {
-        ref = fmax(ref, __shfl_xor_sync(kFullMask, ref, d));
-        sums.most = max_nan(sums.most, __shfl_xor_sync(kFullMask, sums.most, d));
-    }
-    if (lp_far(sums.most)) ref = static_cast<double>(sums.most) * static_cast<double>(kLpLog2e);
-    const float below = static_cast<float>(fmax(own - ref, -1000.0)), f = lp_ex2(below);
-    sums.t = f * fmaf(below, sums.s, sums.t);
-    sums.s = f * sums.s;
-    for (int d = count / 2; d > 0; d /= 2) {
-        sums.s += __shfl_xor_sync(kFullMask, sums.s, d);
-        sums.t += __shfl_xor_sync(kFullMask, sums.t, d);
-    }
-    return ref;
 }
 
 // The elements of a part of a row: vectors, and single ones in front of (first part) and behind (last part) the row's 16-byte boundaries.
@@ -270,13 +312,14 @@ __device__ __forceinline__ int lp_above(const uint64_t* list, int n, uint64_t ke
 }
 // the sums of `count` lanes (a power of two) together, in all of them
 __device__ __forceinline__ void lp_join_lanes(LpSums& sums, int count) {
+    const float own = sums.most;
+    for (int d = count / 2; d > 0; d /= 2) sums.most = max_nan(sums.most, __shfl_xor_sync(kFullMask, sums.most, d));
+    const float below = own == __int_as_float(0xff800000) ? -1000.0f : fmaxf((own - sums.most) * kLpLog2e, -1000.0f), f = lp_ex2(below);
+    sums.t = f * fmaf(below, sums.s, sums.t);
+    sums.s = f * sums.s;
     for (int d = count / 2; d > 0; d /= 2) {
-        LpSums o;
-        o.most = __shfl_xor_sync(kFullMask, sums.most, d);
-        o.ref = __shfl_xor_sync(kFullMask, sums.ref, d);
-        o.s = __shfl_xor_sync(kFullMask, sums.s, d);
-        o.t = __shfl_xor_sync(kFullMask, sums.t, d);
-        lp_join(sums, o);
+        sums.s += __shfl_xor_sync(kFullMask, sums.s, d);
+        sums.t += __shfl_xor_sync(kFullMask, sums.t, d);
     }
 }
 
@@ -318,7 +361,7 @@ __device__ __noinline__ void lp_again(LpShared<TOP>& sh, const LpPart<T>& p) {
         s += __shfl_xor_sync(kFullMask, s, d);
         t += __shfl_xor_sync(kFullMask, t, d);
     }
-    if (lane == 0) sh.sums[warp] = {most, 0.0f, s, t};  // (one reference for all)
+    if (lane == 0) sh.sums[warp] = {most, s, t};
     __syncthreads();
 }
 
@@ -469,7 +512,7 @@ __device__ void lp_select(LpShared<true>& sh, const LpPart<T>& p, int top, float
 }
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kLpMaxThreads) logprobs_kernel(const LpArgs a, int parts) {
+__global__ void __launch_bounds__(kLpMaxThreads, 3) logprobs_kernel(const LpArgs a, int parts) {
     constexpr int N = LpVec<T>::N;
     __shared__ LpShared<TOP> sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
@@ -485,63 +528,53 @@ __global__ void __launch_bounds__(kLpMaxThreads) logprobs_kernel(const LpArgs a,
     p.num_vec = min(share, vecs - first);
     p.tail_id = head + vecs * N;
     p.tail = rank == parts - 1 ? a.vocab - p.tail_id : 0;
-    int64_t token = -1;
-    float token_logit = 0.0f;
     if (rank == 0 && tid == 0) {
-        token = a.tokens[r];
-        if (token >= 0 && token < a.vocab) token_logit = LpVec<T>::one(p.row + token);
+        const int64_t token = a.tokens[r];
+        sh.token = token;
+        sh.token_logit = token >= 0 && token < a.vocab ? LpVec<T>::one(p.row + token) : 0.0f;
     }
 
     if (parts > 1) lp_cluster_arrive();  // (waited for before the first CTA is written to)
     LpThread th;
     th.start();
-    if (tid < p.head) th.take({LpVec<T>::one(p.row + tid)});
-    if (tid < p.tail) th.take({LpVec<T>::one(p.row + p.tail_id + tid)});
+    if (tid < p.head) th.take_one(LpVec<T>::one(p.row + tid));
+    if (tid < p.tail) th.take_one(LpVec<T>::one(p.row + p.tail_id + tid));
     int v = tid;
     for (; v + 3 * threads < p.num_vec; v += 4 * threads) {
         uint4 u[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) u[i] = p.vec(v + i * threads);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float x[N];
-            LpVec<T>::get(u[i], x);
-            th.take(x);
-        }
+        th.take_vectors<LpVec<T>>(u);
     }
     for (; v < p.num_vec; v += threads) {
-        float x[N];
-        LpVec<T>::get(p.vec(v), x);
-        th.take(x);
+        const uint4 u[1] = {p.vec(v)};
+        th.take_vectors<LpVec<T>>(u);
     }
-    const float most = th.sums.most;
+    const float most = th.most;
     // the block's sums
-    lp_join_lanes(th.sums, 32);
-    if (lane == 0) sh.sums[warp] = th.sums;
-    if (__syncthreads_or(lane == 0 && lp_far(th.sums.most))) lp_again<T, TOP>(sh, p);
-    LpSums sums = {__int_as_float(0xff800000), kLpFloor, 0.0f, 0.0f};
+    LpSums sums = th.warp_sums();
+    if (lane == 0) sh.sums[warp] = sums;
+    if (__syncthreads_or(lane == 0 && lp_far(sums.most))) lp_again<T, TOP>(sh, p);
     if (warp == 0) {
+        sums.none();
         if (lane < warps) sums = sh.sums[lane];
         lp_join_lanes(sums, 16);
     }
     if constexpr (TOP) lp_select<T>(sh, p, a.top, most);
-    double ref = 0.0;
     if (parts > 1) {
         // what the parts have meets in the first one's shared memory
         lp_cluster_wait();  // (it runs)
-        if (tid == 0) lp_put(lp_first(&sh.part[rank]), sums.most, sums.ref, sums.s, sums.t);
+        if (tid == 0) lp_put(lp_first(&sh.part[rank]), sums.most, sums.s, sums.t);
         if (TOP && tid < a.top) lp_put(lp_first(&sh.parts_best[rank * a.top + tid]), sh.best[tid]);
         lp_cluster_arrive();
         lp_cluster_wait();
         if (rank != 0) return;
         if (warp == 0) {
             sums = sh.part[lane & (parts - 1)];
-            ref = lp_join_parts(sums, parts);
+            lp_join_lanes(sums, parts);
         }
-    } else {
-        ref = lp_ref(sums);
     }
-    if (tid == 0) sh.whole = lp_finish(a, r, sums, ref, token, token_logit);
+    if (tid == 0) sh.whole = lp_finish(a, r, sums, sh.token, sh.token_logit);
     if (TOP) {
         const uint64_t* best = sh.best;
         if (parts > 1) {
@@ -579,19 +612,25 @@ __global__ void __launch_bounds__(32 * kLpShortRows) logprobs_short_kernel(const
     for (int i = 0; i < COUNT; ++i) x[i] = i * 32 + lane < a.vocab ? LpVec<T>::one(row + i * 32 + lane) : __int_as_float(0xff800000);
     LpThread th;
     th.start();
-    th.take(x);
-    lp_join_lanes(th.sums, 32);
-    if (lp_far(th.sums.most)) {  // (see lp_again)
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < COUNT; ++i) m = max_nan(m, x[i]);
+    th.take<8, COUNT / 8>(m, [&](int k, float (&y)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = x[k * 8 + i];
+    });
+    LpSums sums = th.warp_sums();
+    if (lp_far(sums.most)) {  // (see lp_again)
         float s = 0.0f, t = 0.0f;
-        lp_take_near(x, th.sums.most, s, t);
+        lp_take_near(x, sums.most, s, t);
         for (int d = 16; d > 0; d /= 2) {
             s += __shfl_xor_sync(kFullMask, s, d);
             t += __shfl_xor_sync(kFullMask, t, d);
         }
-        th.sums.s = s, th.sums.t = t;
+        sums.s = s, sums.t = t;
     }
     LpRow whole = {};
-    if (lane == 0) whole = lp_finish(a, r, th.sums, lp_ref(th.sums), token, token_logit);
+    if (lane == 0) whole = lp_finish(a, r, sums, token, token_logit);
     uint32_t order[COUNT], most = 0;
 #pragma unroll
     for (int i = 0; i < COUNT; ++i) {

@@ -924,3 +924,62 @@ def test_tensors_that_autograd_has_saved_and_a_call_writes(ops):
     ops.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], decays(2), state)
     with torch.inference_mode():
         ops.linear_attention(q, k, v, decays(2), state=state)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,vocab", [(5, 200), (7, 1000), (3, 5003), (40, 32000), (2, 131072), (200, 32001)])
+def test_logprobs_of_confident_rows(ops, rows, vocab, dtype):
+    """One logit far above the others, wherever it lies, as a model's answers mostly are.  Against its power, which is 1, the others sum to
+    `rest`.  On its way into a sum of 1 and more an addend is rounded by half a step, 2^-24, and by no more than itself (leaving it out is
+    one of the two neighbours): 17 times at most (3 in a vector's tree, 4 between vectors, 5 and 4 in the warp and the block, 1 for the
+    logarithm's result), together by no more than `rest`.  Every power is off by less than 2^-20 of itself (its exponent, below 2^7, is
+    rounded by 2^-24 of itself twice, the power by 2^-22).  The entropy has that error of ln s, the same relative to its other part, which is
+    divided by s, and its own terms off by 2^-20 too.  That part's sum passes by the largest element's exponent against its rounded
+    reference, r <= 2^-24 |m| log2 e, which is added and taken off again: 32 roundings between, each of half of 2^-23 r at most."""
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    for gap in (3.0, 10.0, 16.0, 17.5, 20.0, 25.0, 30.0, 48.0):
+        for base in (0.0, -30.0, 50.0):
+            x = (torch.randn(rows, vocab, generator=g, device="cuda") + base).to(dtype)
+            at = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+            at[0], at[-1] = vocab - 1, 0
+            x[torch.arange(rows, device="cuda"), at] = base + gap + 4
+            lp, entropy, top_lp, top_ids = ops.token_logprobs(x, at, top=2)
+            assert torch.equal(top_ids[:, 0], at) and torch.equal(top_lp[:, 0], lp)
+            assert bool((lp <= 0).all()) and bool((top_lp <= 0).all()) and bool((entropy >= 0).all())
+            p = torch.log_softmax(x.double(), dim=1)
+            want = p.gather(1, at[:, None])[:, 0]
+            others = p.scatter(1, at[:, None], -math.inf)
+            rest = torch.exp(torch.logsumexp(others, dim=1) - want)
+            want = -torch.log1p(rest)  # (log_softmax itself is off by 2^-53 of the logits)
+            tol = torch.minimum(rest, torch.full_like(rest, 17 * 2.0 ** -24)) + 2.0 ** -20 * rest + 2.0 ** -24 * want.abs()
+            assert bool(((lp.double() - want).abs() <= tol).all()), (gap, base, float((lp.double() - want).abs().max()))
+            h = -want * torch.exp(want) - (torch.exp(others) * others.clamp(min=-1e300)).sum(1)
+            r = 2.0 ** -24 * x.double().abs().amax(1) * 1.4427
+            assert bool(((entropy.double() - h).abs() <= tol * (1 + h) + 2.0 ** -20 * h + 32 * 2.0 ** -24 * r).all()), (gap, base, float((entropy.double() - h).abs().max()))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("vocab", [64, 1000, 9001, 140000])
+def test_logprobs_are_not_above_zero_nor_entropies_below(ops, vocab, dtype):
+    rows = 64
+    r = torch.arange(rows, device="cuda")
+    for kind in range(6):
+        x = torch.randn(rows, vocab, device="cuda")
+        if kind == 1:
+            x[r, torch.randint(0, vocab, (rows,), device="cuda")] += torch.linspace(0, 90, rows, device="cuda")
+        elif kind == 2:  # two that share the row
+            x[r, torch.randint(0, vocab, (rows,), device="cuda")] = 30.0
+            x[r, torch.randint(0, vocab, (rows,), device="cuda")] = 30.0
+        elif kind == 3:  # rising, so that every element is the largest so far
+            x = torch.arange(vocab, device="cuda", dtype=F32)[None] * torch.linspace(0.001, 3, rows, device="cuda")[:, None]
+        elif kind == 4:  # one of many is left
+            x[:] = -math.inf
+            x[r, torch.randint(0, vocab, (rows,), device="cuda")] = torch.linspace(-200, 200, rows, device="cuda")
+        elif kind == 5:
+            x = x * 1e5
+        x = x.to(dtype)
+        lp, entropy, top_lp, _ = ops.token_logprobs(x, torch.randint(0, vocab, (rows,), device="cuda"), top=8)
+        assert bool((lp <= 0).all()) and bool((top_lp <= 0).all()) and bool((entropy >= 0).all())
+        if kind == 4:
+            assert bool((entropy == 0).all()) and bool((top_lp[:, 0] == 0).all())
+        check_logprobs(ops, x, torch.randint(0, vocab, (rows,), device="cuda"), 8)
