@@ -100,6 +100,7 @@ struct LtPlan {
     int mode;        // 0: whole sequences; 1: the state that each part adds, 2: outputs of the parts
     int boundary;    // of which all rows lie: 16, 8, 4 or 2 bytes
     float* states;   // [batch * heads][segs][dk][dv]
+    float2* decays;  // [batch * heads][segs]: of each part, as a sum of two floats
     uint32_t wait_limit;  // tries of a wait
     int drop_state;       // the switch below
 };
@@ -357,6 +358,11 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
             m.power_gap = near > 0.0f ? fabsf(next - near) / near : 1.0f;
             m.power_off = near > 0.0f ? fabsf(off) / near : 0.0f;
         }
+    }
+    if (plan.mode == 1 && tid == kLtChunk + 1) {  // the decay of the whole part
+        const double p = exp(log_decay * static_cast<double>(max(0, seg_end - seg0)));
+        const float near = static_cast<float>(p);
+        plan.decays[(static_cast<int64_t>(b) * a.heads + h) * plan.segs + seg] = make_float2(near, static_cast<float>(p - static_cast<double>(near)));
     }
     if (tid < 128) m.first_bad[tid] = 0x7fffffff;
     if (tid < kLtChunk) m.scaled_front[tid] = 0.0f;
@@ -895,9 +901,10 @@ static bool lt_encode(CUtensorMap* map, const void* base, const int64_t* stride,
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// The states in front of a sequence's parts, from what each part adds, and the state behind the last one.  One thread per cell of S: the
-// parts' decays are products of decays of whole parts.
-__global__ void __launch_bounds__(256) linattn_carry_kernel(const LinArgs a, float* __restrict__ states, int segs, int seg_tokens) {
+// The states in front of a sequence's parts, from what each part adds, and the state behind the last one.  One thread per cell of S.  The decay
+// of a part is a sum of two floats: rounded to one, it would be off the same way for every part (2.3e-6 of a state that passed 64 of them).
+__global__ void __launch_bounds__(256) linattn_carry_kernel(const LinArgs a, float* __restrict__ states, const float2* __restrict__ decays, int segs,
+                                                            int seg_tokens) {
     const int64_t cells = static_cast<int64_t>(a.dk) * a.dv, cell = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     const int h = blockIdx.y % a.heads, b = blockIdx.y / a.heads, lane = threadIdx.x & 31;
     int bits;
@@ -905,23 +912,14 @@ __global__ void __launch_bounds__(256) linattn_carry_kernel(const LinArgs a, flo
     pdl_wait();
     if (slot < 0 || cell >= cells) return;
     const int length = lin_length(a, b);
-    const int64_t own = (static_cast<int64_t>(slot) * a.heads + h) * cells + cell;
-    float* part = states + (static_cast<int64_t>(b) * a.heads + h) * segs * cells + cell;
+    const int64_t own = (static_cast<int64_t>(slot) * a.heads + h) * cells + cell, first = (static_cast<int64_t>(b) * a.heads + h) * segs;
+    float* part = states + first * cells + cell;
     float s = a.state_in != nullptr ? a.state_in[own] : 0.0f;
-    // The decay of a part as a sum of two floats: rounded to one, it would be off the same way for every part (and expf takes an exponent that
-    // is rounded itself: 2.7e-6 of a state that passed 64 parts).
-    const double log_decay = static_cast<double>(lin_log_decay(a, h));
-    float decay = 1.0f, decay_lo = 0.0f;
-    int of = 0;  // tokens that they are of
     for (int i = 0; i < segs; ++i) {
-        const int n = min(max(length - i * seg_tokens, 0), i + 1 < segs ? seg_tokens : length);
-        if (n > 0 && n != of) {
-            const double exact = exp(log_decay * static_cast<double>(n));
-            decay = static_cast<float>(exact), decay_lo = static_cast<float>(exact - static_cast<double>(decay)), of = n;
-        }
         const float added = part[i * cells];
+        const float2 decay = decays[first + i];
         part[i * cells] = s;
-        if (n > 0) s = fmaf(decay, s, fmaf(decay_lo, s, added));  // (no tokens, no decay: not even one that is NaN)
+        if (i * seg_tokens < length) s = fmaf(decay.x, s, fmaf(decay.y, s, added));  // (no tokens, no decay: not even one that is NaN)
     }
     a.state_out[own] = s;
 }
@@ -952,10 +950,14 @@ static void lt_cut(const LinArgs& a, int64_t rows, int& segs, int& seg_tokens) {
     }
 }
 
+// floats of the parts' states; their decays lie behind them
+static int64_t lt_state_floats(const LinArgs& a, int segs) {
+    return (static_cast<int64_t>(a.batch) * a.heads * segs * a.dk * a.dv + 3) / 4 * 4;
+}
 int64_t linattn_chunk_scratch_bytes(const LinArgs& a) {
     int segs, seg_tokens;
     lt_cut(a, static_cast<int64_t>(a.batch) * a.heads, segs, seg_tokens);
-    return segs == 1 ? 0 : static_cast<int64_t>(a.batch) * a.heads * segs * a.dk * a.dv * 4;
+    return segs == 1 ? 0 : lt_state_floats(a, segs) * 4 + static_cast<int64_t>(a.batch) * a.heads * segs * 8;
 }
 
 template <auto kernel>
@@ -972,7 +974,8 @@ static int launch_chunk(dim3 grid, int threads, int bytes, cudaStream_t st, cons
     plan.mode = 1;
     FB_TRY(launch_after(kernel, grid, dim3(threads), bytes, st, false, "linear_attention", a, plan, maps[0], maps[1], maps[2]));
     const dim3 carry(static_cast<unsigned>((a.dk * a.dv + 255) / 256), static_cast<unsigned>(a.batch * a.heads));
-    FB_TRY(launch_after(linattn_carry_kernel, carry, dim3(256), 0, st, true, "linear_attention", a, plan.states, plan.segs, plan.seg_tokens));
+    FB_TRY(launch_after(linattn_carry_kernel, carry, dim3(256), 0, st, true, "linear_attention", a, plan.states,
+                        static_cast<const float2*>(plan.decays), plan.segs, plan.seg_tokens));
     plan.mode = 2;
     return launch_after(kernel, grid, dim3(threads), bytes, st, true, "linear_attention", a, plan, maps[0], maps[1], maps[2]);
 }
@@ -990,6 +993,7 @@ static int launch_chunk(const LinArgs& a, void* scratch, cudaStream_t st) {
     lt_cut(a, rows, plan.segs, plan.seg_tokens);
     FB_REQUIRE(plan.segs == 1 || (scratch != nullptr && reinterpret_cast<uintptr_t>(scratch) % 16 == 0), "linear_attention: scratch must be given, 16-byte aligned");
     plan.states = static_cast<float*>(scratch);
+    if (plan.segs > 1) plan.decays = reinterpret_cast<float2*>(plan.states + lt_state_floats(a, plan.segs));
     const int64_t ctas = static_cast<int64_t>(a.batch) * a.heads * plan.tiles * plan.segs;
     FB_REQUIRE(ctas < (1ll << 31), "linear_attention: batch * heads is too large");
     const void* base[3] = {a.q, a.k, a.v};
