@@ -5,7 +5,7 @@
 // which is four products:  G = Q K^T,  X = S^T Q^T,  Y = V^T P^T with P = G masked and decayed,  U = K^T W with W = decayed V.
 // S is decayed and added to in fp32 outside the tensor core (which truncates when it adds).
 //
-// Operands have 8 bits, so what has more is a sum of parts: S and P of two (what they make is rounded to 16 bits at once, 2^-16 apart;
+// Operands have 8 bits, so what has more is a sum of parts: S and P of two (what they make is rounded to 16 bits at once, 2^-17 apart;
 // three where the outputs are fp32), W of three (it makes the state, which is fp32: two would leave 2^-16 of each term, with three it is 2e-7 off).  Q, K and V are
 // their own part in bf16, two in fp16 (exact), three in fp32; products of parts that are below the result's precision are left out, and the
 // small ones are added first.
@@ -214,11 +214,18 @@ __device__ __forceinline__ void lt_arrive_read(uint64_t* bar, int lane) {
     if (lane == 0) mbar_arrive(bar);
 }
 
-// A bf16 part of two values: their upper halves, taken out of them; as the last part what is left, rounded.
-__device__ __forceinline__ uint32_t lt_part(float& x, float& y, bool last) {
-    if (last) {
+// A bf16 part of two values: of two parts both are rounded (2^-8 of its power of two is left for the second, 2^-17 lost, at most);
+// of three the first two are the values' upper halves, taken out of them, which is exact and does not overflow, and the last what is left, rounded.
+template <int N>
+__device__ __forceinline__ uint32_t lt_part(float& x, float& y, int p) {
+    if (p + 1 == N || N == 2) {
         const __nv_bfloat162 r = __floats2bfloat162_rn(x, y);
-        return *reinterpret_cast<const uint32_t*>(&r);
+        const uint32_t u = *reinterpret_cast<const uint32_t*>(&r);
+        if (p + 1 < N) {
+            x = __fsub_rn(x, __uint_as_float(u << 16));
+            y = __fsub_rn(y, __uint_as_float(u & 0xFFFF0000u));
+        }
+        return u;
     }
     const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
     x = __fsub_rn(x, __uint_as_float(a & 0xFFFF0000u));
@@ -232,7 +239,7 @@ __device__ __forceinline__ void lt_store_parts(unsigned char* at, int stride, fl
     for (int p = 0; p < N; ++p) {
         uint32_t u[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = lt_part(x[2 * i], x[2 * i + 1], p + 1 == N);
+        for (int i = 0; i < 4; ++i) u[i] = lt_part<N>(x[2 * i], x[2 * i + 1], p);
         *reinterpret_cast<uint4*>(at + p * stride) = make_uint4(u[0], u[1], u[2], u[3]);
     }
 }
@@ -412,7 +419,7 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
             for (int p = 0; p < C::NS; ++p) {
                 uint32_t u[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) u[e] = lt_part(s[2 * e], s[2 * e + 1], p + 1 == C::NS);
+                for (int e = 0; e < 8; ++e) u[e] = lt_part<C::NS>(s[2 * e], s[2 * e + 1], p);
                 lt_st(lane_base + C::kParts + p * kHalf + (k0 + g) / 2, u);
             }
         };

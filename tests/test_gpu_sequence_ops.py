@@ -983,3 +983,25 @@ def test_logprobs_are_not_above_zero_nor_entropies_below(ops, vocab, dtype):
         if kind == 4:
             assert bool((entropy == 0).all()) and bool((top_lp[:, 0] == 0).all())
         check_logprobs(ops, x, torch.randint(0, vocab, (rows,), device="cuda"), 8)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_outputs_of_states_that_cancel(ops, dtype, d):
+    """Two rows of the state that differ by 2^-10 of themselves, one taken from the other.  A value in [1, 2) as two parts of 8 bits: the first
+    leaves 2^-8 at most, which lies in a binade whose half step is 2^-17.  So that is what a product with a query of one part is off by; of
+    two (fp16) the product of the second parts, 2^-8 of each, is left out too.  Beside that fp32 sums of a few terms, 2^-21, and half a step
+    of the output."""
+    tokens, h = 130, 4
+    q, k, v = (torch.zeros(2, tokens, h, d, device="cuda", dtype=dtype) for _ in range(3))
+    q[..., 3], q[..., 7] = 1 + 2.0 ** -7, -1 - 2.0 ** -7
+    if dtype == F16:
+        q[..., 3], q[..., 7] = 1 + 2.0 ** -9 + 2.0 ** -10, -1 - 2.0 ** -9 - 2.0 ** -10
+    state = torch.zeros(2, h, d, d, device="cuda")
+    state[:, :, 3] = torch.randn(2, h, d, device="cuda")
+    state[:, :, 7] = state[:, :, 3] * (1 + 2.0 ** -10 * torch.rand(2, h, d, device="cuda"))
+    a, b = (q[:, 0, 0, 3].double()[:, None, None] * state[:, :, i].double() for i in (3, 7))
+    out, _ = ops.linear_attention(q, k, v, torch.zeros(h, device="cuda"), state=state.clone())
+    want = (a - b)[:, None]
+    tol = torch.finfo(dtype).eps / 2 * want.abs() + ((3 if dtype == F16 else 1) * 2.0 ** -17 + 2.0 ** -21) * (a.abs() + b.abs())[:, None] + torch.finfo(dtype).tiny
+    assert bool(((out.double() - want).abs() <= tol).all())
