@@ -13,11 +13,10 @@ constexpr int kRecurTokens = 16;  // tokens staged at a time
 
 // One token of 16 states of 128 x 128 3.9 us, of 1536 42 (4.8 TB/s), of 8192 187 (5.75 TB/s).
 //
-// A CTA owns COLS = 4 * CG columns of one state: thread -> (column group tid % CG, rows tid / CG + i * RG), so a warp reads whole
-// sectors of 32 / CG rows, and every thread keeps its part of S in registers over all tokens.
-template <typename T, int CG, bool VEC>
+// A CTA owns 32 columns of one state: thread -> (column group tid % CG, rows tid / CG + i * RG), so a warp reads whole sectors of four rows, and every thread keeps its part of S in registers over all tokens.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(kRecurThreads) linattn_recurrent_kernel(const LinArgs a, int tiles) {
-    constexpr int RG = kRecurThreads / CG, ROWS = kLinMaxDim / RG, COLS = 4 * CG, WARPS = kRecurThreads / 32;
+    constexpr int CG = 8, RG = kRecurThreads / CG, ROWS = kLinMaxDim / RG, COLS = 4 * CG, WARPS = kRecurThreads / 32;
     __shared__ float s_q[kRecurTokens][kLinMaxDim], s_k[kRecurTokens][kLinMaxDim], s_v[kRecurTokens][COLS];
     __shared__ float s_part[kRecurTokens][WARPS][COLS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -242,8 +241,8 @@ static int launch_recurrent(const LinArgs& a, cudaStream_t st) {
     if (a.tokens == 1 && a.lengths == nullptr && (a.dk * a.dv <= 64 * 64 || bh >= kNumSMs / 2))
         return vec ? launch_step<T, true>(a, st) : launch_step<T, false>(a, st);
     const dim3 grid(static_cast<unsigned>(bh * tiles));
-    if (vec) return launch_after(linattn_recurrent_kernel<T, 8, true>, grid, dim3(kRecurThreads), 0, st, false, "linear_attention", a, tiles);
-    return launch_after(linattn_recurrent_kernel<T, 8, false>, grid, dim3(kRecurThreads), 0, st, false, "linear_attention", a, tiles);
+    if (vec) return launch_after(linattn_recurrent_kernel<T, true>, grid, dim3(kRecurThreads), 0, st, false, "linear_attention", a, tiles);
+    return launch_after(linattn_recurrent_kernel<T, false>, grid, dim3(kRecurThreads), 0, st, false, "linear_attention", a, tiles);
 }
 
 }  // namespace fb

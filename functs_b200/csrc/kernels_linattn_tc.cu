@@ -94,7 +94,6 @@ struct LtMisc {
 };
 
 struct LtPlan {
-    int tiles;       // of DV columns
     int segs;        // parts of a sequence
     int seg_tokens;  // a multiple of the chunk
     int mode;        // 0: whole sequences; 1: the state that each part adds, 2: outputs of the parts
@@ -306,8 +305,7 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
     LtMisc& m = *reinterpret_cast<LtMisc*>(smem + C::oMisc);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int seg = blockIdx.x % plan.segs, rest = blockIdx.x / plan.segs;
-    const int tile = rest % plan.tiles, h = (rest / plan.tiles) % a.heads, order = rest / (plan.tiles * a.heads);
-    const int hk = h / (a.heads / a.kv_heads), col0 = tile * DV, dv = min(DV, a.dv - col0);
+    const int h = rest % a.heads, order = rest / a.heads, hk = h / (a.heads / a.kv_heads);
 
     if (plan.mode == 1) pdl_launch_dependents();
     // long sequences first, so that the last CTAs are short ones
@@ -328,15 +326,15 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
     const int b = m.b;
     int bits;
     const int slot = lin_slot(a, b, lane, bits);
-    if (bits != 0 && a.status != nullptr && tid == 0 && tile == 0 && seg == 0) atomicOr(a.status, bits);
+    if (bits != 0 && a.status != nullptr && tid == 0 && seg == 0) atomicOr(a.status, bits);
     const int length = slot < 0 ? 0 : lin_length(a, b);
     const int seg0 = plan.segs > 1 ? seg * plan.seg_tokens : 0;                                        // first token of this part
     const int seg_end = plan.segs > 1 && seg + 1 < plan.segs ? min(length, seg0 + plan.seg_tokens) : length;
     const bool outputs = plan.mode != 1;
-    T* out = static_cast<T*>(a.out) + b * a.out_stride[0] + h * a.out_stride[2] + col0;
+    T* out = static_cast<T*>(a.out) + b * a.out_stride[0] + h * a.out_stride[2];
     if (outputs) {  // rows behind the sequence, those that fall in this part
         const int z0 = max(length, seg0), z1 = plan.segs > 1 && seg + 1 < plan.segs ? min(a.tokens, seg0 + plan.seg_tokens) : a.tokens;
-        lin_clear(out, a.out_stride[1], z0, z1, dv);
+        lin_clear(out, a.out_stride[1], z0, z1, a.dv);
     }
     if (slot < 0 || (plan.mode == 2 && seg_end <= seg0)) return;
     const int chunks = max(0, seg_end - seg0 + kLtChunk - 1) / kLtChunk;
@@ -407,8 +405,8 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
         // ---- S: row = channel of V
         constexpr int kHalf = DK / 2;
         const int row = (warp & 3) * 32 + lane, k0 = (warp >> 2) * kHalf;
-        const bool has_row = row < dv;
-        const int64_t cell = static_cast<int64_t>(k0) * a.dv + col0 + row;
+        const bool has_row = row < a.dv;
+        const int64_t cell = static_cast<int64_t>(k0) * a.dv + row;
         const int64_t own = (static_cast<int64_t>(slot) * a.heads + h) * a.dk * a.dv + cell;
         const int64_t part = ((static_cast<int64_t>(b) * a.heads + h) * plan.segs + seg) * a.dk * a.dv + cell;
         const float* from = plan.mode == 2 ? plan.states + part : plan.mode == 0 && a.state_in != nullptr ? a.state_in + own : nullptr;
@@ -531,7 +529,7 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
         const int rank = warp - C::kFirstW, id = rank * 32 + lane;
         const T* q = static_cast<const T*>(a.q) + b * a.q_stride[0] + h * a.q_stride[2] + seg0 * a.q_stride[1];
         const T* k = static_cast<const T*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[2] + seg0 * a.k_stride[1];
-        const T* v = static_cast<const T*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2] + seg0 * a.v_stride[1] + col0;
+        const T* v = static_cast<const T*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[2] + seg0 * a.v_stride[1];
         uint32_t w[3] = {0, 0, 0};  // the weight of this thread's token
 #pragma unroll 1
         for (int c = 0; c < chunks; ++c) {
@@ -555,7 +553,7 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
                     const int t = t0 + kLtChunk + (i & (kLtChunk - 1));
                     if (t >= seg_end - seg0) continue;
                     const char* row = reinterpret_cast<const char*>(i < kLtChunk ? k + t * a.k_stride[1] : i < 2 * kLtChunk ? v + t * a.v_stride[1] : q + t * a.q_stride[1]);
-                    const int bytes = (i < kLtChunk || i >= 2 * kLtChunk ? a.dk : dv) * static_cast<int>(sizeof(T));
+                    const int bytes = (i < kLtChunk || i >= 2 * kLtChunk ? a.dk : a.dv) * static_cast<int>(sizeof(T));
                     for (int at = 0; at < bytes; at += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + at));
                 }
                 static_assert(TMA || kLtChunk * DK / 8 / threads % 2 == 0, "pieces");
@@ -623,7 +621,7 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         const int g = (g0 + j) * 4 + (lane >> 3);
-                        lt_load8(v + (t0 + t) * a.v_stride[1] + g * 8, t < n ? max(0, min(8, dv - g * 8)) : 0, LOADS == kLtWide ? 16 : plan.boundary, x[j]);
+                        lt_load8(v + (t0 + t) * a.v_stride[1] + g * 8, t < n ? max(0, min(8, a.dv - g * 8)) : 0, LOADS == kLtWide ? 16 : plan.boundary, x[j]);
                     }
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
@@ -661,7 +659,7 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
                 if (!lt_wait(m, &m.y_full, c & 1)) break;
                 tc_fence_after();
                 const int first = *reinterpret_cast<volatile int*>(&m.bad) < (c + 1) * kLtChunk ? m.first_bad[row] - c * kLtChunk : kLtChunk;
-                const int t0 = c * kLtChunk + token0, n = row < dv ? min(kShare, seg_end - seg0 - t0) : 0;
+                const int t0 = c * kLtChunk + token0, n = row < a.dv ? min(kShare, seg_end - seg0 - t0) : 0;
                 T* at = out + t0 * a.out_stride[1];
                 const bool whole = n == kShare;
 #pragma unroll 1
@@ -846,7 +844,7 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
             uint64_t* bar = &m.full_v[c % C::kStagesV];
             mbar_arrive_expect_tx(bar, C::kTileV);
             for (int i = 0; i < DV / 64; ++i)
-                lt_tma(smem + C::oV + (c % C::kStagesV) * C::kTileV + i * 8192, &map_v, col0 + i * 64, seg0 + c * kLtChunk, hk, b, bar);
+                lt_tma(smem + C::oV + (c % C::kStagesV) * C::kTileV + i * 8192, &map_v, i * 64, seg0 + c * kLtChunk, hk, b, bar);
             issued_v = c + 1;
         };
         if (chunks > 0) copy_v(0);
@@ -995,13 +993,12 @@ static int launch_chunk(const LinArgs& a, void* scratch, cudaStream_t st) {
     LtPlan plan = {};
     plan.drop_state = t_lt_drop;
     plan.wait_limit = t_lt_drop ? kLtWaitLimitDropped : kLtWaitLimit;
-    plan.tiles = (a.dv + DV - 1) / DV;
     const int64_t rows = static_cast<int64_t>(a.batch) * a.heads;
     lt_cut(a, rows, plan.segs, plan.seg_tokens);
     FB_REQUIRE(plan.segs == 1 || (scratch != nullptr && reinterpret_cast<uintptr_t>(scratch) % 16 == 0), "linear_attention: scratch must be given, 16-byte aligned");
     plan.states = static_cast<float*>(scratch);
     if (plan.segs > 1) plan.decays = reinterpret_cast<float2*>(plan.states + lt_state_floats(a, plan.segs));
-    const int64_t ctas = static_cast<int64_t>(a.batch) * a.heads * plan.tiles * plan.segs;
+    const int64_t ctas = static_cast<int64_t>(a.batch) * a.heads * plan.segs;
     FB_REQUIRE(ctas < (1ll << 31), "linear_attention: batch * heads is too large");
     const void* base[3] = {a.q, a.k, a.v};
     const int64_t* stride[3] = {a.q_stride, a.k_stride, a.v_stride};

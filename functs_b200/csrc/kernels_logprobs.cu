@@ -679,7 +679,7 @@ static int launch_logprobs(const LpArgs& a, int rows, cudaStream_t st) {
     int parts = 1;
     while (parts < most && static_cast<int64_t>(rows) * parts * 2 <= kNumSMs && vecs / (parts * 2) >= 512) parts *= 2;
     const int each = vecs / parts;
-    const int threads = each >= 1024 ? (rows >= 4 * kNumSMs ? 256 : 512) : each >= 512 ? 256 : each >= 128 ? 128 : 64;
+    const int threads = each >= 1024 ? (rows >= 4 * kNumSMs ? 256 : 512) : each >= 512 ? 256 : 128;  // (a row has 128 vectors at least, a part 512)
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(rows) * parts);
     cfg.blockDim = dim3(threads);
