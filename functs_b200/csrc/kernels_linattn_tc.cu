@@ -47,6 +47,7 @@
 namespace fb {
 
 constexpr int kLtChunk = 64;
+constexpr int kLtRanked = 128;  // sequences, as many as a CTA has threads for at least
 constexpr int kLtWarpsS = 8, kLtWarpsP = 8;  // (of the P group four make P, two issue products, one copies)
 constexpr uint32_t kLtWaitLimit = 200000u, kLtWaitLimitDropped = 5000u;
 // Development switch (functs_b200_debug_set "linattn_drop_state"): in this thread's calls nobody says that S is there, so that the waits for it,
@@ -308,10 +309,12 @@ linattn_chunk_kernel(const LinArgs a, const LtPlan plan, const __grid_constant__
     const int h = rest % a.heads, order = rest / a.heads, hk = h / (a.heads / a.kv_heads);
 
     if (plan.mode == 1) pdl_launch_dependents();
-    // long sequences first, so that the last CTAs are short ones
+    // Long sequences first, so that the last CTAs are short ones.  Every CTA ranks all of them, so not beyond kLtRanked: uneven sequences of 4 to 8
+    // heads of 128 in bf16, 128 of up to 1024 tokens 121 us (in the order given 134), 96 with few long ones 89 (119), 128 of up to 256 108 (104);
+    // but 200 of up to 128 154 ranked and 123 in the order given, 600 of 512 325 and 171, 1000 of 64 1530 and 253.
     if (tid == 0) m.b = order;
     __syncthreads();
-    if (a.lengths != nullptr && a.batch <= C::kThreads) {
+    if (a.lengths != nullptr && a.batch <= kLtRanked) {
         if (tid < a.batch) {
             const int mine = lin_length(a, tid);
             int before = 0;

@@ -1005,3 +1005,14 @@ def test_outputs_of_states_that_cancel(ops, dtype, d):
     want = (a - b)[:, None]
     tol = torch.finfo(dtype).eps / 2 * want.abs() + ((3 if dtype == F16 else 1) * 2.0 ** -17 + 2.0 ** -21) * (a.abs() + b.abs())[:, None] + torch.finfo(dtype).tiny
     assert bool(((out.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("b", [2, 127, 128, 129, 1100])
+def test_uneven_sequences_in_any_order(ops, b):
+    """Batches on either side of those whose sequences are taken longest first."""
+    t, h, d = 140, 2, 32
+    q, k, v = make(b, t, h, h, d, d, BF16)
+    lengths = torch.randint(0, t + 1, (b,), device="cuda", dtype=torch.int32)
+    lengths[::5] = 70  # (and equal ones)
+    out, state = ops.linear_attention(q, k, v, decays(h), lengths=lengths)
+    check_attention(out, state, recurrence(q, k, v, decays(h), 1.0, None, lengths), BF16, t, d)
