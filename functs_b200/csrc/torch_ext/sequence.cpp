@@ -176,16 +176,19 @@ void written(const at::Tensor& t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
-// Whether the memory from the first element of one to its last lies apart from the other's.
-bool apart(const at::Tensor& a, const at::Tensor& b) {
-    if (a.numel() == 0 || b.numel() == 0) return true;
-    const auto end = [](const at::Tensor& t) {
+// The memory from a tensor's first element to its last.
+struct Span {
+    uintptr_t first = 0, end = 0;
+    explicit Span(const at::Tensor* t) {
+        if (t == nullptr || t->numel() == 0) return;
         int64_t last = 0;
-        for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
-        return reinterpret_cast<uintptr_t>(t.data_ptr()) + (last + 1) * t.element_size();
-    };
-    return end(a) <= reinterpret_cast<uintptr_t>(b.data_ptr()) || end(b) <= reinterpret_cast<uintptr_t>(a.data_ptr());
-}
+        const auto sizes = t->sizes(), strides = t->strides();
+        for (size_t d = 0; d < sizes.size(); ++d) last += (sizes[d] - 1) * strides[d];
+        first = reinterpret_cast<uintptr_t>(t->const_data_ptr());
+        end = first + (last + 1) * t->element_size();
+    }
+    bool apart(const Span& o) const { return end <= o.first || o.end <= first || first == end || o.first == o.end; }
+};
 
 // Whether no two elements of `t` can be the same: every stride steps over all that the smaller ones reach.
 bool elementsApart(const at::Tensor& t) {
@@ -204,14 +207,16 @@ bool elementsApart(const at::Tensor& t) {
 // What is written (the output, a given state) lies apart from all that is read while it is, and from one another.
 void checkWritten(const at::Tensor* out, const at::Tensor* state, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                   const at::Tensor& log_decay, const MaybeTensor& slots, const MaybeTensor& lengths, const MaybeTensor& status) {
-    std::vector<const at::Tensor*> others{&q, &k, &v, &log_decay};
+    const Span to(out), kept(state);
+    TORCH_CHECK_VALUE(to.apart(kept), "out must not share memory with the state");
+    const auto check = [&](const at::Tensor* t) {
+        const Span read(t);
+        TORCH_CHECK_VALUE(kept.apart(read), "state must not share memory with the inputs");
+        TORCH_CHECK_VALUE(to.apart(read), "out must not share memory with the inputs (from its first element to its last)");
+    };
+    for (const at::Tensor* t : {&q, &k, &v, &log_decay}) check(t);
     for (const MaybeTensor* t : {&slots, &lengths, &status})
-        if (t->has_value()) others.push_back(&**t);
-    for (const at::Tensor* t : others) {
-        TORCH_CHECK_VALUE(state == nullptr || apart(*state, *t), "state must not share memory with the inputs");
-        TORCH_CHECK_VALUE(out == nullptr || apart(*out, *t), "out must not share memory with the inputs (from its first element to its last)");
-    }
-    TORCH_CHECK_VALUE(out == nullptr || state == nullptr || apart(*out, *state), "out must not share memory with the state");
+        if (t->has_value()) check(&**t);
 }
 
 at::Tensor output(const MaybeTensor& out, const at::Tensor& q, const at::Tensor& v) {
