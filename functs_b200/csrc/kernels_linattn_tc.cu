@@ -26,10 +26,11 @@
 //
 // What bounds it: 128 x 128 heads in bf16 take 2.8 us per chunk and SM, where HBM would let 64 tokens pass in 1.5.  The chunk's 44 products
 // alone take 2100 cycles (2700 where a lane is chosen by comparison instead of election), and more beside the other warps, whose reads and
-// writes of shared memory they share; the warps' 13 600 instructions of a chunk issue at 2.4 of 4 per cycle.  No single role or pipe is the
-// bound: when a chunk took 4.2 us, leaving out the work of one role saved 3 to 13 %, of four together 34 %.  16 x 2048 tokens of 16 heads 187 us (2.9 TB/s),
-// 8192 tokens of 16 heads 97, 16 uneven prompts of up to 2048 tokens 117.  In fp16 and fp32 the threads split every tile into parts:
-// 4 to 5 us per chunk of 64 x 64 heads, 10 of 128 x 128, which shared memory holds once.
+// writes of shared memory they share; the warps' 13 850 instructions of a chunk issue at 2.4 of 4 per cycle, and no pipe is busy more than 41 % of
+// the time.  The roles wait for one another: U for W, S for U, X for S, the outputs for X, chunk after chunk (when a chunk took 4.2 us, leaving
+// out the work of one role saved 3 to 13 %, of four together 34 %).  16 x 2048 tokens of 16 heads 186 us (2.9 TB/s), 8192 tokens of 16 heads 93,
+// 16 uneven prompts of up to 2048 tokens 108.  In fp16 and fp32 the threads split every tile into parts: 4.4 us per chunk of 64 x 64 heads,
+// 10.4 of 128 x 128, which shared memory holds once.
 // Tried and slower: G in columns of its own behind X, so that it does not wait for U to be read (2.95 and 3.3 us per chunk against 2.75);
 // S read eight columns at a time with the next eight on their way (2.82); the roles' loops unrolled (4.5: instruction cache); one lane of a
 // warp waiting for all (6.5); all of a chunk's phases by all warps between block barriers (6.8).
@@ -293,7 +294,7 @@ __device__ __forceinline__ bool lt_finite(float x) { return fabsf(x) <= 3.402823
 // ---- the kernel -----------------------------------------------------------------------------------------------------
 
 // LOADS: how the rows are read.  By TMA; by loads of 16 bytes; or by those that plan.boundary allows (a kernel of its own: their code beside
-// the others' costs: 16 x 2048 tokens of 16 heads of 64 in fp32 297 us, with it 317).
+// the others' costs: 16 x 2048 tokens of 16 heads of 64 in fp32 279 us; when it was taken out 297, with it 317).
 enum LtLoads { kLtTma, kLtWide, kLtAny };
 template <typename T, int DK, int DV, LtLoads LOADS>
 __global__ void __launch_bounds__(LtCfg<T, DK, DV>::kThreads, 1)
@@ -911,8 +912,8 @@ static bool lt_encode(CUtensorMap* map, const void* base, const int64_t* stride,
 
 // The states in front of a sequence's parts, from what each part adds, and the state behind the last one.  One thread per cell of S.  The decay
 // of a part is a sum of two floats: rounded to one, it would be off the same way for every part (2.3e-6 of a state that passed 64 of them).
-__global__ void __launch_bounds__(256) linattn_carry_kernel(const LinArgs a, float* __restrict__ states, const float2* __restrict__ decays, int segs,
-                                                            int seg_tokens) {
+__global__ void __launch_bounds__(256) linattn_carry_kernel(const LinArgs a, float* states, float2* decays, int segs, int seg_tokens) {
+    // (plain pointers: both are written by the kernel before, and nothing may read them ahead of the wait for it)
     const int64_t cells = static_cast<int64_t>(a.dk) * a.dv, cell = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     const int h = blockIdx.y % a.heads, b = blockIdx.y / a.heads, lane = threadIdx.x & 31;
     int bits;
@@ -932,10 +933,10 @@ __global__ void __launch_bounds__(256) linattn_carry_kernel(const LinArgs a, flo
     a.state_out[own] = s;
 }
 
-// How many parts a sequence is cut into, by the time that it would take (in us; fitted to 66 sizes with 1 to 32 parts, and within a tenth of the
-// best of those).  Cutting costs a second reading of K and V, a start of both kernels for every wave of parts, and the states in between; it
-// pays where whole sequences leave SMs without work.  128 x 128 heads in bf16: 8192 tokens of 16 heads 354 whole and 92 in nine parts, 1024
-// tokens 46 and 33 in eight; but 8 x 1024 tokens of 8 heads 50 and 65 in two, 3 x 640 tokens of 16 heads 33 and 54 in three.
+// How many parts a sequence is cut into, by the time that it would take (in us; fitted to 66 sizes with 1 to 32 parts, and
+// within a hundredth of the best of those at 65 of them: 256 tokens of 8 heads of 64 in fp32 take 23.3 whole and 21.7 in four parts).  Cutting costs a second reading of K and V, a start of both kernels for every wave of parts, and the states in between; it
+// pays where whole sequences leave SMs without work.  128 x 128 heads in bf16: 8192 tokens of 16 heads 354 whole and 93 in nine parts, 1024
+// tokens 47 and 33 in eight; but 8 x 1024 tokens of 8 heads 50 and 65 in two, 3 x 640 tokens of 16 heads 33 and 54 in three.
 static void lt_cut(const LinArgs& a, int64_t rows, int& segs, int& seg_tokens) {
     const int chunks = (a.tokens + kLtChunk - 1) / kLtChunk;
     segs = 1;
@@ -982,8 +983,7 @@ static int launch_chunk(dim3 grid, int threads, int bytes, cudaStream_t st, cons
     plan.mode = 1;
     FB_TRY(launch_after(kernel, grid, dim3(threads), bytes, st, false, "linear_attention", a, plan, maps[0], maps[1], maps[2]));
     const dim3 carry(static_cast<unsigned>((a.dk * a.dv + 255) / 256), static_cast<unsigned>(a.batch * a.heads));
-    FB_TRY(launch_after(linattn_carry_kernel, carry, dim3(256), 0, st, true, "linear_attention", a, plan.states,
-                        static_cast<const float2*>(plan.decays), plan.segs, plan.seg_tokens));
+    FB_TRY(launch_after(linattn_carry_kernel, carry, dim3(256), 0, st, true, "linear_attention", a, plan.states, plan.decays, plan.segs, plan.seg_tokens));
     plan.mode = 2;
     return launch_after(kernel, grid, dim3(threads), bytes, st, true, "linear_attention", a, plan, maps[0], maps[1], maps[2]);
 }
