@@ -1016,3 +1016,22 @@ def test_uneven_sequences_in_any_order(ops, b):
     lengths[::5] = 70  # (and equal ones)
     out, state = ops.linear_attention(q, k, v, decays(h), lengths=lengths)
     check_attention(out, state, recurrence(q, k, v, decays(h), 1.0, None, lengths), BF16, t, d)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("vocab", [200, 1000, 3001, 40003, 140007])
+def test_logprobs_of_rows_with_values_that_are_not_finite(ops, vocab, dtype):
+    """A NaN of either sign or an infinity wherever it lies: in vectors, in front of and behind them, in every block's part."""
+    places = [0, 1, 5, vocab // 7, vocab // 3, vocab // 2 + 1, vocab - 9, vocab - 2, vocab - 1]
+    for value in (math.nan, -math.nan, math.inf):
+        x = torch.randn(len(places) + 1, vocab + 1, device="cuda").to(dtype)[:, :vocab]  # (rows on every boundary)
+        for r, at in enumerate(places):
+            x[r, at] = value
+        ids = torch.tensor(places + [3], device="cuda")
+        for top in (0, 3):
+            lp, entropy, top_lp, top_ids = ops.token_logprobs(x, ids, top=top)
+            assert bool(torch.isnan(lp[:-1]).all()) and bool(torch.isnan(entropy[:-1]).all()) and bool(torch.isnan(top_lp[:-1]).all())
+            assert bool(torch.isfinite(lp[-1])) and bool(torch.isfinite(entropy[-1]))
+            if top:
+                assert torch.equal(top_ids[:-1, 0], ids[:-1])
+        check_logprobs(ops, x[-1:], ids[-1:], 3)
