@@ -16,8 +16,10 @@
 //
 // A row is one CTA, or a cluster of up to eight whose parts meet in the first one's shared memory; a short row is a warp.
 //
-// Bound by HBM where rows are many (4096 rows of 32000 in bf16: 57 us, 4.6 TB/s; exponentials and issue take half of the time beside it)
-// and by latency where they are few (one row of 32000 in fp32 4.8 us, with five alternatives 7.6: the choice is eight block barriers).
+// Bound by HBM beside exponentials and issue where rows are many (4096 rows of 32000 in bf16 and in fp16 52 us, 5.0 TB/s, in fp32 89, 5.9 TB/s)
+// and by latency where they are few (one row of 32000 in fp32 4.5 us, with five alternatives 7.1: the choice is eight block barriers).
+// Three blocks of 512 threads an SM are worth 40 registers a thread: with 50, two of them, 600 rows of 50001 in bf16 with 20 alternatives take
+// 31 us (24.7), 2410 of 12838 in fp16 with five 41 (31.5).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -340,7 +342,7 @@ __device__ __forceinline__ void lp_each(const LpPart<T>& p, F f) {
 
 // A part whose largest element is 2^28 or more from 0, once more: there x log2e is rounded by so much that powers of the remainder overflow
 // (and -inf, where a mask is the type's lowest value).  Nothing else comes here: masked elements below a row of usual ones count as nothing.
-// (A call: inlined, the loop over usual rows came out slower, 4096 rows of 32000 in bf16 65 us and 57.)
+// (A call: inlined, the loop over usual rows came out slower, 4096 rows of 32000 in bf16 65 us and 57 when that was tried.)
 template <typename T, bool TOP>
 __device__ __noinline__ void lp_again(LpShared<TOP>& sh, const LpPart<T>& p) {
     constexpr int N = LpVec<T>::N;
@@ -671,10 +673,11 @@ static int launch_logprobs_short(const LpArgs& a, int rows, cudaStream_t st) {
 template <typename T, bool TOP>
 static int launch_logprobs(const LpArgs& a, int rows, cudaStream_t st) {
     const int vecs = a.vocab / LpVec<T>::N;
-    // (figures that were timed together)  One CTA per row, unless rows are few and long.  Without alternatives a part of 512 vectors at least (one row of 32000 fp32 logits 4.3 us
-    // in eight parts, 4.5 in four, 5.2 in one).  With alternatives the parts' lists have to meet: four parts from 8192 vectors on (8 rows of
-    // 65536 in bf16 8.9 us in one, 7.6 in four, 7.7 in eight), fewer vectors in one (one row of 32000 in fp32 7.1, in eight 8.2).  With several
-    // rows per SM 256 threads a row (4096 rows of 32000: 54 us, with 512 threads 62), else 512 (256 rows of 131072: 24 and 37).
+    // One CTA per row, unless rows are few and long.  Without alternatives a part of 512 vectors at least (one row of 32000 fp32 logits 4.4 us in
+    // eight parts or four, 4.9 in one).  With alternatives the parts' lists have to meet: four parts from 8192 vectors on (8 rows of 65536 in
+    // bf16 from HBM 10.9 us in one, 9.8 in four; of 131072 16.2 and 10.8), fewer vectors in one (one row of 32000 in fp32 7.4, in four 8.2).
+    // With several rows per SM 256 threads a row (4096 rows of 32000 in bf16: 52.5 us, with 512 threads 62.4), else 512 (256 rows of 131072
+    // with 20 alternatives 23.1, with 256 threads 32.1).
     const int most = !TOP ? kLpMaxParts : vecs >= 8192 ? kLpTopParts : 1;
     int parts = 1;
     while (parts < most && static_cast<int64_t>(rows) * parts * 2 <= kNumSMs && vecs / (parts * 2) >= 512) parts *= 2;
