@@ -317,7 +317,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, sta
     """What a model answers with: logits [R, V] (float32, float16 or bfloat16; rows any distance apart), tokens int64 [R] ->
     (logprobs float32 [R] of the tokens, entropy float32 [R] in nats, top_logprobs float32 [R, top], top_ids int64 [R, top]).
 
-    top: up to 64 alternatives, best first, of equal ones the lowest id first.  -inf masks a token.  A row of -inf alone: log
+    No log probability is above 0, no entropy below.  top: up to 64 alternatives, best first, of equal ones the lowest id first.  -inf masks
+    a token.  A row of -inf alone: log
     probabilities -inf, entropy 0, the lowest ids.  A row with NaN or +inf: NaN (the ids still in order, NaN first).  A negative token:
     0, nothing is scored; a token of V or above: NaN, and `status` (int32, on the device or pinned) gets FB_STATUS_INDEX_RANGE."""
     return _native()._token_logprobs(logits, tokens, top, status)
