@@ -7,7 +7,7 @@
 // The order is that of the scores in 64 bits.  A row's logarithm out of the pass is off by some 2^-19 at most (5e-8 as measured), the same for all of
 // its candidates, so only neighbours from different rows that lie nearer to one another than that can be the wrong way round.  Where there are any
 // among the best (one call of 64 groups of 8 in ten), the rows in question are summed again in 64 bits by the group's block, and the lists
-// merged again: 16 us more for every row of 50001, bound by the block's SM, which does some 16 products in 64 bits a cycle (with the library's
+// merged again: 14 us more for every row of 50001, bound by the block's SM, which does some 16 products in 64 bits a cycle (with the library's
 // exponentials, four at a time, 25).  Tried for that: a cluster of eight blocks a group that shares the rows, 14 us instead of 50 for two of them, but 3.5 us
 // more for every call of many groups.
 //
@@ -103,17 +103,18 @@ __device__ __forceinline__ double beam_double(float x) {
 }
 // exp(x - base), x <= base, for sums in 64 bits.  With y = x - base, k = y 256 / ln 2 rounded to a whole number and r = y - k ln 2 / 256, |r| <= 0.0014, it is 2^(k / 256),
 // from a table of kBeamPowers powers, times the first terms of exp(r)'s Taylor series (4e-17 are left out).  Eight products in 64 bits, of which an SM does 16 a
-// cycle.  What lies 600 below base counts as that.
+// cycle.  What lies 600 or more below base, -inf too, counts as nothing: by the difference, since next to a base far from 0 there may be no float 600 below.
 __device__ __forceinline__ double beam_exp(float x, float base, const double* power) {
-    x = fmaxf(x, base - 600.0f);
-    const float whole = fmaf(x - base, kBeamPowers * kLpLog2e, 12582912.0f);  // 1.5 * 2^23: a sum with it is a whole number, in its last bits
+    const float apart = x - base;
+    const float whole = fmaf(fmaxf(apart, -600.0f), kBeamPowers * kLpLog2e, 12582912.0f);  // 1.5 * 2^23: a sum with it is a whole number, in its last bits
     const int k = __float_as_int(whole) - __float_as_int(12582912.0f);
     const double y = beam_double(x) - beam_double(base), r = fma(beam_double(whole - 12582912.0f), -0.69314718055994530942 / kBeamPowers, y);
     double p = fma(1.0 / 24.0, r, 1.0 / 6.0);
     p = fma(p, r, 0.5);
     p = fma(p, r, 1.0);
     p = fma(p, r, 1.0) * power[k & (kBeamPowers - 1)];
-    return __hiloint2double(__double2hiint(p) + (k >> 8) * (1 << 20), __double2loint(p));
+    p = __hiloint2double(__double2hiint(p) + (k >> 8) * (1 << 20), __double2loint(p));
+    return apart > -600.0f ? p : 0.0;
 }
 
 // entries of a list in descending order that are above `x`, or, where `equal`, not below it
@@ -258,10 +259,7 @@ __global__ void __launch_bounds__(kBeamMergeThreads) beam_merge_kernel(const Bea
                     x[e] = at < a.vocab ? LpVec<T>::one(row + at) : __int_as_float(0xff800000);
                 }
 #pragma unroll
-                for (int e = 0; e < kBeamLoads; ++e) {
-                    const double power = beam_exp(x[e], base, sh.power);
-                    some[e % 4] += v + e * kBeamMergeThreads < a.vocab ? power : 0.0;
-                }
+                for (int e = 0; e < kBeamLoads; ++e) some[e % 4] += beam_exp(x[e], base, sh.power);
             }
             double s = (some[0] + some[1]) + (some[2] + some[3]);
             for (int d = 16; d > 0; d /= 2) s += __shfl_xor_sync(kFullMask, s, d);

@@ -421,3 +421,29 @@ def test_a_beam_search(ops):
                 new.append((float(want[0][0, k]), parent[1] or int(want[2][0, k]) == end, state, at))
                 assert torch.allclose(logits[g, k].double(), at, rtol=1e-3, atol=1e-3 * float(at.abs().max()))
             plain[g] = new
+
+
+# ---- logits and scores far from 0 -----------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("most", [2.0 ** 31, 1.2e10, -1.2e10, 1e11, 1e30, -1e30, "max", "min"])
+def test_beams_that_are_alike_far_from_0(ops, most, dtype):
+    """Two beams of the same score and row, whose largest logits (five of them) lie far from 0, beside lower ones and -inf; a third that is less likely than
+    they are by less than log(vocabulary)."""
+    v = 1300
+    most = torch.tensor({"max": torch.finfo(dtype).max, "min": torch.finfo(dtype).min}.get(most, most), device="cuda").to(dtype)
+    logits = torch.full((3, 4, v), -math.inf, device="cuda", dtype=dtype)
+    logits[:, 1::2] = torch.randn(3, 2, v, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
+    logits[:, 1::2, 77] = 40.0
+    logits[1, ::2] = most - most.abs() * 2.0 ** -6  # (lower by far, or, where that is none, -inf again)
+    logits[2, ::2, 9::2] = most - most.abs()
+    logits[:, ::2, 100:600:100] = most
+    scores = torch.tensor([[-1.0, -2.0, -1.0, -5.0]], device="cuda").expand(3, -1)
+    want = select_reference(logits, scores, 12)
+    got = ops.beam_select(logits, scores, top=12)
+    assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+    # rows far from 0 have sums of at most 11 elements a thread, each rounded, joined in 32 more
+    fine = torch.isfinite(want[0])
+    assert torch.equal(torch.isfinite(got[0]), fine)
+    assert bool(((got[0].double() - want[0]).abs()[fine] <= 2.0 ** -24 * want[0].abs()[fine] + (11 + 32) * 2.0 ** -24).all())
