@@ -116,6 +116,14 @@ __device__ __forceinline__ void scan_store(float* p, int n, int states, bool vec
     }
 }
 
+// A log2 e, two at a time, for exponentials of 2.  No further from 0 than a float goes: a rate of -inf (or one whose product is) forgets at a step above 0 all
+// the same, and a step of 0, which also stands for tokens behind the last, leaves a state as it is.  A NaN stays one.
+__device__ __forceinline__ uint64_t scan_rate(uint64_t a) {
+    const float2 r = pair_get(pair_mul(a, pair_of(kActLog2e, kActLog2e)));
+    const auto limited = [](float x) { return -max_nan(-max_nan(x, -3.402823466e38f), -3.402823466e38f); };
+    return pair_of(limited(r.x), limited(r.y));
+}
+
 struct ScanPlan {
     int32_t tiles, parts, part_tokens;  // channel tiles of a group; parts of a sequence
     bool vec_rows, vec_bc, vec_states;  // whether rows of channels, rows of B and C, states lie on boundaries of 16 bytes
@@ -256,7 +264,7 @@ __global__ void __launch_bounds__(32 * kScanWarps, 3) scan_kernel(const ScanArgs
     if (lives && slot >= 0) {
         scan_load<PER>(a.A + static_cast<int64_t>(c0 + mine) * a.states, n0, a.states, false, rate);
 #pragma unroll
-        for (int i = 0; i < PAIRS; ++i) rate[i] = pair_mul(rate[i], pair_of(kActLog2e, kActLog2e));
+        for (int i = 0; i < PAIRS; ++i) rate[i] = scan_rate(rate[i]);
         if (a.dt_bias != nullptr) bias = a.dt_bias[c0 + mine];
         if (!ENDS && a.D != nullptr) direct = a.D[c0 + mine];
         if (plan.parts == 1 || (ENDS && part == 0)) {
@@ -448,7 +456,7 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtas) scan_step_kernel(cons
         if (a.D != nullptr) direct = a.D[c];
     }
 #pragma unroll
-    for (int p = 0; p < PAIRS; ++p) rate[p] = pair_mul(rate[p], pair_of(kActLog2e, kActLog2e));
+    for (int p = 0; p < PAIRS; ++p) rate[p] = scan_rate(rate[p]);
     for (int i = warp; i < count; i += kStepThreads / 32) {
         int bits;
         const int slot = lin_slot(a.slots, a.num_slots, b0 + i, lane, bits);

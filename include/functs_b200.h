@@ -313,7 +313,8 @@ int functs_b200_causal_conv(const functs_b200_causal_conv_args* args, void* stre
  *   d = dt[t][c] + dt_bias[c]  (softplus != 0: log(1 + exp(d)));  h[c][n] = exp(d A[c][n]) h[c][n] + d x[t][c] B[t][g][n]
  *   y = sum_n C[t][g][n] h[c][n] + D[c] x[t][c];  out[t][c] = y  (z given: y z / (1 + exp(-z)), z = z[t][c])
  * x, dt, z (optional), out [batch, tokens, channels], B, C [batch, tokens, groups, states]: elements of `dtype`, the last index adjacent, the
- * other strides free.  A [channels, states], D, dt_bias [channels] (both optional) fp32.  1 <= states <= 64.
+ * other strides free.  A [channels, states], D, dt_bias [channels] (both optional) fp32; an A beyond +-2.3e38, an infinite one too, counts as
+ * that (a step of 0 leaves a state as it is).  1 <= states <= 64.
  * state_in (NULL: zeros), state_out: [num_slots, channels, states] fp32, the same memory or apart.  slots, lengths, status: as above.
  * scratch: functs_b200_selective_scan_scratch_bytes, 16-byte aligned (may be NULL where that is 0). */
 typedef struct {

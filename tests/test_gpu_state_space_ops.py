@@ -581,3 +581,50 @@ def test_deterministic(ops):
     for _ in range(3):
         again = ops.selective_scan(x, dt, A, B, C, D=D, z=z, dt_bias=bias, softplus=True)
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+# ---- rates that are not finite, states that grow ----------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("t,c,n", [(1, 40, 16), (5, 33, 5), (16, 40, 16), (33, 64, 8), (130, 36, 3), (1203, 48, 16)])
+def test_states_that_forget_at_once(ops, t, c, n, dtype):
+    """A rate of -inf, or one whose product with log2 e is: every token but the last is forgotten, at whatever token a sequence ends."""
+    b = 4
+    x, dt, A, B, C, D, z, bias = make(b, t, c, n, 1, dtype)
+    A[::2, 0], A[1::3, n - 1] = -math.inf, -3e38
+    lengths = torch.tensor([t, t // 2, 1, max(t - 3, 0)], dtype=torch.int32, device="cuda")
+    start = torch.randn(b, c, n, device="cuda")
+    pool = start.clone()
+    out, _ = ops.selective_scan(x, dt, A, B, C, D=D, z=z, dt_bias=bias, softplus=True, state=pool, lengths=lengths)
+    plain = A.clamp(min=-1e15)  # (steps are some 1e-5 at least: nothing is left either)
+    check_scan(out, pool, recurrence(x, dt, plain, B, C, D, z, bias, True, start, lengths), dtype)
+    pool = start.clone()
+    out = ops.selective_scan_step(x[:, 0], dt[:, 0], A, B[:, 0], C[:, 0], pool, D=D, z=z[:, 0], dt_bias=bias, softplus=True)
+    want = recurrence(x[:, :1], dt[:, :1], plain, B[:, :1], C[:, :1], D, z[:, :1], bias, True, start, torch.ones(b, device="cuda"))
+    check_scan(out[:, None], pool, want, dtype)
+
+
+@pytest.mark.parametrize("t", [3, 17, 700])
+def test_rates_without_bound_and_steps_of_either_sign(ops, t):
+    """A step of 0 leaves every state as it is, and a step below 0 with a rate of +inf nothing of it; a rate that is no number reaches its own channel alone."""
+    x, _, A, B, C, D, _, _ = make(2, t, 24, 16, 1, F32)
+    start = torch.randn(2, 24, 16, device="cuda")
+    A[:, 2], A[:, 5] = -math.inf, math.inf
+    none = torch.zeros(2, t, 24, device="cuda")
+    out, state = ops.selective_scan(x, none, A, B, C, D=D, state=start.clone())
+    assert torch.equal(state, start) and bool(torch.isfinite(out).all())
+    pool = start.clone()
+    ops.selective_scan_step(x[:, 0], none[:, 0], A, B[:, 0], C[:, 0], pool)
+    assert torch.equal(pool, start)
+    A[:, 2] = -1.0
+    back = none - 0.001
+    out, state = ops.selective_scan(x, back, A, B, C, D=D, state=start.clone())
+    want = recurrence(x, back, A.clamp(max=1e15), B, C, D, None, None, False, start, torch.full((2,), t, device="cuda"))
+    check(out, want[0], want[1], F32)
+    assert bool(((state.double() - want[2]).abs() <= want[3]).all())
+    A[3, 4] = math.nan
+    out, state = ops.selective_scan(x, back, A, B, C, D=D, state=start.clone())
+    bad = torch.zeros(24, 16, dtype=torch.bool, device="cuda")
+    bad[3, 4] = True
+    assert torch.equal(torch.isnan(state), bad.expand(2, -1, -1)) and torch.equal(torch.isnan(out), bad.any(1).expand(2, t, -1))
