@@ -281,9 +281,14 @@ __global__ void __launch_bounds__(32 * kScanWarps, 3) scan_kernel(const ScanArgs
                 uint64_t left[PAIRS];
                 const int64_t at = scratch + static_cast<int64_t>(p) * a.channels;
                 scan_load<PER>(plan.ends + at * a.states, n0, a.states, plan.vec_states, left);
-                const float sum = plan.sums[at];
+                // (a power by its cube root: where a part's tokens let a state grow the power itself may pass 32 bits, and the state, small or 0 before, need not)
+                const float third = plan.sums[at] * (1.0f / 3.0f);
 #pragma unroll
-                for (int i = 0; i < PAIRS; ++i) h[i] = pair_fma(pair_ex2(pair_mul(rate[i], pair_of(sum, sum))), h[i], left[i]);
+                for (int i = 0; i < PAIRS; ++i) {
+                    const float2 e = pair_get(pair_mul(rate[i], pair_of(third, third)));
+                    const uint64_t root = pair_of(act_ex2(-max_nan(-e.x, -127.0f)), act_ex2(-max_nan(-e.y, -127.0f)));
+                    h[i] = pair_fma(root, pair_mul(root, pair_mul(root, h[i])), left[i]);
+                }
             }
         }
     }

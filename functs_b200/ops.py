@@ -366,7 +366,8 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     Returns (out [B, T, C], states).
     state: float32 [S, C, N], contiguous, read and updated in place; slots, lengths, out and status are as in linear_attention.
     Rates beyond +-2.3e38, infinite ones too, count as that: with A = -inf a step d > 0 leaves nothing of a state, and d = 0 (log(1 + exp(d)) from
-    d = -88 down) all of it.  A token with a NaN or an infinity leaves the outputs before it alone; from it on they are not finite where the formula's are not (an infinity
+    d = -88 down) all of it.  Powers are in fp32: from d A = 88.8 in one token on they are infinite, whatever the state.
+    A token with a NaN or an infinity leaves the outputs before it alone; from it on they are not finite where the formula's are not (an infinity
     of the formula may be a NaN).  No derivatives: inputs that require a gradient or carry a tangent are refused."""
     return _native()._selective_scan(x, dt, A, B, C, D, z, dt_bias, softplus, state, slots, lengths, out, status)
 

@@ -628,3 +628,27 @@ def test_rates_without_bound_and_steps_of_either_sign(ops, t):
     bad = torch.zeros(24, 16, dtype=torch.bool, device="cuda")
     bad[3, 4] = True
     assert torch.equal(torch.isnan(state), bad.expand(2, -1, -1)) and torch.equal(torch.isnan(out), bad.any(1).expand(2, t, -1))
+
+
+def grows(ops, x, dt, A, B, C, D, state):
+    want = recurrence(x, dt, A, B, C, D, None, None, False, state, torch.full((x.size(0),), x.size(1), device="cuda"))
+    out, state = ops.selective_scan(x, dt, A, B, C, D=D, state=state)
+    check(out, want[0], want[1], F32)
+    assert bool(((state.double() - want[2]).abs() <= want[3]).all())
+
+
+def test_states_of_0_while_others_would_grow(ops):
+    """Rates above 0 whose growth over a part of a prompt passes 32 bits: nothing but zeros until late."""
+    t = 4096
+    x, dt, A, B, C, D, _, _ = make(1, t, 24, 16, 1, F32)
+    x[:, :t - 50] = 0.0
+    grows(ops, x, torch.ones_like(dt), torch.ones_like(A), B, C, D, None)
+
+
+@pytest.mark.parametrize("first", [200, 290, 380, 470, 560])
+def test_states_that_grow_over_a_part_of_a_prompt(ops, first):
+    """Growth by e^144 within 72 tokens, of a state that starts small and stays finite."""
+    x, dt, A, B, C, D, _, _ = make(1, 1500, 24, 16, 1, F32)
+    dt = torch.zeros_like(dt)
+    dt[:, first:first + 72] = 2.0
+    grows(ops, x * 1e-28, dt, torch.ones_like(A), B, C, D, torch.full((1, 24, 16), 1e-28, device="cuda"))
