@@ -20,6 +20,8 @@ namespace fb {
 
 constexpr int kBeamMaxBeams = FB_BEAM_MAX_BEAMS, kBeamMaxTop = FB_BEAM_MAX_TOP;
 constexpr int kBeamMergeThreads = 256;
+constexpr int kBeamInParts = 128;  // candidates of a group whose rows are in parts, at most
+static_assert(kBeamMaxBeams <= kBeamMergeThreads - kBeamInParts, "the rows' sums are for the other threads");
 
 enum BeamKind : int32_t { kBeamLive = 0, kBeamFlat = 1, kBeamNan = 2, kBeamEnded = 3 };  // flat: -inf for all
 
@@ -93,6 +95,7 @@ struct BeamShared {
     float score[kBeamMaxBeams], off[kBeamMaxBeams];
     uint8_t again[kBeamMaxBeams];
     double part[kBeamMergeThreads / 32], power[kBeamPowers];
+    uint64_t in_parts[kBeamInParts];  // keys of a group whose rows are in parts
     int any;
 };
 
@@ -128,21 +131,18 @@ __device__ __forceinline__ int beam_above(const double* list, int n, double x, b
     return lo;
 }
 
-// The candidates' scores (a NaN as +inf, which no other has; NaN behind a list's last), and who is at each place: order[place] = candidate.  Lists follow
-// one another by beam and part, and with that, of equal scores, by beam and token.
+// The candidates' scores (a NaN as +inf, which no other has), and who is at each place: order[place] = candidate.  Lists follow one another by beam: of equal
+// scores the lowest beam comes first, and of one beam's the largest logit, then the lowest token, which is a list's own order.  (Next to a score far from 0 logits
+// that differ make the same score.)
 constexpr int kBeamCount = 512;  // candidates whose places are counted one by one: a halving is a chain of loads
 __device__ __forceinline__ void beam_place(const BeamArgs& a, const BeamShared& sh, const uint64_t* keys, double* score, int* order) {
-    const int lists = a.beams * a.parts, count = lists * a.listed;
+    const int count = a.beams * a.listed;
     for (int c = threadIdx.x; c < count; c += kBeamMergeThreads) {
-        const int list = c / a.listed, i = c % a.listed, k = list / a.parts, part = list % a.parts;
+        const int k = c / a.listed, i = c % a.listed;
         const BeamRow& row = sh.row[k];
         double s = -INFINITY;
         if (row.kind == kBeamLive) {
-            const uint64_t key = keys[c];
-            s = static_cast<double>(sh.score[k]) + ((static_cast<double>(lp_value(static_cast<uint32_t>(key >> 32))) - row.base) - row.log_s);
-            if (key == 0) s = NAN;
-        } else if (part > 0) {
-            s = NAN;  // (one list does for a row whose logits do not count)
+            s = static_cast<double>(sh.score[k]) + ((static_cast<double>(lp_value(static_cast<uint32_t>(keys[c] >> 32))) - row.base) - row.log_s);
         } else if (row.kind == kBeamNan) {
             s = INFINITY;
         } else if (row.kind == kBeamEnded && i == 0) {
@@ -160,16 +160,16 @@ __device__ __forceinline__ void beam_place(const BeamArgs& a, const BeamShared& 
                 const double other = score[o];
                 place += other > own || (other == own && o < c);
             }
-            if (own == own) order[place] = c;
+            order[place] = c;
         }
     } else {
         for (int c = threadIdx.x; c < count; c += kBeamMergeThreads) {
             const int list = c / a.listed;
             const double own = score[c];
             int place = c % a.listed;
-            for (int o = 0; o < lists; ++o)
+            for (int o = 0; o < a.beams; ++o)
                 if (o != list) place += beam_above(score + o * a.listed, a.listed, own, o < list);
-            if (own == own) order[place] = c;
+            order[place] = c;
         }
     }
     __syncthreads();
@@ -180,10 +180,10 @@ template <typename T>
 __global__ void __launch_bounds__(kBeamMergeThreads) beam_merge_kernel(const BeamArgs a) {
     extern __shared__ __align__(16) unsigned char beam_smem[];
     __shared__ BeamShared sh;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, lists = a.beams * a.parts, count = lists * a.listed;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, count = a.beams * a.listed;
     const int64_t first = static_cast<int64_t>(blockIdx.x) * a.beams;
     double* score = reinterpret_cast<double*>(beam_smem);
-    uint64_t* keys = reinterpret_cast<uint64_t*>(score + count);
+    uint64_t* keys = reinterpret_cast<uint64_t*>(score + count);  // of every row, best first
     int* order = reinterpret_cast<int*>(keys + count);
     int kind = kBeamLive;
     if (tid < a.beams) {
@@ -192,9 +192,21 @@ __global__ void __launch_bounds__(kBeamMergeThreads) beam_merge_kernel(const Bea
         sh.again[tid] = 0;
     }
     if (tid == 0) sh.any = 0;
-    for (int c = tid; c < count; c += kBeamMergeThreads) order[c] = -1;
+    for (int c = tid; c < count; c += kBeamMergeThreads) order[c] = c;  // (a candidate whatever the scores)
     pdl_wait();
-    for (int c = tid; c < count; c += kBeamMergeThreads) keys[c] = a.keys[first * a.parts * a.listed + c];
+    if (a.parts == 1) {
+        for (int c = tid; c < count; c += kBeamMergeThreads) keys[c] = a.keys[first * a.listed + c];
+    } else if (tid >= kBeamMergeThreads - kBeamInParts) {
+        // a row's lists become one, by their keys (upper warps: beside the rows' sums)
+        const int c = tid - (kBeamMergeThreads - kBeamInParts), span = a.parts * a.listed, k = c / span;
+        const bool there = k < a.beams;
+        uint64_t key = 0;
+        if (there) key = sh.in_parts[c] = a.keys[first * span + c];
+        asm volatile("bar.sync 1, %0;" ::"n"(kBeamInParts) : "memory");
+        int place = 0;
+        for (int o = k * span; there && o < (k + 1) * span; ++o) place += sh.in_parts[o] > key;
+        if (there && place < a.listed) keys[k * a.listed + place] = key;
+    }
     if (tid < a.beams) {
         BeamRow row = {0.0, 0.0, kind};
         float off = 0.0f;
@@ -232,8 +244,8 @@ __global__ void __launch_bounds__(kBeamMergeThreads) beam_merge_kernel(const Bea
     // neighbours that may be the wrong way round; behind the last place as long as they lie as near
     const auto check = [&](int p) {
         const int c = order[p], d = order[p + 1];
-        if (c < 0 || d < 0 || !(score[c] < INFINITY && score[d] > -INFINITY && score[c] - score[d] <= near)) return false;
-        const int k = c / (a.listed * a.parts), o = d / (a.listed * a.parts);
+        if (!(score[c] < INFINITY && score[d] > -INFINITY && score[c] - score[d] <= near)) return false;
+        const int k = c / a.listed, o = d / a.listed;
         if (k != o) sh.again[k] = sh.again[o] = 1, sh.any = 1;
         return true;
     };
@@ -276,7 +288,7 @@ __global__ void __launch_bounds__(kBeamMergeThreads) beam_merge_kernel(const Bea
         beam_place(a, sh, keys, score, order);
     }
     for (int p = tid; p < a.top; p += kBeamMergeThreads) {
-        const int c = order[p], k = c / (a.listed * a.parts), i = c % a.listed;
+        const int c = order[p], k = c / a.listed, i = c % a.listed;
         const int settled = sh.row[k].kind;
         int64_t token = i;
         if (settled == kBeamLive) token = static_cast<int64_t>(0xFFFFFFFFu - static_cast<uint32_t>(keys[c]));
@@ -303,7 +315,7 @@ static int launch_beam(BeamArgs& a, int groups, cudaStream_t st) {
     // parts cost (8 rows of 131072 in bf16 with 16 candidates: 64 lists 96 us, 32 24, 8 22)
     const int most = beam_most_parts(groups, a.beams);
     a.parts = 1;
-    while (a.parts < most && vecs / (a.parts * 2) >= 2048 && a.beams * a.parts * 2 * a.listed <= 128) a.parts *= 2;
+    while (a.parts < most && vecs / (a.parts * 2) >= 2048 && a.beams * a.parts * 2 * a.listed <= kBeamInParts) a.parts *= 2;
     a.left = reinterpret_cast<BeamPart*>(a.keys);
     a.keys = reinterpret_cast<uint64_t*>(a.left + rows * a.parts);
     // 512 threads a block are three blocks an SM.  384 are four: long rows in one wave instead of two (512 rows of 131072 in bf16 47 us and 56, of 50001
@@ -312,7 +324,7 @@ static int launch_beam(BeamArgs& a, int groups, cudaStream_t st) {
     const bool wave = rows * a.parts > 3 * kNumSMs && rows * a.parts <= 4 * kNumSMs && each >= 6144;
     const int threads = wave ? 384 : each >= 1024 ? 512 : each >= 512 ? 256 : 128;
     FB_TRY(launch_after(beam_rows_kernel<T>, dim3(static_cast<unsigned>(rows * a.parts)), dim3(threads), 0, st, false, "beam_select", a));
-    const size_t smem = static_cast<size_t>(a.beams) * a.parts * a.listed * (sizeof(double) + sizeof(uint64_t) + sizeof(int));
+    const size_t smem = static_cast<size_t>(a.beams) * a.listed * (sizeof(double) + sizeof(uint64_t) + sizeof(int));
     if (smem > 40 * 1024)
         FB_TRY(check_cuda(cudaFuncSetAttribute(beam_merge_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)), "beam_select"));
     return launch_after(beam_merge_kernel<T>, dim3(groups), dim3(kBeamMergeThreads), smem, st, true, "beam_select", a);

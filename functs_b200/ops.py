@@ -391,8 +391,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, top: Optional[int] =
 
     Beam k followed by token v has the score scores[k] + log_softmax(logits[k])[v].  A beam that has ended (`ended`, bool [G, K]) stays as it
     is: its one continuation is end_token at the beam's own score, the others have -inf.  top: K where it is not given, up to 64; K up to 64.
-    The order is that of the scores in 64 bits (they are rounded on the way out); of equal ones the lowest (parent, token) comes first, -inf
-    last: a row of logits that leaves nothing and a beam whose score is -inf have nothing else.  A row with a NaN or +inf, and
+    The order is that of the scores in 64 bits (they are rounded on the way out); of equal ones the lowest parent comes first, and of one
+    parent's the largest logit (a score far from 0 may leave no difference), then the lowest token.  -inf comes last: a row of logits that leaves nothing and a beam whose score is -inf have nothing else.  A row with a NaN or +inf, and
     one whose score is NaN or +inf, has NaN for all, and NaN comes first."""
     return _native()._beam_select(logits, scores, top, ended, end_token)
 

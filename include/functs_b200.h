@@ -338,8 +338,8 @@ int functs_b200_selective_scan(const functs_b200_selective_scan_args* args, void
  *   scores[g][k] + x[v] - log sum_i exp(x[i]),  x = logits[g][k]   (a row of nothing but -inf: -inf)
  * and of a beam that has ended (ended[g][k] != 0; optional) its end token the beam's own score, all others -inf; its logits are not read,
  * nor are those of a beam whose score is -inf, all of whose candidates have that score.  A row with a NaN or +inf, and one whose beam's
- * score is NaN or +inf, has NaN for all its candidates, and NaN comes first.  Of equal scores the lowest (k, v) comes first.  The order is that
- * of the scores in 64 bits, before they are rounded to fp32.
+ * score is NaN or +inf, has NaN for all its candidates, and NaN comes first.  The order is that of the scores in 64 bits, before they are
+ * rounded to fp32.  Of equal ones the lowest k comes first, and of one beam's the largest x[v], then the lowest v.
  * logits [groups, beams, vocab]: elements of `dtype`, those of a row adjacent, strides in elements; beams <= 64, top <= 64 and <= beams * vocab.
  * out_scores fp32, parents, tokens int64 [groups, top].  scratch: functs_b200_beam_select_scratch_bytes, 16-byte aligned. */
 #define FB_BEAM_MAX_BEAMS 64

@@ -447,3 +447,29 @@ def test_beams_that_are_alike_far_from_0(ops, most, dtype):
     fine = torch.isfinite(want[0])
     assert torch.equal(torch.isfinite(got[0]), fine)
     assert bool(((got[0].double() - want[0]).abs()[fine] <= 2.0 ** -24 * want[0].abs()[fine] + (11 + 32) * 2.0 ** -24).all())
+
+
+def by_logit(logits, scores, top):
+    """Of candidates with equal scores in 64 bits: the lowest beam first, and of one beam the largest logit, then the lowest token."""
+    total = torch.log_softmax(logits.double(), dim=2) + scores.double()[..., None]
+    tokens = torch.sort(logits.double(), dim=2, descending=True, stable=True)[1]
+    score, place = torch.sort(total.gather(2, tokens).flatten(1), dim=1, descending=True, stable=True)
+    v = logits.size(2)
+    return score[:, :top], place[:, :top] // v, tokens.flatten(1).gather(1, place[:, :top])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("shape", [(1, 1, 140003, 8), (1, 4, 140003, 8), (2, 8, 70001, 6), (3, 5, 3001, 40), (1, 64, 300, 64)], ids=str)
+def test_beams_whose_score_leaves_no_room_for_their_logits(ops, shape, dtype):
+    """A beam's score so far from 0 that logits which differ make the same score in 64 bits: the order of a beam is that of its logits, whether its row is one
+    part or several."""
+    g, k, v, top = shape
+    logits, _, _ = inputs(g, k, v, dtype, 21)
+    for low in (torch.finfo(F32).min, -1e30):
+        scores = torch.full((g, k), low, device="cuda")
+        got, want = ops.beam_select(logits, scores, top=top), by_logit(logits, scores, top)
+        assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2]) and torch.equal(got[0], want[0].float())
+        if k > 1:
+            scores[:, 1] = -2.0  # (one that goes on: its own come first)
+            got, want = ops.beam_select(logits, scores, top=top), by_logit(logits, scores, top)
+            assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
