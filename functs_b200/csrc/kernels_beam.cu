@@ -241,10 +241,10 @@ __global__ void __launch_bounds__(kBeamMergeThreads) beam_merge_kernel(const Bea
     float off = 0.0f;
     for (int k = 0; k < a.beams; ++k) off = fmaxf(off, sh.off[k]);
     const double near = 2.0 * static_cast<double>(off);
-    // neighbours that may be the wrong way round; behind the last place as long as they lie as near
+    // neighbours that may be the wrong way round; behind the last place as long as they lie as near (or where a score's own rounding may part or join them)
     const auto check = [&](int p) {
         const int c = order[p], d = order[p + 1];
-        if (!(score[c] < INFINITY && score[d] > -INFINITY && score[c] - score[d] <= near)) return false;
+        if (!(score[c] < INFINITY && score[d] > -INFINITY && score[c] - score[d] <= near + (fabs(score[c]) + fabs(score[d])) * 0x1p-52)) return false;
         const int k = c / a.listed, o = d / a.listed;
         if (k != o) sh.again[k] = sh.again[o] = 1, sh.any = 1;
         return true;

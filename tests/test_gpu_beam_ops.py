@@ -473,3 +473,20 @@ def test_beams_whose_score_leaves_no_room_for_their_logits(ops, shape, dtype):
             scores[:, 1] = -2.0  # (one that goes on: its own come first)
             got, want = ops.beam_select(logits, scores, top=top), by_logit(logits, scores, top)
             assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+
+
+def test_scores_on_either_side_of_a_rounding_in_64_bits(ops):
+    """Beams at -2^40, where a score in 64 bits is a multiple of 2^-12: one beam's lies next to the border of two such numbers, nearer than a pass over its
+    logits knows it, the other's is the upper of them.  Equal they are (the lower beam first), or one is below."""
+    n = torch.arange(300, 300 + 512 * 4, 4, dtype=torch.float64)
+    x = torch.log(torch.expm1((n + 0.5) / 4096)).float()          # -log(1 + exp(x)) = -(n + 1/2) / 4096
+    x = torch.cat([x, torch.nextafter(x, x.new_tensor(9.0)), torch.nextafter(x, x.new_tensor(-9.0))])
+    logits = torch.full((x.numel(), 2, 64), -math.inf)
+    logits[:, :, 3] = 0.0
+    logits[:, 0, 60] = x
+    logits[:, 1, 60] = torch.log(torch.expm1(n / 4096)).float().repeat(3)
+    logits, scores = logits.cuda(), torch.full((x.numel(), 2), -2.0 ** 40, device="cuda")
+    want = select_reference(logits, scores, 2)
+    assert 0 < int((want[1][:, 0] == 1).sum()) < x.numel() and bool((want[2] == 3).all())  # (some of each)
+    got = ops.beam_select(logits, scores)
+    assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
