@@ -403,7 +403,8 @@ def beam_reorder(states: List[torch.Tensor], parents: torch.Tensor, slots: torch
     slot, every other gets the slot of a beam that has no child (both in ascending order), and the rows of all pools are copied there, in place.
 
     So no state moves that has one child.  A group whose first slot is negative is none: its slots come back as they are.  So do those of a group with
-    a parent or a slot out of range, or with a slot that stands earlier in the table; `status` gets the bit that raise_on_status reports."""
+    a parent or a slot out of range, or with a slot that stands earlier in the table; `status` gets the bit that raise_on_status reports.  K is up to
+    64, G * K up to 2^20 (every slot is compared with all before it)."""
     return _native()._beam_reorder(states, parents, slots, status)
 
 

@@ -354,7 +354,8 @@ int functs_b200_beam_select(const void* logits, int32_t dtype, int64_t group_str
  * other gets the slot of a beam that has no child (both in ascending order), and the rows of all pools are copied there.
  * A group whose first slot is negative is none: its row of new_slots is that of slots.  So is, with a status bit (optional), a group with a
  * parent outside [0, beams) or a slot outside [0, num_slots) (FB_STATUS_INDEX_RANGE), or with a slot that stands earlier in the table
- * (FB_STATUS_INDEX_TWICE).  pools (HOST memory): `count` of them, rows of row_bytes one after another.  beams <= 64.  One launch for every 32 pools. */
+ * (FB_STATUS_INDEX_TWICE).  pools (HOST memory): `count` of them, rows of row_bytes one after another.  beams <= 64, groups * beams <=
+ * 2^20 (every slot is compared with all before it).  One launch for every 32 pools. */
 typedef struct {
     void* data;
     int64_t row_bytes;

@@ -132,3 +132,10 @@ def test_there_is_no_cpu_path():
         ops.beam_select(x, torch.zeros(2, 3))
     with pytest.raises(ValueError, match="CUDA"):
         ops.beam_reorder([x], torch.zeros(1, 2, dtype=torch.int64), torch.zeros(1, 2, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("groups,beams", [((1 << 14) + 1, 64), ((1 << 20) // 3 + 1, 3), (1 << 20, 2)])
+def test_beam_reorder_of_too_many_beams(groups, beams):
+    """Every slot is compared with all that stand before it: a table has 2^20 beams at most."""
+    rc, why = reorder(groups=groups, beams=beams)
+    assert rc == -1 and "too large" in why
