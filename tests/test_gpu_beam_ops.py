@@ -490,3 +490,30 @@ def test_scores_on_either_side_of_a_rounding_in_64_bits(ops):
     assert 0 < int((want[1][:, 0] == 1).sum()) < x.numel() and bool((want[2] == 3).all())  # (some of each)
     got = ops.beam_select(logits, scores)
     assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("shape", [(1, 4, 140003, 8), (1, 8, 140003, 4), (2, 8, 70001, 8), (4, 4, 131072, 16), (1, 2, 66000, 32), (3, 5, 40000, 12)], ids=str)
+def test_beams_of_long_rows_in_parts(ops, shape, dtype):
+    """Few candidates of few long rows, which are cut into parts: masked rows, flat ones, one whose parts but the last are empty, beams that end, rows that are
+    not finite in one part, and beams that lie next to one another."""
+    g, k, v, top = shape
+    for masked in (False, True):
+        logits, scores, flags = inputs(g, k, v, dtype, 31, masked=masked)
+        check_select(ops.beam_select(logits, scores, top=top, ended=flags, end_token=v - 1), select_reference(logits, scores, top, flags, v - 1), v)
+    logits[:, 0] = -math.inf
+    logits[:, 0, v - 5:] = 1.5
+    logits[:, k - 1, 70:] = -math.inf
+    check_select(ops.beam_select(logits, scores, top=top), select_reference(logits, scores, top), v)
+    logits[0, k // 2, v - 2] = math.inf
+    logits[g - 1, 0, v // 2] = math.nan
+    check_select(ops.beam_select(logits, scores, top=top), select_reference(logits, scores, top), v)
+    flat = torch.zeros(g, k, v, device="cuda", dtype=dtype)
+    scores[:] = -1.0
+    check_select(ops.beam_select(flat, scores, top=top), select_reference(flat, scores, top), v)
+    logits, _, _ = inputs(g, k, v, dtype, 32)
+    lse = torch.logsumexp(logits.double(), dim=2)
+    scores = (-20.0 - (logits.double().amax(dim=2) - lse)).float()
+    want = select_reference(logits, scores, top)
+    assert bool((want[0][:, 0] - want[0][:, 1] < 4e-6).all())  # (near indeed)
+    check_select(ops.beam_select(logits, scores, top=top), want, v)
