@@ -158,6 +158,23 @@ def test_step(ops, shape, dtype):
     assert torch.equal(pool[others], before[others])
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_step_whose_terms_cancel(ops, dtype):
+    """States of one number that a token all but takes away: what 32 bits lose is relative to the terms (four roundings: the decay's two, the product, the sum),
+    not to what is left of them."""
+    b = 4096
+    q, k, v = (x[:, 0] for x in make(b, 1, 1, 1, 1, 1, dtype, "fused"))
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    near = 1 + torch.randn(b, generator=gen, device="cuda") * 0.05
+    start = (-(k.double() * v.double()).flatten() / math.exp(float(decays(1)[0])) * near).float().view(b, 1, 1, 1)
+    out, state, mag, m = recurrence(q[:, None], k[:, None], v[:, None], decays(1), 0.5, start, torch.ones(b, device="cuda"))
+    assert float((state.abs() < 0.05 * m).double().mean()) > 0.9  # (they do)
+    got = ops.linear_attention_step(q, k, v, decays(1), start, scale=0.5)
+    assert bool(((start.double() - state).abs() <= 4 * 2.0 ** -24 * m).all())
+    half = 0.0 if dtype == F32 else torch.finfo(dtype).eps / 2
+    assert bool(((got[:, None].double() - out).abs() <= half * out.abs() + 6 * 2.0 ** -24 * mag + (torch.finfo(dtype).tiny if dtype != F32 else 0.0)).all())
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("shape", [(73, 1, 1, 128, 128), (74, 1, 1, 128, 128), (1, 1, 1, 128, 32), (1, 2, 1, 128, 36), (3, 2, 2, 33, 124), (2, 3, 1, 3, 4),
                                    (5, 2, 2, 64, 64), (5, 2, 2, 65, 64), (40, 2, 1, 128, 127), (74, 1, 1, 127, 65), (5, 2, 2, 65, 39), (7, 3, 1, 128, 31),
