@@ -1,18 +1,19 @@
 // Beam search: the best continuations of every group of beams, and the states of the beams that go on.
 //
 // Selection.  score(k, v) = scores[k] + x_k[v] - log sum exp x_k.  Within a beam the order is that of its logits, so only the `top` best of each row
-// can be among the group's: one pass over a row gives its sum and those (as token_logprobs has it; few long rows are cut into parts, whose
-// lists are lists like the others), then a block per group joins the sums and merges the lists: a candidate's place is the number of better ones.
+// can be among the group's: one pass over a row gives its sum and those (as token_logprobs has it; few long rows are cut into parts), then a block per
+// group joins the parts' sums and lists and merges the rows' lists: a candidate's place is the number of better ones.
 //
 // The order is that of the scores in 64 bits.  A row's logarithm out of the pass is off by some 2^-19 at most (5e-8 as measured), the same for all of
 // its candidates, so only neighbours from different rows that lie nearer to one another than that can be the wrong way round.  Where there are any
 // among the best (one call of 64 groups of 8 in ten), the rows in question are summed again in 64 bits by the group's block, and the lists
 // merged again: 14 us more for every row of 50001, bound by the block's SM, which does some 16 products in 64 bits a cycle (with the library's
-// exponentials, four at a time, 25).  Tried for that: a cluster of eight blocks a group that shares the rows, 14 us instead of 50 for two of them, but 3.5 us
+// exponentials, four at a time, 25); 8 beams that are alike 129 us, 64 of 32000 in fp32 1450.  Tried for that: a cluster of eight blocks a group that shares the rows, 14 us instead of 50 for two of them, but 3.5 us
 // more for every call of many groups.
 //
-// Two launches, 10 us for 4 rows of 32000 in fp32 (7 the pass and the choice, whose block barriers are the latency, 3 the merging); 64 groups of 8 rows of
-// 50001 in bf16 25.5 us, 2.0 TB/s: a row's choice follows its pass, and 512 blocks are one wave and a part.  Tried: rows of a group as a cluster
+// Two launches, 9.5 us for 4 rows of 32000 in fp32 (7 the pass and the choice, whose block barriers are the latency, the rest the merging); 64 groups of 8 rows of
+// 50001 in bf16 24 us, 2.1 TB/s (27 with a few near neighbours): a row's choice follows its pass, which a block loads nothing behind.  In 16 bits the rows' kernel spills 24 to 28
+// bytes of 40 registers.  64 beams with 64 candidates 440 us: places by halving, a chain of loads.  Tried, when those were 10 and 25.5: rows of a group as a cluster
 // that merges in its first block's shared memory 10.5 and 32.7 (all blocks stay until the slowest has finished), 256 threads a row 14 and 28.
 #include "logprobs.cuh"
 
@@ -311,8 +312,9 @@ template <typename T>
 static int launch_beam(BeamArgs& a, int groups, cudaStream_t st) {
     const int64_t rows = static_cast<int64_t>(groups) * a.beams;
     const int vecs = a.vocab / LpVec<T>::N;
-    // a part has 2048 vectors at least (one row of 32000 in fp32 and one of 65536 in 16 bits are two), and a group 128 candidates at most: merging them is what
-    // parts cost (8 rows of 131072 in bf16 with 16 candidates: 64 lists 96 us, 32 24, 8 22)
+    // a part has 2048 vectors at least (one row of 32000 in fp32 is two, one of 65536 in 16 bits four), and a group 128 candidates at most: merging them is what
+    // parts cost (8 rows of 131072 in bf16 with 16 candidates, when every part's list was merged by scores: 64 lists 96 us, 32 24, 8 22; with 8 candidates, two parts
+    // a row, 12.9)
     const int most = beam_most_parts(groups, a.beams);
     a.parts = 1;
     while (a.parts < most && vecs / (a.parts * 2) >= 2048 && a.beams * a.parts * 2 * a.listed <= kBeamInParts) a.parts *= 2;

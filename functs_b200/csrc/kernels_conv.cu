@@ -3,8 +3,9 @@
 // A pass over the rows: every input is read once and every output written once, but for the W - 1 rows in front of a thread's tokens, which it
 // reads again (from L2).  A thread has V adjacent channels (of 16 or 8 bytes where the rows lie on such boundaries) and a run of tokens, whose last W - 1
 // inputs it keeps in registers; sums are in fp32, in the order of the formula, two channels an instruction.  Bound by HBM beside two exponential-unit
-// results an element (30 us of 8 x 2048 tokens of 4096 channels in bf16, which take 55 in all: 4.9 TB/s; by single products 83, with eight
-// channels a thread 60, four tokens ahead 61, at four blocks an SM instead of five 59).  192 single tokens of 4096 channels 4.5 us (9.3 by the prompts' kernel).
+// results an element (30 us of 8 x 2048 tokens of 4096 channels in bf16, which take 56 in all: 4.8 TB/s; by single products 83, with eight
+// channels a thread 60, four tokens ahead 61, at four blocks an SM instead of five 59: five leave 96 registers a thread, and at width 4 36 bytes are spilled).  In fp32
+// half as many tokens take 46 us, 5.8 TB/s; 4095 channels, whose rows no vector fits, 106.  192 single tokens of 4096 channels 4.5 us (9.3 by the prompts' kernel).
 #include <type_traits>
 
 #include "activation.cuh"

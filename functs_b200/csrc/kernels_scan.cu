@@ -8,9 +8,9 @@
 //
 // What a token costs a warp of 16 channels of 16 states: eight exponentials (64 cycles of a scheduler), 16 products by pairs (34 cycles), eight loads from
 // shared memory and shuffles, and some 35 instructions to prepare and finish it, 70 in all.  Exponentials are 16 per cycle and SM, and 19 a channel with the step's
-// and the gate's, which bounds 8 x 1024 tokens of 4096 channels at 141 us.  They take 225: a warp's instructions wait for one another, and there are
-// only 3.5 warps for a scheduler (issue 58 %, exponentials 60 %, shared memory 44 %).  Without the exponentials 208, without loads of B and C 236,
-// without shuffles 203, without copies ahead 211: nothing by itself.  DRAM would take 42.
+// and the gate's, which bounds 8 x 1024 tokens of 4096 channels at 141 us.  They take 232: a warp's instructions wait for one another, and there are
+// only 3.5 warps for a scheduler (issue 57 %, exponentials 55 %, shared memory 58 %).  With one thing left out at a time, all of one build: without the exponentials 218,
+// without loads of B and C 221, without shuffles 205; with tiles copied when they are needed, not ahead, 333.  DRAM would take 42.
 //
 // Few channels and many tokens: sequences are cut into parts.  One launch goes through all parts but the last from a state of zero and leaves what each
 // adds and the sum of its steps; in the second every part makes its start of what the parts before it left, h = exp(A sum d) h + end, and forms the outputs.
@@ -403,10 +403,12 @@ __global__ void __launch_bounds__(32 * kScanWarps, 3) scan_kernel(const ScanArgs
 
 // One token per sequence: a pass over the states, LANES lanes a channel, eight states a lane.  A CTA goes through `each` sequences with the same
 // channels, so that their rates are read once and addresses only move on.
-// Bound by the states' traffic and its latency: 192 sequences of 4096 channels of 16 states 30 us from HBM (3.6 TB/s; 24.5 where the states are in L2).  What
+// Bound by the states' traffic and its latency (of the 13 cycles between a warp's instructions 6.5 are waits for a load): 192 sequences of 4096 channels of 16 states 31 us
+// from HBM (3.5 TB/s; 24.5 where the states are in L2), 35 with fp32 inputs, whose registers spill (52 bytes of 64 registers).  What
 // is on its way at once are the warps' loads, so more warps are worth more than a warp's loads ahead: two sequences ahead in five CTAs an SM 33, three in
 // four 36, four through shared memory by asynchronous copies 30; the next piece of four states beside its neighbour lanes' 32.6; four states a
-// lane, with addresses worked out anew for every sequence (260 instructions for 16 bytes of each lane), 40.
+// lane, with addresses worked out anew for every sequence (260 instructions for 16 bytes of each lane), 40.  (With the depth of 1 written out, not as kStepAhead, the
+// loop comes out otherwise: that call 29 us, 300 sequences of 1536 channels 18.1 for 16.9, 512 of 1024 20.7 for 19.9.)
 constexpr int kStepThreads = 128, kStepMostEach = 32, kStepAhead = 1, kStepCtas = 8, kStepPer = 8;
 template <typename T, int LANES>
 __global__ void __launch_bounds__(kStepThreads, kStepCtas) scan_step_kernel(const ScanArgs a, const ScanPlan plan, int each) {
